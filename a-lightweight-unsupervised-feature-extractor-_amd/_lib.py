@@ -16,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("TRK_LIB_PATH") or os.path.join(_HERE, "libtrk_amd.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "trk_amd.h")
 
-TRK_F32, TRK_BF16, TRK_F64 = 0, 1, 2
+TRK_F32, TRK_BF16, TRK_F64, TRK_F16, TRK_E4M3 = 0, 1, 2, 3, 4
 TRK_NCHW, TRK_NHWC = 0, 1
 TRK_LSAP_MAX_DIM = 2048
 TRK_ENC_PARTS = 3  # per-ROI partial sums of the encoder GEMMs (trk_amd.h)

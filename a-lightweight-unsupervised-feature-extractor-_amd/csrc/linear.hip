@@ -1,0 +1,546 @@
+// Matrix products of rows and weights: 8-bit codes with an f32 scale for each block of 128
+// columns, and rows sorted by group (a stream, an expert) with one weight for each group, in
+// 8 or 16 bits, with the 16-bit form's two gradients.
+//
+//   8 bits:  y[m][n] = sum_kb sx[m][kb] sw[n][kb] (sum of the block's 128 products x w) + bias[n]
+//   grouped: the counts[0] first rows by w[0], the counts[1] next by w[1], ..
+//   gradients: dx = dy w[g] (row by row),  dw[g] = sum over the group's rows of dy^T x
+//
+// The product runs transposed on the matrix cores: w rows are the A operand and x rows the B
+// operand, so a lane ends up with four consecutive columns of one row of y (one 8-byte store)
+// and needs one row scale per tile.  A K step is 128 bytes of every row (one 16x16x128 e4m3 or
+// two 16x16x32 16-bit matrix instructions a tile).  Which k a lane's bytes hold does not matter
+// as long as both operands agree: a lane of group g = lane / 16 takes the 16-byte chunks g and
+// g + 4 of its row.
+#include "trk_common.h"
+
+using namespace trk;
+
+namespace {
+
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef int i8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+
+constexpr int kStep = 128;  // bytes of K a step
+constexpr int kBK = 128;    // columns that share a scale
+
+struct MmArgs {
+  const uint8_t *x, *w;      // rows; strides below in bytes
+  const float *sx, *sw, *bias;
+  void* y;
+  const int32_t* counts;     // grouped: rows of each group (null: one group of M rows)
+  int64_t ldx, ldw, wg;      // wg: bytes from a group's weight to the next
+  int64_t sx_row, sx_kb, sw_row, sw_kb, sw_g;
+  int64_t ldy;               // elements
+  int64_t M, N, K, G;        // K in elements
+  int zero_tail;             // rows behind the last group are written as zeros
+};
+
+// ------------------------------------------------------------------ which rows a tile has
+struct Tile {
+  int64_t row0;
+  int rows;   // rows of the tile; 0: none
+  int g;      // group, or -1: rows behind the last group
+};
+
+// The rows of tile `t` (TM rows each, a group's last one shorter), found by all BT threads from
+// the counts: each thread sums a run of groups, the sums are scanned, the thread whose run
+// holds tile t walks it.  Negative counts are 0 and the sum stops at M, so no count reaches
+// past the rows.
+template <int TM, int BT>
+__device__ Tile find_tile(const MmArgs& A, int64_t t, int64_t (*scan)[2], Tile* found) {
+  const int tid = threadIdx.x;
+  const int64_t run = (A.G + BT - 1) / BT, g0 = tid * run, g1 = min(A.G, g0 + run);
+  if (tid == 0) *found = Tile{0, 0, 0};
+  int64_t rows = 0;
+  for (int64_t g = g0; g < g1; ++g) rows += max(0, A.counts[g]);
+  // exclusive scan of the rows over the threads
+  const int lane = tid & 63, wave = tid >> 6;
+  int64_t incl = rows;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 63) scan[wave][0] = incl;
+  __syncthreads();
+  int64_t first = incl - rows, total = 0;
+  for (int w = 0; w < BT / 64; ++w) {
+    if (w < wave) first += scan[w][0];
+    total += scan[w][0];
+  }
+  // tiles of this thread's groups, with the rows cut at M
+  int64_t tiles = 0, at = min(first, A.M);
+  for (int64_t g = g0; g < g1; ++g) {
+    const int64_t c = min((int64_t)max(0, A.counts[g]), A.M - at);
+    tiles += (c + TM - 1) / TM;
+    at += c;
+  }
+  incl = tiles;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 63) scan[wave][1] = incl;
+  __syncthreads();
+  int64_t t0 = incl - tiles, all = 0;
+  for (int w = 0; w < BT / 64; ++w) {
+    if (w < wave) t0 += scan[w][1];
+    all += scan[w][1];
+  }
+  if (t >= t0 && t < t0 + tiles) {
+    at = min(first, A.M);
+    int64_t k = t0;
+    for (int64_t g = g0; g < g1; ++g) {
+      const int64_t c = min((int64_t)max(0, A.counts[g]), A.M - at);
+      const int64_t n = (c + TM - 1) / TM;
+      if (t < k + n) {
+        const int64_t o = (t - k) * TM;
+        *found = Tile{at + o, (int)min((int64_t)TM, c - o), (int)g};
+        break;
+      }
+      k += n;
+      at += c;
+    }
+  }
+  if (tid == 0 && t >= all && A.zero_tail) {
+    const int64_t end = min(total, A.M), o = end + (t - all) * TM;
+    if (o < A.M) *found = Tile{o, (int)min((int64_t)TM, A.M - o), -1};
+  }
+  __syncthreads();
+  return *found;
+}
+
+// ------------------------------------------------------------------ stores of four columns
+__device__ __forceinline__ void put(void* y, int dt, int64_t at, float v) {
+  if (dt == TRK_F32) ((float*)y)[at] = v;
+  else if (dt == TRK_BF16) ((uint16_t*)y)[at] = f32_to_bf16(v);
+  else ((_Float16*)y)[at] = (_Float16)v;
+}
+
+// y[at .. at + 3] (`left` of them exist); gfx950 takes the wide store at any alignment
+__device__ __forceinline__ void put4(void* y, int dt, int64_t at, int64_t left, f4v v) {
+  if (left >= 4) {
+    if (dt == TRK_F32) {
+      __builtin_memcpy((float*)y + at, &v, 16);
+    } else {
+      uint2 p;
+      if (dt == TRK_BF16) {
+        p = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+      } else {
+        p = make_uint2(__builtin_bit_cast(uint32_t, h2v{(_Float16)v[0], (_Float16)v[1]}),
+                       __builtin_bit_cast(uint32_t, h2v{(_Float16)v[2], (_Float16)v[3]}));
+      }
+      __builtin_memcpy((uint16_t*)y + at, &p, 8);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) put(y, dt, at + j, v[j]);
+  }
+}
+
+// ------------------------------------------------------------------ one K step of one tile
+enum { IN_E4M3 = 0, IN_BF16 = 1, IN_F16 = 2, IN_E4M3X = 3 };
+
+constexpr bool is8(int in) { return in == IN_E4M3 || in == IN_E4M3X; }
+
+// A lane's 32 bytes of a row's K step, as the matrix instruction takes them.  IN_E4M3 is the 8-bit
+// instruction: it cuts each product at 2^-13 of the largest of its chunk's 16 (measured: 1.5e-5 of
+// the sum in the root mean square), far below half a step of a 16-bit y, so 16-bit outputs use
+// it.  IN_E4M3X, for f32 outputs, widens the codes to bf16 (exact) and multiplies at half the rate
+// with f32 sums.
+template <int IN> struct Frag {
+  uint4 v[2];
+  __device__ __forceinline__ void set(uint4 a, uint4 b) { v[0] = a; v[1] = b; }
+};
+template <> struct Frag<IN_E4M3X> {
+  b8v v[4];
+  __device__ __forceinline__ void set(uint4 a, uint4 b) {
+    const uint32_t t[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      typedef __bf16 b2v __attribute__((ext_vector_type(2)));
+      const b2v p0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(t[2 * q], 1.0f, false);
+      const b2v p1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(t[2 * q], 1.0f, true);
+      const b2v p2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(t[2 * q + 1], 1.0f, false);
+      const b2v p3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(t[2 * q + 1], 1.0f, true);
+      v[q] = b8v{p0[0], p0[1], p1[0], p1[1], p2[0], p2[1], p3[0], p3[1]};
+    }
+  }
+};
+
+template <int IN>
+__device__ __forceinline__ f4v mma(const Frag<IN>& a, const Frag<IN>& b, f4v c) {
+  if constexpr (IN == IN_E4M3) {
+    const i8v x = {(int)a.v[0].x, (int)a.v[0].y, (int)a.v[0].z, (int)a.v[0].w,
+                   (int)a.v[1].x, (int)a.v[1].y, (int)a.v[1].z, (int)a.v[1].w};
+    const i8v y = {(int)b.v[0].x, (int)b.v[0].y, (int)b.v[0].z, (int)b.v[0].w,
+                   (int)b.v[1].x, (int)b.v[1].y, (int)b.v[1].z, (int)b.v[1].w};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+  } else if constexpr (IN == IN_E4M3X) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[q], b.v[q], c, 0, 0, 0);
+    return c;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      if constexpr (IN == IN_BF16)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a.v[q]), __builtin_bit_cast(b8v, b.v[q]), c,
+                                                    0, 0, 0);
+      else
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a.v[q]), __builtin_bit_cast(h8v, b.v[q]), c,
+                                                   0, 0, 0);
+    }
+    return c;
+  }
+}
+
+// LDS tile of rows of 128 bytes; a row's 16-byte chunks are rotated by XOR with the row so that
+// eight rows' reads of one chunk fall into different banks
+__device__ __forceinline__ int lds_at(int row, int chunk) { return row * kStep + ((chunk ^ (row & 7)) << 4); }
+
+template <int IN>
+__device__ __forceinline__ Frag<IN> frag(const uint8_t* tile, int row, int lg) {
+  Frag<IN> f;
+  f.set(*(const uint4*)(tile + lds_at(row, lg)), *(const uint4*)(tile + lds_at(row, lg + 4)));
+  return f;
+}
+
+// 16 bytes of a row from byte k on, of which `left` exist (the rest 0)
+__device__ __forceinline__ uint4 load16(const uint8_t* p, int64_t left) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (left >= 16) {
+    __builtin_memcpy(&v, p, 16);
+  } else if (left > 0) {
+    uint8_t t[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t[j] = j < left ? p[j] : 0;
+    __builtin_memcpy(&v, t, 16);
+  }
+  return v;
+}
+
+// 128 x 128 tile, 4 waves of 64 x 64.  Rows of the tile past their end are read from the last
+// row and never stored; columns of w likewise.
+template <int IN, bool WROW>
+__global__ __launch_bounds__(256) void mm_kernel(MmArgs A, int dt) {
+  constexpr int TM = 128, TN = 128;
+  __shared__ uint4 smem[(TM + TN) * kStep / 16];
+  __shared__ int64_t scan[4][2];
+  __shared__ Tile found;
+  uint8_t* xs = (uint8_t*)smem;
+  uint8_t* ws = xs + TM * kStep;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Tile T;
+  if (A.counts) {
+    T = find_tile<TM, 256>(A, blockIdx.y, scan, &found);
+  } else {
+    T.row0 = (int64_t)blockIdx.y * TM;
+    T.rows = (int)min((int64_t)TM, A.M - T.row0);
+    T.g = 0;
+  }
+  if (T.rows <= 0) return;
+  const int64_t n0 = (int64_t)blockIdx.x * TN;
+  const int cols = (int)min((int64_t)TN, A.N - n0);
+  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
+  const int64_t kbytes = T.g < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
+  const int64_t g = max(0, T.g);
+  const uint8_t* xb = A.x + T.row0 * A.ldx;
+  const uint8_t* wb = A.w + g * A.wg + n0 * A.ldw;
+  const float* sw = A.sw + g * A.sw_g;
+  f4v acc[4][4];  // [n tile][m tile]
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = f4v{0, 0, 0, 0};
+  for (int64_t k = 0; k < kbytes; k += kStep) {
+    const int c = tid & 7;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (tid >> 3) + 32 * i;
+      *(uint4*)(xs + lds_at(r, c)) = load16(xb + min(r, T.rows - 1) * A.ldx + k + c * 16, kbytes - k - c * 16);
+      *(uint4*)(ws + lds_at(r, c)) = load16(wb + min(r, cols - 1) * A.ldw + k + c * 16, kbytes - k - c * 16);
+    }
+    __syncthreads();
+    Frag<IN> b[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
+    float s[4];
+    const int64_t kb = k / kBK;  // e4m3: one block of columns a step
+    if constexpr (is8(IN)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j] = A.sx[(T.row0 + min(wm + j * 16 + lr, T.rows - 1)) * A.sx_row + kb * A.sx_kb];
+        if constexpr (!WROW) s[j] *= sw[(n0 / 128) * A.sw_row + kb * A.sw_kb];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const Frag<IN> a = frag<IN>(ws, wn + i * 16 + lr, lg);
+      float wr[4];
+      if constexpr (is8(IN) && WROW) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          wr[e] = sw[(n0 + min(wn + i * 16 + lg * 4 + e, cols - 1)) * A.sw_row + kb * A.sw_kb];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (is8(IN)) {
+          const f4v p = mma<IN>(a, b[j], f4v{0, 0, 0, 0});
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], WROW ? s[j] * wr[e] : s[j], acc[i][j][e]);
+        } else {
+          acc[i][j] = mma<IN>(a, b[j], acc[i][j]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = wn + i * 16 + lg * 4;
+    if (n >= cols) continue;
+    f4v b = {0, 0, 0, 0};
+    if (A.bias && T.g >= 0)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? A.bias[n0 + n + e] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = wm + j * 16 + lr;
+      if (m < T.rows) put4(A.y, dt, (T.row0 + m) * A.ldy + n0 + n, cols - n, acc[i][j] + b);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gradients (16 bits)
+// Both contract over an index that is not contiguous in memory, so their tiles are turned while
+// they are written to LDS: src is [64 k][128 cols] with row stride ld, LDS gets [col][k].
+__device__ __forceinline__ void stage_turned(uint8_t* lds, const uint16_t* src, int64_t ld, int64_t ks, int cols) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int k = (tid >> 4) + 16 * i, c0 = (tid & 15) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (k < ks) v = load16((const uint8_t*)(src + k * ld + c0), 2 * (int64_t)(cols - c0));
+    uint16_t t[8];
+    __builtin_memcpy(t, &v, 16);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *(uint16_t*)(lds + lds_at(c0 + j, k >> 3) + (k & 7) * 2) = t[j];
+  }
+}
+
+struct GradArgs {
+  const uint16_t *dy, *x, *w;
+  void* out;
+  const int32_t* counts;
+  int64_t ldy, ldx, ldw, wg, ldo, og;  // elements
+  int64_t M, N, K, G;
+};
+
+__device__ __forceinline__ void store_tile(const f4v (&acc)[4][4], void* out, int dt, int64_t row0, int rows, int64_t ldo,
+                                           int64_t n0, int cols, int wn, int wm, int lr, int lg) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int n = wn + i * 16 + lg * 4;
+    if (n >= cols) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int m = wm + j * 16 + lr;
+      if (m < rows) put4(out, dt, (row0 + m) * ldo + n0 + n, cols - n, acc[i][j]);
+    }
+  }
+}
+
+template <int IN>
+__device__ __forceinline__ void mm_tile16(const uint8_t* ws, const uint8_t* xs, f4v (&acc)[4][4], int wn, int wm, int lr,
+                                          int lg) {
+  Frag<IN> b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const Frag<IN> a = frag<IN>(ws, wn + i * 16 + lr, lg);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = mma<IN>(a, b[j], acc[i][j]);
+  }
+}
+
+// dx[m][k] = sum_n dy[m][n] w[g][n][k]
+template <int IN>
+__global__ __launch_bounds__(256) void grouped_dx_kernel(GradArgs A, int dt) {
+  constexpr int TM = 128;
+  __shared__ uint4 smem[2 * 128 * kStep / 16];
+  __shared__ int64_t scan[4][2];
+  __shared__ Tile found;
+  uint8_t* xs = (uint8_t*)smem;
+  uint8_t* ws = xs + 128 * kStep;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  MmArgs F{};
+  F.counts = A.counts;
+  F.G = A.G;
+  F.M = A.M;
+  F.zero_tail = 1;
+  const Tile T = find_tile<TM, 256>(F, blockIdx.y, scan, &found);
+  if (T.rows <= 0) return;
+  const int64_t c0 = (int64_t)blockIdx.x * 128;
+  const int cols = (int)min((int64_t)128, A.K - c0);
+  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
+  const uint8_t* xb = (const uint8_t*)(A.dy + T.row0 * A.ldy);
+  const uint16_t* wb = A.w + max(0, T.g) * A.wg + c0;
+  f4v acc[4][4] = {};
+  for (int64_t k = 0; k < (T.g < 0 ? 0 : A.N); k += 64) {
+    __syncthreads();
+    const int c = tid & 7;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (tid >> 3) + 32 * i;
+      *(uint4*)(xs + lds_at(r, c)) =
+          load16(xb + (min(r, T.rows - 1) * A.ldy + k + c * 8) * 2, 2 * (A.N - k - c * 8));
+    }
+    stage_turned(ws, wb + k * A.ldw, A.ldw, A.N - k, cols);
+    __syncthreads();
+    mm_tile16<IN>(ws, xs, acc, wn, wm, lr, lg);
+  }
+  store_tile(acc, A.out, dt, T.row0, T.rows, A.ldo, c0, cols, wn, wm, lr, lg);
+}
+
+// dw[g][n][k] = sum over the rows m of group g of dy[m][n] x[m][k]
+template <int IN>
+__global__ __launch_bounds__(256) void grouped_dw_kernel(GradArgs A, int dt) {
+  __shared__ uint4 smem[2 * 128 * kStep / 16];
+  __shared__ int64_t red[4][2];
+  uint8_t* xs = (uint8_t*)smem;
+  uint8_t* ws = xs + 128 * kStep;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t g = blockIdx.z;
+  int64_t before = 0;
+  for (int64_t i = tid; i < g; i += 256) before += max(0, A.counts[i]);
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
+  if (lane == 0) red[wave][0] = before;
+  __syncthreads();
+  const int64_t row0 = min(A.M, red[0][0] + red[1][0] + red[2][0] + red[3][0]);
+  const int64_t rows = min((int64_t)max(0, A.counts[g]), A.M - row0);
+  const int64_t n0 = (int64_t)blockIdx.y * 128, k0 = (int64_t)blockIdx.x * 128;
+  const int nr = (int)min((int64_t)128, A.N - n0), kc = (int)min((int64_t)128, A.K - k0);
+  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
+  f4v acc[4][4] = {};
+  for (int64_t r = 0; r < rows; r += 64) {
+    __syncthreads();
+    stage_turned(xs, A.dy + (row0 + r) * A.ldy + n0, A.ldy, rows - r, nr);
+    stage_turned(ws, A.x + (row0 + r) * A.ldx + k0, A.ldx, rows - r, kc);
+    __syncthreads();
+    mm_tile16<IN>(ws, xs, acc, wn, wm, lr, lg);
+  }
+  store_tile(acc, (uint16_t*)A.out + g * A.og, dt, n0, nr, A.ldo, k0, kc, wn, wm, lr, lg);
+}
+
+int check_out(const char* what, int dt) {
+  TRK_REQUIRE(dt == TRK_F32 || dt == TRK_BF16 || dt == TRK_F16, "%s: output must be TRK_F32, TRK_BF16 or TRK_F16", what);
+  return TRK_OK;
+}
+
+int check_mm(const char* what, const MmArgs& A, int64_t item, bool scaled) {
+  TRK_REQUIRE(A.M >= 0 && A.N >= 0 && A.K >= 0 && A.M < ((int64_t)1 << 31) && A.N < ((int64_t)1 << 31) &&
+                  A.K < ((int64_t)1 << 31),
+              "%s: bad shape M=%lld N=%lld K=%lld", what, (long long)A.M, (long long)A.N, (long long)A.K);
+  if (A.M == 0 || A.N == 0) return TRK_OK;
+  TRK_REQUIRE(A.y && (A.K == 0 || (A.x && A.w)) && (!scaled || A.K == 0 || (A.sx && A.sw)), "%s: null pointer", what);
+  TRK_REQUIRE(A.ldx >= A.K * item && A.ldw >= A.K * item && A.ldy >= A.N, "%s: row stride below the row's length", what);
+  return TRK_OK;
+}
+
+int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t mtiles, void* stream) {
+  TRK_REQUIRE(mtiles <= 65535, "%s: too many row tiles (%lld)", what, (long long)mtiles);
+  const dim3 grid((unsigned)((A.N + 127) / 128), (unsigned)mtiles);
+  hipStream_t st = (hipStream_t)stream;
+  if (in == IN_E4M3 && dt == TRK_F32 && wrow) mm_kernel<IN_E4M3X, true><<<grid, 256, 0, st>>>(A, dt);
+  else if (in == IN_E4M3 && dt == TRK_F32) mm_kernel<IN_E4M3X, false><<<grid, 256, 0, st>>>(A, dt);
+  else if (in == IN_E4M3 && wrow) mm_kernel<IN_E4M3, true><<<grid, 256, 0, st>>>(A, dt);
+  else if (in == IN_E4M3) mm_kernel<IN_E4M3, false><<<grid, 256, 0, st>>>(A, dt);
+  else if (in == IN_BF16) mm_kernel<IN_BF16, false><<<grid, 256, 0, st>>>(A, dt);
+  else mm_kernel<IN_F16, false><<<grid, 256, 0, st>>>(A, dt);
+  return trk::check_launch(what);
+}
+
+}  // namespace
+
+extern "C" {
+
+int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                   int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_kb, int w_block_rows, const float* bias,
+                   int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, void* stream) {
+  const char* what = "trk_matmul_fp8";
+  if (int rc = check_out(what, out_dtype)) return rc;
+  TRK_REQUIRE(w_block_rows == 1 || w_block_rows == 128, "%s: w_block_rows must be 1 or 128", what);
+  const MmArgs A{(const uint8_t*)x, (const uint8_t*)w, sx, sw, bias, y, nullptr, ldx, ldw, 0, sx_row, sx_kb,
+                 sw_row, sw_kb, 0, ldy, M, N, K, 1, 0};
+  if (int rc = check_mm(what, A, 1, true)) return rc;
+  if (M == 0 || N == 0) return TRK_OK;
+  return launch_mm(what, A, IN_E4M3, w_block_rows == 1, out_dtype, (M + 127) / 128, stream);
+}
+
+int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                       int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
+                       int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype,
+                       void* y, int64_t ldy, int out_dtype, int zero_tail, void* stream) {
+  const char* what = "trk_matmul_grouped";
+  if (int rc = check_out(what, out_dtype)) return rc;
+  TRK_REQUIRE(in_dtype == TRK_E4M3 || in_dtype == TRK_BF16 || in_dtype == TRK_F16,
+              "%s: input must be TRK_E4M3, TRK_BF16 or TRK_F16", what);
+  const bool f8 = in_dtype == TRK_E4M3;
+  TRK_REQUIRE(!f8 || w_block_rows == 1 || w_block_rows == 128, "%s: w_block_rows must be 1 or 128", what);
+  TRK_REQUIRE(G >= 1 && G <= 65535 && counts, "%s: 1 to 65535 groups and their counts are required", what);
+  const int64_t item = f8 ? 1 : 2;
+  const MmArgs A{(const uint8_t*)x, (const uint8_t*)w, sx, sw, nullptr, y, counts, ldx * item, ldw * item, wg * item,
+                 sx_row, sx_kb, sw_row, sw_kb, sw_g, ldy, M, N, K, G, zero_tail};
+  if (int rc = check_mm(what, A, item, f8)) return rc;
+  if (M == 0 || N == 0) return TRK_OK;
+  return launch_mm(what, A, f8 ? IN_E4M3 : in_dtype == TRK_BF16 ? IN_BF16 : IN_F16, f8 && w_block_rows == 1, out_dtype,
+                   M / 128 + G + 1, stream);
+}
+
+int trk_matmul_grouped_dx(const void* dy, int64_t ldy, const void* w, int64_t ldw, int64_t wg, const int32_t* counts,
+                          int64_t G, int64_t M, int64_t N, int64_t K, int dtype, void* dx, int64_t ldx, void* stream) {
+  const char* what = "trk_matmul_grouped_dx";
+  TRK_REQUIRE(dtype == TRK_BF16 || dtype == TRK_F16, "%s: dtype must be TRK_BF16 or TRK_F16", what);
+  TRK_REQUIRE(G >= 1 && G <= 65535 && counts, "%s: 1 to 65535 groups and their counts are required", what);
+  TRK_REQUIRE(M >= 0 && N >= 0 && K >= 0 && M < ((int64_t)1 << 31) && N < ((int64_t)1 << 31) && K < ((int64_t)1 << 31),
+              "%s: bad shape", what);
+  if (M == 0 || K == 0) return TRK_OK;
+  TRK_REQUIRE(dx && (N == 0 || (dy && w)), "%s: null pointer", what);
+  TRK_REQUIRE(ldy >= N && ldw >= K && ldx >= K, "%s: row stride below the row's length", what);
+  TRK_REQUIRE(M / 128 + G + 1 <= 65535, "%s: too many row tiles", what);
+  const GradArgs A{(const uint16_t*)dy, nullptr, (const uint16_t*)w, dx, counts, ldy, 0, ldw, wg, ldx, 0, M, N, K, G};
+  const dim3 grid((unsigned)((K + 127) / 128), (unsigned)(M / 128 + G + 1));
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == TRK_BF16) grouped_dx_kernel<IN_BF16><<<grid, 256, 0, st>>>(A, dtype);
+  else grouped_dx_kernel<IN_F16><<<grid, 256, 0, st>>>(A, dtype);
+  return trk::check_launch(what);
+}
+
+int trk_matmul_grouped_dw(const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* counts, int64_t G,
+                          int64_t M, int64_t N, int64_t K, int dtype, void* dw, int64_t ldw, int64_t wg, void* stream) {
+  const char* what = "trk_matmul_grouped_dw";
+  TRK_REQUIRE(dtype == TRK_BF16 || dtype == TRK_F16, "%s: dtype must be TRK_BF16 or TRK_F16", what);
+  TRK_REQUIRE(G >= 1 && G <= 65535 && counts, "%s: 1 to 65535 groups and their counts are required", what);
+  TRK_REQUIRE(M >= 0 && N >= 0 && K >= 0 && M < ((int64_t)1 << 31) && N <= 65535 * 128 && K < ((int64_t)1 << 31),
+              "%s: bad shape", what);
+  if (N == 0 || K == 0) return TRK_OK;
+  TRK_REQUIRE(dw && (M == 0 || (dy && x)), "%s: null pointer", what);
+  TRK_REQUIRE(ldy >= N && ldx >= K && ldw >= K, "%s: row stride below the row's length", what);
+  const GradArgs A{(const uint16_t*)dy, (const uint16_t*)x, nullptr, dw, counts, ldy, ldx, 0, 0, ldw, wg, M, N, K, G};
+  const dim3 grid((unsigned)((K + 127) / 128), (unsigned)((N + 127) / 128), (unsigned)G);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == TRK_BF16) grouped_dw_kernel<IN_BF16><<<grid, 256, 0, st>>>(A, dtype);
+  else grouped_dw_kernel<IN_F16><<<grid, 256, 0, st>>>(A, dtype);
+  return trk::check_launch(what);
+}
+
+}  // extern "C"

@@ -1,0 +1,420 @@
+"""Linear layers in 8 bits and over ragged groups (csrc/norm_fp8.hip, csrc/linear.hip).
+
+8-bit values are float8_e4m3fn codes with one f32 scale for each block of 128 columns, either of one
+row (activations, embeddings) or of 128 rows (weights).  Codes have shape [.., rows, cols] (a row is
+padded with zeros to a multiple of 16 bytes), scales [.., rows or ceil(rows / 128), ceil(cols / 128)]
+with the rows next to each other in memory.  A call takes scales of any strides.
+
+    q, s, h = rms_norm_fp8(x, weight, residual=r)        # normalise what a layer reads, in 8 bits
+    wq, ws = quantize_fp8(w, block_rows=128)             # once, when the weights are loaded
+    y = matmul_fp8(q, s, wq, ws)                         # [rows, N]
+    y = matmul_grouped(x, w, counts)                     # rows sorted by stream, one weight for each
+
+Every call runs on the current stream of its inputs' device and never waits for it; each may be
+captured into a graph.  The 16- and 32-bit norm and the 16-bit grouped product have gradients; the
+8-bit forms are for serving and refuse inputs that require one.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+from .ops import _need_gpu, _raw_stream
+
+__all__ = ["rms_norm", "rms_norm_fp8", "quantize_fp8", "matmul_fp8", "matmul_grouped"]
+
+_P, _I, _I64, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
+_lib.register({
+    "trk_rms_norm": ([_P, _I64, _P, _I64, _P, _F, _I64, _I64, _I, _P, _I64, _P, _I64, _P, _P], _I),
+    "trk_rms_norm_fp8": ([_P, _I64, _P, _I64, _P, _F, _I64, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P], _I),
+    "trk_rms_norm_bwd_parts": ([_I64, _I64], _I64),
+    "trk_rms_norm_bwd": ([_P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _P, _I64, _P, _P], _I),
+    "trk_quantize_fp8": ([_P, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P], _I),
+    "trk_matmul_fp8": ([_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _I64, _P, _I64, _I, _P],
+                       _I),
+    "trk_matmul_grouped": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I64,
+                            _I64, _I, _P, _I64, _I, _I, _P], _I),
+    "trk_matmul_grouped_dx": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P], _I),
+    "trk_matmul_grouped_dw": ([_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _P], _I),
+})
+
+FP8 = torch.float8_e4m3fn
+_FLOAT = {torch.float32: _lib.TRK_F32, torch.bfloat16: _lib.TRK_BF16, torch.float16: _lib.TRK_F16}
+_HALF = {torch.bfloat16: _lib.TRK_BF16, torch.float16: _lib.TRK_F16}
+
+
+class _on:
+    """The device of the inputs made current for a launch (nothing where it already is)."""
+
+    __slots__ = ("idx", "before")
+
+    def __init__(self, dev: torch.device):
+        self.idx = dev.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.idx:
+            torch._C._cuda_setDevice(self.idx)
+        return _raw_stream(self.idx)
+
+    def __exit__(self, *exc):
+        if self.before != self.idx:
+            torch._C._cuda_setDevice(self.before)
+        return False
+
+
+def _type(t: torch.Tensor, of: dict, what: str, name: str) -> int:
+    dt = of.get(t.dtype)
+    if dt is None:
+        raise TypeError(f"{what}: {name} must be one of {', '.join(str(k)[6:] for k in of)}, got {t.dtype}")
+    return dt
+
+
+def _same(x: torch.Tensor, t: torch.Tensor, what: str, name: str):
+    _need_gpu(t, what)
+    if t.device != x.device:
+        raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
+
+
+def _no_grad(what: str, *ts):
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"{what}: the 8-bit form has no gradient; call it under torch.no_grad()")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t [.., D] as [R, D] with unit column stride and a row stride >= D (a view where t allows it)"""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    """row stride of a [R, D] from _rows (a single row's is not meaningful)"""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _codes(shape, device):
+    """e4m3 codes of `shape`, rows padded to 16 bytes: (tensor, row stride)"""
+    ld = (shape[-1] + 15) // 16 * 16
+    q = torch.empty((*shape[:-1], ld), device=device, dtype=FP8)
+    return (q if ld == shape[-1] else q[..., :shape[-1]]), ld
+
+
+# ------------------------------------------------------------------------------------------- norm
+def _norm_inputs(what, x, weight, residual, eps):
+    _need_gpu(x, what)
+    dt = _type(x, _FLOAT, what, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what}: x must be [.., D] with D >= 1")
+    if weight is not None:
+        _same(x, weight, what, "weight")
+        if weight.dtype != x.dtype:
+            raise TypeError(f"{what}: weight is {weight.dtype}, x {x.dtype}")
+        if weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
+            raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {list(weight.shape)}")
+    if residual is not None:
+        _same(x, residual, what, "residual")
+        if residual.dtype != x.dtype:
+            raise TypeError(f"{what}: residual is {residual.dtype}, x {x.dtype}")
+        if residual.shape != x.shape:
+            raise ValueError(f"{what}: residual is {list(residual.shape)}, x {list(x.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"{what}: eps must not be negative")
+    return dt
+
+
+def _norm_forward(dt, x, weight, residual, eps, want_rstd):
+    x2 = _rows(x)
+    R, D = x2.shape
+    r2 = _rows(residual) if residual is not None else None
+    w = weight.contiguous() if weight is not None else None
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
+    rstd = torch.empty(R, device=x.device, dtype=torch.float32) if want_rstd else None
+    with _on(x.device) as st:
+        check(lib().trk_rms_norm(
+            x2.data_ptr(), _ld(x2), r2.data_ptr() if r2 is not None else None, _ld(r2) if r2 is not None else 0,
+            w.data_ptr() if w is not None else None, eps, R, D, dt, y.data_ptr(), D,
+            h.data_ptr() if h is not None else None, D, rstd.data_ptr() if rstd is not None else None, st), "rms_norm")
+    return y, h, rstd
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, dt, eps):
+        y, h, rstd = _norm_forward(dt, x, weight, residual, eps, True)
+        ctx.save_for_backward(x if h is None else h, weight, rstd)
+        ctx.dt, ctx.pair = dt, h is not None
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:  # only the sum was used
+            return dh if need_x else None, None, dh if need_r else None, None, None
+        h2, y2 = _rows(h), _rows(dy)
+        R, D = h2.shape
+        e2 = _rows(dh) if dh is not None else None
+        w = weight.contiguous() if weight is not None else None
+        dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+        part = dw = None
+        parts = 1
+        if need_w:
+            parts = lib().trk_rms_norm_bwd_parts(R, D)
+            part = torch.empty((parts, D), device=h.device, dtype=torch.float32)
+            dw = torch.empty(D, device=h.device, dtype=h.dtype)
+        with _on(h.device) as st:
+            check(lib().trk_rms_norm_bwd(
+                h2.data_ptr(), _ld(h2), w.data_ptr() if w is not None else None, rstd.data_ptr(), y2.data_ptr(), _ld(y2),
+                e2.data_ptr() if e2 is not None else None, _ld(e2) if e2 is not None else 0, R, D, ctx.dt, dx.data_ptr(), D,
+                part.data_ptr() if part is not None else None, parts, dw.data_ptr() if dw is not None else None, st),
+                "rms_norm backward")
+        return dx if need_x else None, dw, dx if need_r else None, None, None
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
+             eps: float = 1e-6):
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x (+ residual).
+
+    x, residual [.., D] and weight [D] in bfloat16, float16 or float32 (one type).  Returns y, or with a
+    residual (y, h): h is what the next layer adds to.  Sums are f32, the norm is of the unrounded f32
+    sum; y and h are rounded once.  Differentiable in all three inputs, and through both outputs."""
+    dt = _norm_inputs("rms_norm", x, weight, residual, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
+        return _RmsNorm.apply(x, weight, residual, dt, eps)
+    y, h, _ = _norm_forward(dt, x, weight, residual, eps, False)
+    return y if h is None else (y, h)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6):
+    """rms_norm whose y is quantised as quantize_fp8(block_rows=1) does it, from f32: (q, scale), or with a
+    residual (q, scale, h).  q [.., D] float8_e4m3fn, scale [.., ceil(D / 128)] f32."""
+    what = "rms_norm_fp8"
+    dt = _norm_inputs(what, x, weight, residual, eps)
+    _no_grad(what, x, weight, residual)
+    x2 = _rows(x)
+    R, D = x2.shape
+    r2 = _rows(residual) if residual is not None else None
+    w = weight.contiguous() if weight is not None else None
+    q, ldq = _codes((R, D), x.device)
+    kb = (D + 127) // 128
+    scale = torch.empty((kb, R), device=x.device, dtype=torch.float32)
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
+    with _on(x.device) as st:
+        check(lib().trk_rms_norm_fp8(
+            x2.data_ptr(), _ld(x2), r2.data_ptr() if r2 is not None else None, _ld(r2) if r2 is not None else 0,
+            w.data_ptr() if w is not None else None, eps, R, D, dt, q.data_ptr(), ldq, scale.data_ptr(), max(R, 1),
+            h.data_ptr() if h is not None else None, D, st), what)
+    s = scale.t()
+    if x.dim() != 2:
+        q, s = q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0], s.unflatten(0, x.shape[:-1]) if x.dim() > 2 else s[0]
+    return (q, s) if h is None else (q, s, h)
+
+
+# ---------------------------------------------------------------------------------------- quantise
+def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
+    """x [rows, cols] (or a batch [B, rows, cols]) in bfloat16, float16 or float32 -> (q, scale): e4m3 codes and
+    the f32 scales of blocks of block_rows (1 or 128) x 128 values.
+
+    scale = max(|x|, 2^-117) / 448 over the block, q = x * 448 / max rounded to the nearest code (ties to
+    even).  NaN values keep a NaN code and are left out of the maximum; a block that holds an infinity has an
+    infinite scale, so that all of it reads back as NaN."""
+    what = "quantize_fp8"
+    _need_gpu(x, what)
+    dt = _type(x, _FLOAT, what, "x")
+    if block_rows not in (1, 128):
+        raise ValueError(f"{what}: block_rows must be 1 or 128")
+    if x.dim() not in (2, 3) or x.shape[-1] < 1:
+        raise ValueError(f"{what}: x must be [rows, cols] or [B, rows, cols] with cols >= 1")
+    _no_grad(what, x)
+    R, D = x.shape[-2:]
+    B = x.shape[0] if x.dim() == 3 else 1
+    if (D > 1 and x.stride(-1) != 1) or (R > 1 and x.stride(-2) < D):
+        x = x.contiguous()
+    ldx = x.stride(-2) if R > 1 else D
+    q, ldq = _codes(x.shape, x.device)
+    rb, kb = (R if block_rows == 1 else (R + 127) // 128), (D + 127) // 128
+    scale = torch.empty((*x.shape[:-2], kb, rb), device=x.device, dtype=torch.float32)
+    with _on(x.device) as st:
+        check(lib().trk_quantize_fp8(x.data_ptr(), ldx, x.stride(0) if x.dim() == 3 else 0, B, R, D, block_rows, dt,
+                                     q.data_ptr(), ldq, R * ldq, scale.data_ptr(), max(rb, 1), kb * rb, st), what)
+    return q, scale.transpose(-1, -2)
+
+
+# ---------------------------------------------------------------------------------------- products
+def _scales(what, t, name, x, rows, kb, lead=()):
+    """(block_rows, strides) of the scales of a [.., rows, K] operand"""
+    if t is None:
+        raise TypeError(f"{what}: {name} is required with 8-bit operands")
+    _same(x, t, what, name)
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
+    few = (rows + 127) // 128
+    if tuple(t.shape) == (*lead, rows, kb):
+        return 1
+    if tuple(t.shape) == (*lead, few, kb):
+        return 128
+    raise ValueError(f"{what}: {name} must be {[*lead, rows, kb]} or {[*lead, few, kb]}, got {list(t.shape)}")
+
+
+def _out(what, out, out_dtype, x, M, N, default):
+    if out is None:
+        dt = out_dtype or default
+        if dt not in _FLOAT:
+            raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {dt}")
+        return torch.empty((M, N), device=x.device, dtype=dt)
+    _same(x, out, what, "out")
+    _type(out, _FLOAT, what, "out")
+    if out_dtype is not None and out.dtype != out_dtype:
+        raise TypeError(f"{what}: out is {out.dtype}, out_dtype {out_dtype}")
+    if tuple(out.shape) != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+        raise ValueError(f"{what}: out must be [{M}, {N}] with unit column stride")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: out must not require a gradient")
+    return out
+
+
+def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
+               bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y [M, N] = x [M, K] @ w [N, K]^T (+ bias [N] f32) of float8_e4m3fn codes with their scales: x_scale
+    [M, ceil(K / 128)]; w_scale [N, ceil(K / 128)] (block_rows 1) or [ceil(N / 128), ceil(K / 128)] (128).
+
+    Each block's products are summed in f32, scaled and added in f32, and y is rounded once to out_dtype
+    (bfloat16 by default; float16, float32).  out: written in place of a new tensor (it must not overlap an
+    input)."""
+    what = "matmul_fp8"
+    _need_gpu(x, what)
+    _same(x, w, what, "w")
+    if x.dtype != FP8 or w.dtype != FP8:
+        raise TypeError(f"{what}: x and w must be float8_e4m3fn, got {x.dtype} and {w.dtype}")
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"{what}: x must be [M, K] and w [N, K], got {list(x.shape)} and {list(w.shape)}")
+    M, K = x.shape
+    N = w.shape[0]
+    kb = (K + 127) // 128
+    _no_grad(what, x_scale, w_scale, bias)
+    if _scales(what, x_scale, "x_scale", x, M, kb) != 1:
+        raise ValueError(f"{what}: x_scale must be [{M}, {kb}]")
+    wb = _scales(what, w_scale, "w_scale", x, N, kb)
+    if bias is not None:
+        _same(x, bias, what, "bias")
+        if bias.dtype != torch.float32 or bias.dim() != 1 or bias.shape[0] != N:
+            raise ValueError(f"{what}: bias must be float32 [{N}]")
+        bias = bias.contiguous()
+    y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
+    x, w = _rows(x), _rows(w)
+    with _on(x.device) as st:
+        check(lib().trk_matmul_fp8(
+            x.data_ptr(), _ld(x), x_scale.data_ptr(), *x_scale.stride(), w.data_ptr(), _ld(w), w_scale.data_ptr(),
+            *w_scale.stride(), wb, bias.data_ptr() if bias is not None else None, M, N, K, y.data_ptr(),
+            y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype], st), what)
+    return y
+
+
+def _weights(w: torch.Tensor) -> torch.Tensor:
+    if (w.shape[2] > 1 and w.stride(2) != 1) or (w.shape[1] > 1 and w.stride(1) < w.shape[2]):
+        return w.contiguous()
+    return w
+
+
+def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_tail):
+    x, w = _rows(x), _weights(w)
+    M, K = x.shape
+    G, N = w.shape[:2]
+    sx = (x_scale.data_ptr(), *x_scale.stride()) if x_scale is not None else (None, 0, 0)
+    sw = (w_scale.data_ptr(), w_scale.stride(1), w_scale.stride(2), w_scale.stride(0)) if x_scale is not None else \
+        (None, 0, 0, 0)
+    with _on(x.device) as st:
+        check(lib().trk_matmul_grouped(
+            x.data_ptr(), _ld(x), *sx, w.data_ptr(), w.stride(1) if N > 1 else max(K, 1), w.stride(0), *sw, wb,
+            counts.data_ptr(), G, M, N, K, in_dt, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype],
+            zero_tail, st), what)
+    return y
+
+
+class _Grouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, counts, dt, out_dtype):
+        ctx.save_for_backward(x, w, counts)
+        ctx.dt = dt
+        y = torch.empty((x.shape[0], w.shape[1]), device=x.device, dtype=out_dtype)
+        return _grouped_forward("matmul_grouped", x, None, w, None, 128, counts, dt, y, 1)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, counts = ctx.saved_tensors
+        x, w = _rows(x), _weights(w)
+        M, K = x.shape
+        G, N = w.shape[:2]
+        dy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        dx = dw = None
+        with _on(x.device) as st:
+            if ctx.needs_input_grad[0]:
+                dx = torch.empty((M, K), device=x.device, dtype=x.dtype)
+                check(lib().trk_matmul_grouped_dx(
+                    dy.data_ptr(), _ld(dy), w.data_ptr(), w.stride(1) if N > 1 else max(K, 1), w.stride(0),
+                    counts.data_ptr(), G, M, N, K, ctx.dt, dx.data_ptr(), max(K, 1), st), "matmul_grouped backward")
+            if ctx.needs_input_grad[1]:
+                dw = torch.empty((G, N, K), device=x.device, dtype=x.dtype)
+                check(lib().trk_matmul_grouped_dw(
+                    dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), counts.data_ptr(), G, M, N, K, ctx.dt, dw.data_ptr(),
+                    max(K, 1), N * K, st), "matmul_grouped backward")
+        return dx, dw, None, None, None
+
+
+def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
+                   w_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y [R, N] = x [R, K] @ w[g]^T with the rows of x sorted by group: the first counts[0] rows belong to
+    w[0], the next counts[1] to w[1], ..  w [G, N, K]; counts [G] int32 on the device (never read by the
+    host; values below 0 count as 0 and their sum is cut at R).
+
+    bfloat16 / float16 x and w (one type; differentiable in both), or float8_e4m3fn with x_scale
+    [R, ceil(K / 128)] and w_scale [G, N or ceil(N / 128), ceil(K / 128)].  y is rounded once to out_dtype
+    (x's type, or bfloat16 for 8 bits; float16, float32).  Rows behind the last group are zeros in a new y;
+    with `out` they are left as they were."""
+    what = "matmul_grouped"
+    _need_gpu(x, what)
+    _same(x, w, what, "w")
+    _same(x, counts, what, "counts")
+    if x.dtype != w.dtype:
+        raise TypeError(f"{what}: x is {x.dtype}, w {w.dtype}")
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2] or w.shape[0] < 1:
+        raise ValueError(f"{what}: x must be [R, K] and w [G >= 1, N, K], got {list(x.shape)} and {list(w.shape)}")
+    G, N, K = w.shape
+    M = x.shape[0]
+    if counts.dtype != torch.int32 or counts.dim() != 1 or counts.shape[0] != G:
+        raise ValueError(f"{what}: counts must be int32 [{G}]")
+    counts = counts.contiguous()
+    if x.dtype == FP8:
+        _no_grad(what, x_scale, w_scale)
+        kb = (K + 127) // 128
+        if _scales(what, x_scale, "x_scale", x, M, kb) != 1:
+            raise ValueError(f"{what}: x_scale must be [{M}, {kb}]")
+        wb = _scales(what, w_scale, "w_scale", x, N, kb, (G,))
+        y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
+        return _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, _lib.TRK_E4M3, y, int(out is None))
+    dt = _type(x, _HALF, what, "x")
+    if x_scale is not None or w_scale is not None:
+        raise TypeError(f"{what}: scales go with float8_e4m3fn operands only")
+    y = _out(what, out, out_dtype, x, M, N, x.dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        if out is not None:
+            raise ValueError(f"{what}: `out` has no gradient; call without it, or under torch.no_grad()")
+        return _Grouped.apply(x, w, counts, dt, y.dtype)
+    return _grouped_forward(what, x, None, w, None, 128, counts, dt, y, int(out is None))

@@ -33,7 +33,7 @@ enum {
   TRK_EUNSUPPORTED = -3/* shape outside what the kernel implements          */
 };
 
-enum { TRK_F32 = 0, TRK_BF16 = 1, TRK_F64 = 2 };
+enum { TRK_F32 = 0, TRK_BF16 = 1, TRK_F64 = 2, TRK_F16 = 3, TRK_E4M3 = 4 };
 enum { TRK_NCHW = 0, TRK_NHWC = 1 };
 
 int trk_abi_version(void);
@@ -299,6 +299,65 @@ int trk_enc_se_means(const float* m_r, int64_t R, int64_t C, const float* w1, co
 int trk_enc_head(const long long* tsums, int64_t R, int64_t P, int64_t C, const float* s, const float* m_r,
                  const float* m_n, double alpha, const float* w0, const float* ln_w, const float* ln_b,
                  float ln_eps, const float* w4, const float* b4, int64_t D, float* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Linear layers in 8 bits and over ragged groups.  Rows have unit column stride
+ * and any row stride >= their length (ld, in elements, as all strides below); rows
+ * may start at any address.  8-bit values are e4m3 codes with one f32 scale for
+ * each block of 128 columns (of one row, or of 128 rows); a block stands for
+ * code * scale.  Sums are f32.
+ *
+ * trk_rms_norm: h = x + residual (residual NULL: x), r = 1 / sqrt(mean(h^2) + eps),
+ *   y = h r weight (weight NULL: 1) for R rows of D; dtype TRK_F32 / BF16 / F16 of x,
+ *   residual, weight, y, h.  h (NULL: not wanted) is rounded once; the norm is of the f32
+ *   sum.  rstd (NULL: not wanted) [R] = r, for the backward pass.
+ * trk_rms_norm_fp8: the same y, quantised: q [R][ldq] e4m3, scale[kb * scale_ld + row],
+ *   kb < ceil(D / 128).  Where ldq has room for it, a row is padded with zeros to a
+ *   multiple of 16 bytes (q must own those bytes).  scale = max(|y|, 2^-117) / 448 over
+ *   the block; NaN values give NaN codes and are left out of the maximum; a block that
+ *   holds an infinity has an infinite scale (all of it comes back as NaN).
+ * trk_rms_norm_bwd: dx = r (g - n mean(g n)) + dh with g = dy weight, n = h r (dh NULL: 0),
+ *   and dw (NULL: not wanted) [D] = sum over rows of dy n, joined in a fixed order from the
+ *   workspace part [parts][D] f32, parts = trk_rms_norm_bwd_parts(R, D).
+ * trk_quantize_fp8: B matrices x [R][D] (xb, qb, sb: strides of the batch) in blocks of
+ *   block_rows (1 or 128) x 128: scale[b * sb + kb * scale_ld + row or row block]; padding
+ *   as above.
+ * ---------------------------------------------------------------------- */
+int trk_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, float eps,
+                 int64_t R, int64_t D, int dtype, void* y, int64_t ldy, void* h, int64_t ldh, float* rstd,
+                 void* stream);
+int trk_rms_norm_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr, const void* weight, float eps,
+                     int64_t R, int64_t D, int dtype, void* q, int64_t ldq, float* scale, int64_t scale_ld, void* h,
+                     int64_t ldh, void* stream);
+int64_t trk_rms_norm_bwd_parts(int64_t R, int64_t D);
+int trk_rms_norm_bwd(const void* h, int64_t ldh, const void* weight, const float* rstd, const void* dy, int64_t ldy,
+                     const void* dh, int64_t lddh, int64_t R, int64_t D, int dtype, void* dx, int64_t ldx,
+                     float* part, int64_t parts, void* dw, void* stream);
+int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t R, int64_t D, int block_rows,
+                     int dtype, void* q, int64_t ldq, int64_t qb, float* scale, int64_t scale_ld, int64_t sb,
+                     void* stream);
+/* trk_matmul_fp8: y [M][N] = x [M][K] . w [N][K]^T + bias (f32 [N], NULL: 0) of e4m3 codes:
+ *   sum over the blocks kb of 128 columns of sx[m * sx_row + kb * sx_kb] *
+ *   sw[(n / w_block_rows) * sw_row + kb * sw_kb] * (the block's products); w_block_rows 1 or
+ *   128; out_dtype TRK_F32 / BF16 / F16.
+ * trk_matmul_grouped: the rows of x sorted by group, counts[g] (device, int32) of them for
+ *   w [g] (wg: stride of the groups): y = x . w[g]^T.  in_dtype TRK_E4M3 (with scales; sw_g:
+ *   stride of the groups) or TRK_BF16 / F16 (scales not read).  Counts below 0 are 0 and
+ *   their sum is cut at M.  Rows behind the last group are written as zeros (zero_tail) or
+ *   left as they were.
+ * trk_matmul_grouped_dx / _dw: the 16-bit product's gradients, dx = dy . w[g] (rows behind
+ *   the last group: zeros) and dw[g] = dy_g^T . x_g (a group without rows: zeros). */
+int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                   int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_kb, int w_block_rows, const float* bias,
+                   int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, void* stream);
+int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                       int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
+                       int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype,
+                       void* y, int64_t ldy, int out_dtype, int zero_tail, void* stream);
+int trk_matmul_grouped_dx(const void* dy, int64_t ldy, const void* w, int64_t ldw, int64_t wg, const int32_t* counts,
+                          int64_t G, int64_t M, int64_t N, int64_t K, int dtype, void* dx, int64_t ldx, void* stream);
+int trk_matmul_grouped_dw(const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* counts, int64_t G,
+                          int64_t M, int64_t N, int64_t K, int dtype, void* dw, int64_t ldw, int64_t wg, void* stream);
 
 /* ------------------------------------------------------------------------
  * Device-resident track state.  Track slots of all

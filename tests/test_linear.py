@@ -1,0 +1,681 @@
+"""The 8-bit and ragged linear operators (rms_norm, rms_norm_fp8, quantize_fp8, matmul_fp8, matmul_grouped)
+against plain 64-bit forms.
+
+Tolerances count roundings, u = 2^-24 for f32:
+  norm      the sum of squares has chains of at most 96 additions and 8 joins, all positive: |d ss| <= 104 u ss, so r is
+            off by 52 u, a division, a square root, two products: |dy| <= 60 u |y| < 2^-18 |y|, plus half a step of y's type
+  codes     half a step (2^-4 of the value, 2^-10 of the scale below the smallest normal code), on a value 2^-18 off
+  products  an f32 sum of n products is off by n u sum |products| at most; plus half a step of y's type
+"""
+import ctypes
+import itertools
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -150}
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+FP8 = torch.float8_e4m3fn
+gpu_test = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------ plain forms
+def norm64(x, w, res, eps):
+    h = x.double() if res is None else x.double() + res.double()
+    r = 1 / torch.sqrt(h.square().mean(-1, keepdim=True) + eps)
+    y = h * r
+    return h, r, y if w is None else y * w.double()
+
+
+def near(got, want, dtype, slack):
+    """|got - want| <= slack + half a step of dtype"""
+    want = want.to(got.device)
+    slack = slack.to(got.device) if isinstance(slack, torch.Tensor) else slack
+    d = (got.double() - want).abs()
+    tol = slack + want.abs() * HALF[dtype] * (1 + 2.0 ** -10) + TINY[dtype]
+    bad = ~(d <= tol)
+    assert not bad.any(), (int(bad.sum()), float((d / tol.clamp_min(1e-300)).max()))
+
+
+def widen(q, s, block):
+    rows, cols = q.shape[-2:]
+    each = s.double().repeat_interleave(128, -1)[..., :cols]
+    if block != 1:
+        each = each.repeat_interleave(128, -2)[..., :rows, :]
+    return q.double() * each
+
+
+def block_top(v, block):
+    rows, cols = v.shape[-2:]
+    kb, rb = -(-cols // 128), -(-rows // block)
+    full = torch.zeros((*v.shape[:-2], rb * block, kb * 128), dtype=torch.float64, device=v.device)
+    full[..., :rows, :cols] = v.abs()
+    return full.view(*v.shape[:-2], rb, block, kb, 128).amax((-3, -1)).clamp_min(2.0 ** -117)
+
+
+def check_codes(q, s, v, block, off=0.0):
+    """codes q and scales s stand for v (known to a relative `off`)"""
+    top = block_top(v, block)
+    assert s.dtype == F32 and q.dtype == FP8 and q.shape == v.shape
+    assert ((s.double() * 448 / top - 1).abs() <= 4 * U + off).all()
+    each = s.double().repeat_interleave(128, -1)[..., :v.shape[-1]]
+    if block != 1:
+        each = each.repeat_interleave(block, -2)[..., :v.shape[-2], :]
+    d = (q.double() * each - v).abs()
+    tol = torch.maximum(v.abs() * 2.0 ** -4, each * 2.0 ** -10) * (1 + 2.0 ** -16) + v.abs() * (off + 4 * U)
+    assert (d <= tol).all(), float((d / tol).max())
+
+
+def codes_of(gen, rows, cols, block, dev, lead=()):
+    """random codes and scales of ordinary sizes"""
+    v = torch.randn((*lead, rows, cols), generator=gen, device=dev)
+    rb = rows if block == 1 else -(-rows // 128)
+    s = torch.rand((*lead, rb, -(-cols // 128)), generator=gen, device=dev) * 0.1 + 0.01
+    return (v * 40).clamp(-448, 448).to(FP8), s
+
+
+def gen_of(dev, *seed):
+    return torch.Generator(device=dev).manual_seed(hash(seed) % (1 << 31))
+
+
+def bounds_of(counts, rows):
+    """the rows of each group"""
+    at, out = 0, []
+    for c in counts:
+        n = min(max(0, c), rows - at)
+        out.append((at, at + n))
+        at += n
+    return out, at
+
+
+# ------------------------------------------------------------------------------------------- refusals
+def test_host_argument_errors(trk):
+    L = trk.lib()
+    v, z = ctypes.c_void_p(256), None
+
+    def refused(rc, text, code=-1):
+        assert rc == code and text in L.trk_last_error(), (rc, L.trk_last_error())
+
+    refused(L.trk_rms_norm(v, 8, z, 0, z, 1e-6, 4, 8, 9, v, 8, z, 0, z, z), b"dtype")
+    refused(L.trk_rms_norm(v, 8, z, 0, z, 1e-6, 4, 0, 0, v, 8, z, 0, z, z), b"bad shape")
+    refused(L.trk_rms_norm(z, 8, z, 0, z, 1e-6, 4, 8, 0, v, 8, z, 0, z, z), b"null")
+    refused(L.trk_rms_norm(v, 7, z, 0, z, 1e-6, 4, 8, 0, v, 8, z, 0, z, z), b"row stride")
+    refused(L.trk_rms_norm(v, 8, z, 0, z, -1.0, 4, 8, 0, v, 8, z, 0, z, z), b"eps")
+    refused(L.trk_rms_norm_fp8(v, 8, z, 0, z, 1e-6, 4, 8, 0, v, 8, z, 4, z, 0, z), b"scale")
+    refused(L.trk_rms_norm_fp8(v, 8, z, 0, z, 1e-6, 4, 8, 0, v, 8, v, 3, z, 0, z), b"scale")
+    refused(L.trk_rms_norm_bwd(v, 8, z, v, v, 8, z, 0, 4, 8, 0, v, 8, z, 1, v, z), b"workspace")
+    refused(L.trk_rms_norm_bwd(v, 8, z, v, v, 8, z, 0, 4, 8, 0, v, 8, v, 77, v, z), b"parts")
+    refused(L.trk_quantize_fp8(v, 8, 0, 1, 4, 8, 64, 0, v, 8, 0, v, 4, 0, z), b"block_rows")
+    refused(L.trk_quantize_fp8(v, 8, 0, 1, 4, 8, 1, 0, v, 8, 0, v, 3, 0, z), b"scale_ld")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 7, z, 4, 4, 8, v, 4, 0, z), b"w_block_rows")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 2, z), b"output")
+    refused(L.trk_matmul_fp8(v, 7, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, z), b"row stride")
+    refused(L.trk_matmul_fp8(v, 8, z, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, z), b"null")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, -8, v, 4, 0, z), b"bad shape")
+    refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, v, 0, 4, 4, 8, 1, v, 4, 1, 0, z), b"groups")
+    refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, v, 2, 4, 4, 8, 0, v, 4, 1, 0, z), b"input")
+    refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, z, 2, 4, 4, 8, 1, v, 4, 1, 0, z), b"groups")
+    refused(L.trk_matmul_grouped_dx(v, 4, v, 8, 32, v, 2, 4, 4, 8, 0, v, 8, z), b"dtype")
+    refused(L.trk_matmul_grouped_dw(v, 3, v, 8, v, 2, 4, 4, 8, 1, v, 8, 32, z), b"row stride")
+    # nothing to do
+    assert L.trk_rms_norm(z, 8, z, 0, z, 1e-6, 0, 8, 0, z, 8, z, 0, z, z) == 0
+    assert L.trk_quantize_fp8(z, 8, 0, 0, 4, 8, 1, 0, z, 8, 0, z, 4, 0, z) == 0
+    assert L.trk_matmul_fp8(z, 8, z, 0, 0, z, 8, z, 0, 0, 1, z, 0, 4, 8, z, 4, 0, z) == 0
+
+
+def test_host_tensors_are_refused(trk):
+    x = torch.zeros(2, 4)
+    q, s = x.to(FP8), torch.ones(2, 1)
+    for call in (lambda: trk.rms_norm(x), lambda: trk.rms_norm_fp8(x), lambda: trk.quantize_fp8(x),
+                 lambda: trk.matmul_fp8(q, s, q, s),
+                 lambda: trk.matmul_grouped(x.bfloat16(), x.bfloat16()[None], torch.tensor([2], dtype=torch.int32))):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+@gpu_test
+def test_refusals(trk, gpu):
+    x = torch.zeros(4, 32, device=gpu, dtype=BF)
+    q, s = torch.zeros(4, 32, device=gpu).to(FP8), torch.ones(4, 1, device=gpu)
+    w3, c = x[None].repeat(2, 1, 1), torch.tensor([1, 3], device=gpu, dtype=torch.int32)
+    T, V, N = TypeError, ValueError, NotImplementedError
+    for err, call in (
+            (T, lambda: trk.rms_norm(x.double())), (T, lambda: trk.rms_norm(x, x[0].float())),
+            (V, lambda: trk.rms_norm(x, x[0, :5])), (V, lambda: trk.rms_norm(x, residual=x[:2])),
+            (T, lambda: trk.rms_norm(x, residual=x.float())), (V, lambda: trk.rms_norm(x, eps=-1.0)),
+            (V, lambda: trk.rms_norm(x, eps=float("nan"))), (V, lambda: trk.rms_norm(x[:, :0])),
+            (RuntimeError, lambda: trk.rms_norm(x, x[0].cpu())),
+            (N, lambda: trk.rms_norm_fp8(x.float().requires_grad_())), (N, lambda: trk.quantize_fp8(x.float().requires_grad_())),
+            (V, lambda: trk.quantize_fp8(x, block_rows=64)), (V, lambda: trk.quantize_fp8(x[0])),
+            (T, lambda: trk.quantize_fp8(x.double())),
+            (T, lambda: trk.matmul_fp8(x, s, q, s)), (V, lambda: trk.matmul_fp8(q, s, q[:, :16], s)),
+            (V, lambda: trk.matmul_fp8(q, s[:1], q, s)), (V, lambda: trk.matmul_fp8(q, s, q, s[:2])),
+            (T, lambda: trk.matmul_fp8(q, s.double(), q, s)), (T, lambda: trk.matmul_fp8(q, s, q, s, out_dtype=torch.float64)),
+            (V, lambda: trk.matmul_fp8(q, s, q, s, bias=s[:, 0].bfloat16())),
+            (V, lambda: trk.matmul_fp8(q, s, q, s, out=torch.empty(4, 5, device=gpu))),
+            (T, lambda: trk.matmul_fp8(q, s, q, s, out=torch.empty(4, 4, device=gpu), out_dtype=BF)),
+            (N, lambda: trk.matmul_fp8(q, s.clone().requires_grad_(), q, s)),
+            (T, lambda: trk.matmul_grouped(x.float(), w3.float(), c)), (T, lambda: trk.matmul_grouped(x, w3.half(), c)),
+            (V, lambda: trk.matmul_grouped(x, w3[0], c)), (V, lambda: trk.matmul_grouped(x, w3, c.long())),
+            (V, lambda: trk.matmul_grouped(x, w3, c[:1])), (RuntimeError, lambda: trk.matmul_grouped(x, w3, c.cpu())),
+            (T, lambda: trk.matmul_grouped(x, w3, c, x_scale=s)), (T, lambda: trk.matmul_grouped(q, q[None], c[:1])),
+            (V, lambda: trk.matmul_grouped(q, q[None], c[:1], x_scale=s, w_scale=s)),
+            (V, lambda: trk.matmul_grouped(x.clone().requires_grad_(), w3, c, out=x.new_empty(4, 4)))):
+        with pytest.raises(err):
+            call()
+
+
+# ----------------------------------------------------------------------------------------------- norm
+NORM = [(1, 1), (3, 7), (5, 16), (17, 127), (16, 128), (33, 129), (7, 500), (9, 512), (3, 513), (5, 1000), (2, 1024),
+        (3, 2047), (2, 2048), (1, 4096), (2, 5001), (2, 8192), (3, 8193), (1, 20001)]
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("rows,cols", NORM)
+def test_norm(trk, gpu, rows, cols, dtype):
+    g = gen_of(gpu, rows, cols)
+    for has_w, has_r in itertools.product((False, True), repeat=2):
+        x = (torch.randn(rows, cols, device=gpu, generator=g) * 3).to(dtype)
+        w = torch.randn(cols, device=gpu, generator=g).to(dtype) if has_w else None
+        r = torch.randn(rows, cols, device=gpu, generator=g).to(dtype) if has_r else None
+        h64, _, y64 = norm64(x, w, r, 1e-5)
+        out = trk.rms_norm(x, w, residual=r, eps=1e-5)
+        y, h = out if has_r else (out, None)
+        near(y, y64, dtype, y64.abs() * 2.0 ** -18)
+        if has_r:
+            near(h, h64, dtype, h64.abs() * U)
+        o8 = trk.rms_norm_fp8(x, w, residual=r, eps=1e-5)
+        check_codes(o8[0], o8[1], y64, 1, 2.0 ** -18)
+        if has_r:
+            assert torch.equal(o8[2], h)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_norm_layouts(trk, gpu, dtype):
+    """strided rows, more dimensions, a transposed and a broadcast input, rows that start at odd addresses"""
+    g = gen_of(gpu, 5)
+    big = torch.randn(6, 5, 301, device=gpu, generator=g).to(dtype)
+    for x in (big[:, 1:3, 5:262], big[..., 1:], big[0, :, ::2], big[0].t(), big[0, 0], big[:1, :1].expand(3, 4, 301),
+              big[:0], big.permute(1, 0, 2)):
+        _, _, y64 = norm64(x, None, x, 1e-6)
+        y, h = trk.rms_norm(x, residual=x)
+        assert y.shape == x.shape and h.shape == x.shape
+        near(y, y64, dtype, y64.abs() * 2.0 ** -18)
+        q, s, h8 = trk.rms_norm_fp8(x, residual=x)
+        assert s.shape == (*x.shape[:-1], -(-x.shape[-1] // 128)) and torch.equal(h, h8)
+        D = x.shape[-1]
+        if x.numel():
+            check_codes(q.reshape(-1, D), s.reshape(-1, s.shape[-1]), y64.reshape(-1, D), 1, 2.0 ** -18)
+
+
+@gpu_test
+def test_norm_special_rows(trk, gpu):
+    """zero rows, an infinity, a NaN: other rows are untouched by them"""
+    x = torch.randn(6, 200, device=gpu, generator=gen_of(gpu, 6))
+    x[1] = 0
+    x[2, 7] = float("inf")
+    x[3, 9] = float("nan")
+    y = trk.rms_norm(x)
+    _, _, y64 = norm64(x, None, None, 1e-6)
+    ok = [0, 1, 4, 5]
+    near(y[ok], y64[ok], F32, y64[ok].abs() * 2.0 ** -18)
+    assert y[2, 7].isnan() and (y[2, :7] == 0).all() and y[3].isnan().all()
+    q, s = trk.rms_norm_fp8(x)
+    check_codes(q[ok], s[ok], y64[ok], 1, 2.0 ** -18)
+    assert q[3].float().isnan().all() and (q[1].float() == 0).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("rows,cols", NORM + [(3000, 96), (2500, 512), (1500, 1500)])
+def test_norm_gradient(trk, gpu, rows, cols, dtype):
+    g = gen_of(gpu, rows, cols, 1)
+    for has_w, has_r in ((True, False), (True, True), (False, False)):
+        x = torch.randn(rows, cols, device=gpu, generator=g).to(dtype).requires_grad_()
+        w = torch.randn(cols, device=gpu, generator=g).to(dtype).requires_grad_() if has_w else None
+        r = torch.randn(rows, cols, device=gpu, generator=g).to(dtype).requires_grad_() if has_r else None
+        dy, dh = (torch.randn(rows, cols, device=gpu, generator=g).to(dtype) for _ in range(2))
+        out = trk.rms_norm(x, w, residual=r, eps=1e-5)
+        leaves = [t for t in (x, w, r) if t is not None]
+        got = torch.autograd.grad(out, leaves, (dy, dh) if has_r else dy)
+        with torch.no_grad():
+            _, r64, _ = norm64(x, w, r, 1e-5)
+            n = (out[1] if has_r else x).double() * r64  # the stored sum is what the gradient is taken at
+            g64 = dy.double() * (1 if w is None else w.double())
+            m = (g64 * n).mean(1, keepdim=True)
+            dx = r64 * (g64 - n * m) + (dh.double() if has_r else 0)
+            # n, m 2^-18 off relative to their own sizes, six more roundings
+            slack = 2.0 ** -17 * (r64 * (g64.abs() + n.abs() * (g64 * n).abs().mean(1, keepdim=True)) +
+                                  (dh.double().abs() if has_r else 0))
+            near(got[0], dx, dtype, slack)
+            if has_w:
+                near(got[1], (dy.double() * n).sum(0), dtype, (dy.double() * n).abs().sum(0) * ((rows + 64) * U + 2.0 ** -18))
+            if has_r:
+                assert torch.equal(got[-1], got[0])
+
+
+@gpu_test
+def test_norm_gradient_against_differences(trk, gpu):
+    g = gen_of(gpu, 8)
+    x, r, dy, dh = (torch.randn(3, 37, device=gpu, generator=g) for _ in range(4))
+    w = torch.randn(37, device=gpu, generator=g)
+    leaves = [t.requires_grad_() for t in (x, w, r)]
+    got = torch.autograd.grad(trk.rms_norm(x, w, residual=r), leaves, (dy, dh))
+
+    def loss(a, b, c):
+        h, _, y = norm64(a, b, c, 1e-6)
+        return (y * dy.double()).sum() + (h * dh.double()).sum()
+
+    args = [t.detach().double() for t in leaves]
+    e = 1e-5
+    for k, i in ((0, 5), (0, 100), (1, 0), (1, 36), (2, 73)):
+        lo, hi = ([t.clone() for t in args] for _ in range(2))
+        lo[k].view(-1)[i] -= e
+        hi[k].view(-1)[i] += e
+        d = float((loss(*hi) - loss(*lo)) / (2 * e))
+        assert abs(float(got[k].reshape(-1)[i]) - d) <= 1e-4 * (1 + abs(d))  # e^2 third derivative: below 1e-8; f32 gradient
+
+
+@gpu_test
+def test_norm_gradient_uses(trk, gpu):
+    """only one output used, gradients of some inputs only, a gradient that is a broadcast"""
+    x = torch.randn(9, 130, device=gpu, dtype=F32, generator=gen_of(gpu, 9)).requires_grad_()
+    r = torch.randn(9, 130, device=gpu, dtype=F32, generator=gen_of(gpu, 10)).requires_grad_()
+    y, h = trk.rms_norm(x, residual=r)
+    assert torch.equal(torch.autograd.grad(h.sum(), x, retain_graph=True)[0], torch.ones_like(x))
+    a = torch.autograd.grad(y.sum(), x, retain_graph=True)[0]
+    b = torch.autograd.grad(y, x, torch.ones_like(y))[0]
+    assert torch.equal(a, b)
+    w = torch.randn(130, device=gpu, generator=gen_of(gpu, 11)).requires_grad_()
+    dw, = torch.autograd.grad(trk.rms_norm(x.detach(), w).sum(), w)
+    n = norm64(x.detach(), None, None, 1e-6)[2]
+    near(dw, n.sum(0), F32, n.abs().sum(0) * 2.0 ** -17)
+    e = trk.rms_norm(torch.zeros(0, 130, device=gpu), w)
+    assert torch.equal(torch.autograd.grad(e.sum(), w)[0], torch.zeros_like(w))
+
+
+# ------------------------------------------------------------------------------------------- quantise
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("shape", [(1, 1), (5, 16), (127, 128), (128, 127), (129, 129), (40, 1111), (300, 640), (3, 65, 200),
+                                   (2, 130, 48), (0, 8), (2, 0, 8)])
+def test_quantize(trk, gpu, shape, dtype, block):
+    x = (torch.randn(*shape, device=gpu, generator=gen_of(gpu, shape)) * 5).to(dtype)
+    q, s = trk.quantize_fp8(x, block_rows=block)
+    assert q.shape == x.shape and s.shape == (*shape[:-2], -(-shape[-2] // block), -(-shape[-1] // 128))
+    if x.numel():
+        check_codes(q, s, x.double(), block)
+        # the padding behind a row's last value is zeros
+        ld = q.stride(-2)
+        assert ld % 16 == 0
+        raw = torch.as_strided(q.view(torch.uint8), (q.numel() // shape[-1], ld), (ld, 1))
+        assert (raw[:, shape[-1]:] == 0).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_special_values(trk, gpu, block):
+    x = torch.randn(256, 384, device=gpu, generator=gen_of(gpu, 3))
+    x[:128, :128] = 0
+    x[128:, :128] = 1e-38 * torch.rand(128, 128, device=gpu, generator=gen_of(gpu, 4))
+    x[:128, 128:256] *= 1e36
+    x[5, 300] = float("nan")
+    x[200, 300] = float("-inf")
+    q, s = trk.quantize_fp8(x, block_rows=block)
+    v = widen(q, s, block)
+    assert (v[:128, :128] == 0).all()
+    check_codes(q[:, :256], s[:, :2], x[:, :256].double(), block)
+    assert v[5, 300].isnan()
+    clean = x[:128, 256:].clone()
+    clean[5, 44] = 0
+    q2 = q[:128, 256:].float()
+    q2[5, 44] = 0
+    check_codes(q2.to(FP8), s[:128 // block, 2:], clean.double(), block)  # the NaN is left out of the maximum
+    hit = slice(200, 201) if block == 1 else slice(128, 256)
+    assert v[hit, 256:].isnan().all()
+
+
+@gpu_test
+def test_quantize_layouts(trk, gpu):
+    big = torch.randn(4, 60, 301, device=gpu, generator=gen_of(gpu, 12))
+    for x in (big[:, ::2, 3:], big[1, 5:, 1:200], big[0].t(), big.transpose(1, 2), big[:1].expand(3, -1, -1)):
+        for block in (1, 128):
+            q, s = trk.quantize_fp8(x, block_rows=block)
+            q2, s2 = trk.quantize_fp8(x.contiguous(), block_rows=block)
+            assert torch.equal(q.float(), q2.float()) and torch.equal(s, s2)
+
+
+# ---------------------------------------------------------------------------------------- 8-bit product
+def product_slack(xv, wv, kb, dtype=F32):
+    """What an 8-bit product may be off before its last rounding.  Each block's 128 products summed, kb scaled sums, the
+    scale's and the bias's roundings: (132 + kb) u sum |products|.  For a 16-bit y the matrix instruction aligns
+    the 16 products of a chunk to the largest of their exponents e and drops what is below 2^(e - 13) of
+    each: a product is off by less than 2^-13 of the chunk's largest, which is at most max |x| max |w| over the chunk."""
+    slack = (xv.abs() @ wv.abs().t()) * (132 + kb) * U
+    if dtype != F32:
+        top = [torch.nn.functional.pad(v.abs(), (0, -v.shape[1] % 16)).unflatten(1, (-1, 16)).amax(2) for v in (xv, wv)]
+        slack = slack + 16 * 2.0 ** -13 * (top[0] @ top[1].t())
+    return slack
+
+
+MM = [(1, 1, 1), (1, 16, 128), (3, 5, 17), (16, 64, 256), (17, 33, 130), (2, 300, 1000), (64, 129, 384), (65, 96, 127),
+      (127, 255, 512), (130, 128, 640), (257, 260, 200), (300, 520, 1024), (31, 1000, 2048), (513, 40, 48), (5, 7, 0)]
+
+
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("M,N,K", MM)
+def test_matmul_fp8(trk, gpu, M, N, K, block):
+    g = gen_of(gpu, M, N, K)
+    x, sx = codes_of(g, M, K, 1, gpu)
+    w, sw = codes_of(g, N, K, block, gpu)
+    xv, wv = widen(x, sx, 1), widen(w, sw, block)
+    kb = sx.shape[1]
+    for dtype, bias in ((BF, None), (F16, torch.randn(N, device=gpu, generator=g)), (F32, None), (None, None)):
+        y = trk.matmul_fp8(x, sx, w, sw, bias=bias, out_dtype=dtype)
+        want = xv @ wv.t() + (0 if bias is None else bias.double())
+        assert y.dtype == (dtype or BF)
+        near(y, want, y.dtype, product_slack(xv, wv, kb, y.dtype) + want.abs() * 2 * U)
+        if M * N * K >= 10000:  # in the root mean square: a rounding of y, and far less than that from the sums
+            assert float((y.double() - want).norm() / want.norm()) <= 0.75 * HALF[y.dtype] + (0 if y.dtype != F32 else 2.0 ** -20)
+
+
+@gpu_test
+def test_matmul_fp8_layouts(trk, gpu):
+    """rows inside wider buffers (aligned and not), scales of other strides, an output inside a wider one"""
+    g = gen_of(gpu, 20)
+    M, N, K = 150, 140, 300
+    big, _ = codes_of(g, 160, 700, 1, gpu)
+    _, sx = codes_of(g, M, K, 1, gpu)
+    _, sw = codes_of(g, N, K, 1, gpu)
+    for off in (0, 1, 16, 37):
+        x, w = big[:M, off:off + K], big[10:10 + N, 350 + off:350 + off + K]
+        want = widen(x, sx, 1) @ widen(w, sw, 1).t()
+        slack = product_slack(widen(x, sx, 1), widen(w, sw, 1), 3)
+        for a, b in ((sx, sw), (sx.t().contiguous().t(), sw), (sx[:, [0, 0, 1, 1, 2, 2]][:, ::2], sw.t().contiguous().t())):
+            y = trk.matmul_fp8(x, a, w, b, out_dtype=F32)
+            near(y, want, F32, slack)
+        out = torch.full((M + 2, N + 5), 7.0, device=gpu)
+        o = trk.matmul_fp8(x, sx, w, sw, out=out[1:-1, 3:-2])
+        assert o.data_ptr() == out[1:-1, 3:-2].data_ptr()
+        near(o, want, F32, slack)
+        edge = out.clone()
+        edge[1:-1, 3:-2] = 7.0
+        assert (edge == 7.0).all()  # nothing around it was written
+
+
+@gpu_test
+def test_matmul_fp8_ignores_what_lies_behind_a_row(trk, gpu):
+    """NaN codes behind the last column and behind the last row are not read into any sum"""
+    g = gen_of(gpu, 21)
+    for K in (5, 100, 144, 200):
+        x, sx = codes_of(g, 20, K, 1, gpu)
+        w, sw = codes_of(g, 30, K, 1, gpu)
+        bx = torch.full((40, 256), 0x7f, device=gpu, dtype=torch.uint8).view(FP8)
+        bw = bx.clone()
+        bx[:20, :K], bw[:30, :K] = x, w
+        assert torch.equal(trk.matmul_fp8(bx[:20, :K], sx, bw[:30, :K], sw, out_dtype=F32).isnan().any(),
+                           torch.tensor(False, device=gpu))
+        want = widen(x, sx, 1) @ widen(w, sw, 1).t()
+        near(trk.matmul_fp8(bx[:20, :K], sx, bw[:30, :K], sw, out_dtype=F32), want, F32,
+             product_slack(widen(x, sx, 1), widen(w, sw, 1), 2))
+
+
+@gpu_test
+def test_matmul_fp8_special_codes(trk, gpu):
+    """a NaN code or an infinite scale reaches its own row (or column) only"""
+    g = gen_of(gpu, 22)
+    x, sx = codes_of(g, 40, 256, 1, gpu)
+    w, sw = codes_of(g, 50, 256, 1, gpu)
+    x[3, 7] = float("nan")
+    sx[5, 1] = float("inf")
+    y = trk.matmul_fp8(x, sx, w, sw, out_dtype=F32)
+    assert y[3].isnan().all() and not y[5].isfinite().any()
+    ok = [i for i in range(40) if i not in (3, 5)]
+    want = widen(x[ok], sx[ok], 1) @ widen(w, sw, 1).t()
+    near(y[ok], want, F32, product_slack(widen(x[ok], sx[ok], 1), widen(w, sw, 1), 2))
+
+
+# ------------------------------------------------------------------------------------------- grouped
+def grouped64(x, w, counts):
+    y = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float64, device=x.device)
+    slack = torch.zeros_like(y)
+    spans, end = bounds_of(counts, x.shape[0])
+    for g, (a, b) in enumerate(spans):
+        y[a:b] = x[a:b].double() @ w[g].double().t()
+        slack[a:b] = x[a:b].double().abs() @ w[g].double().abs().t()
+    return y, slack, end
+
+
+COUNTS = [[5], [0], [3, 0, 4], [1] * 9, [200, 1, 0, 0, 130], [128, 128], [0, 0, 300], [17, -3, 40], [90, 1000], [0] * 70 + [33] + [2] * 60]
+DIMS = [(16, 64), (1, 1), (33, 70), (128, 256), (130, 100), (200, 130)]
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("counts", COUNTS, ids=lambda c: f"{len(c)}g{sum(c)}")
+def test_matmul_grouped_and_gradients(trk, gpu, counts, dtype):
+    g = gen_of(gpu, len(counts), sum(counts))
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    total = sum(max(0, v) for v in counts)
+    for (N, K), rows in zip(DIMS, (total, total + 3, total, total + 140, total if total < 900 else 400, total + 1)):
+        x = torch.randn(rows, K, device=gpu, generator=g).to(dtype).requires_grad_()
+        w = torch.randn(len(counts), N, K, device=gpu, generator=g).to(dtype).requires_grad_()
+        dy = torch.randn(rows, N, device=gpu, generator=g).to(dtype)
+        y = trk.matmul_grouped(x, w, c)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        with torch.no_grad():
+            want, slack, end = grouped64(x, w, counts)
+            near(y, want, dtype, slack * (K + 4) * U)
+            assert (y[end:] == 0).all() and (dx[end:] == 0).all()
+            wx, sx, _ = grouped64(dy, w.transpose(1, 2), counts)
+            near(dx, wx, dtype, sx * (N + 4) * U)
+            for i, (a, b) in enumerate(bounds_of(counts, rows)[0]):
+                d, v = dy[a:b].double(), x[a:b].double()
+                near(dw[i], d.t() @ v, dtype, (d.abs().t() @ v.abs()) * (b - a + 4) * U)
+            # another output type, an output whose tail stays as it was
+            near(trk.matmul_grouped(x, w, c, out_dtype=F32), want, F32, slack * (K + 4) * U)
+            out = torch.full((rows, N + 3), 9.0, device=gpu, dtype=dtype)
+            trk.matmul_grouped(x, w, c, out=out[:, 1:-2])
+            assert torch.equal(out[:end, 1:-2], y[:end]) and (out[end:] == 9).all()
+            assert (out[:, 0] == 9).all() and (out[:, -2:] == 9).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("counts", COUNTS, ids=lambda c: f"{len(c)}g{sum(c)}")
+def test_matmul_grouped_fp8(trk, gpu, counts, block):
+    g = gen_of(gpu, len(counts), sum(counts), 1)
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    total = sum(max(0, v) for v in counts)
+    for (N, K), rows in zip(DIMS + [(300, 384)], (total, total + 3, total, total + 140, total if total < 900 else 400,
+                                                   total + 1, total)):
+        x, sx = codes_of(g, rows, K, 1, gpu)
+        w, sw = codes_of(g, N, K, block, gpu, (len(counts),))
+        xv, wv = widen(x, sx, 1), widen(w, sw, block)
+        want, _, end = grouped64(xv, wv, counts)
+        slack = {t: torch.zeros_like(want) for t in (BF, F32)}
+        for i, (a, b) in enumerate(bounds_of(counts, rows)[0]):
+            for t in slack:
+                slack[t][a:b] = product_slack(xv[a:b], wv[i], sx.shape[1], t)
+        for dtype in (BF, F32):
+            y = trk.matmul_grouped(x, w, c, x_scale=sx, w_scale=sw, out_dtype=dtype)
+            near(y, want, dtype, slack[dtype] + want.abs() * 2 * U)
+            assert (y[end:] == 0).all()
+        out = torch.full((rows, N), 9.0, device=gpu, dtype=BF)
+        trk.matmul_grouped(x, w, c, x_scale=sx, w_scale=sw, out=out)
+        assert (out[end:] == 9).all()
+        near(out[:end], want[:end], BF, slack[BF][:end] + want[:end].abs() * 2 * U)
+
+
+@gpu_test
+def test_matmul_grouped_layouts(trk, gpu):
+    """rows and weights inside wider buffers, a weight shared by all groups, a broadcast gradient"""
+    g = gen_of(gpu, 30)
+    counts = [40, 0, 90, 3]
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    bx, bw = (torch.randn(n, 211, device=gpu, generator=g).to(BF) for n in (140, 4 * 60))
+    for a, b in ((0, 128), (1, 70), (8, 200)):
+        x = bx[:133, a:b].requires_grad_()
+        w = bw.view(4, 60, 211)[:, 5:, a:b].detach().requires_grad_()
+        y = trk.matmul_grouped(x, w, c)
+        dx, dw = torch.autograd.grad(y.sum(), (x, w))
+        y2 = trk.matmul_grouped(x.contiguous(), w.contiguous(), c)
+        dx2, dw2 = torch.autograd.grad(y2, (x, w), torch.ones_like(y2))
+        want, slack, _ = grouped64(x.detach(), w.detach(), counts)
+        near(y.detach(), want, BF, slack * (b - a + 4) * U)
+        for p, q in ((dx, dx2), (dw, dw2)):
+            assert torch.equal(p, q)
+        bx = bx.detach()
+    one = bw[:55, :64].expand(4, 55, 64)
+    want, slack, _ = grouped64(bx[:133, :64], one, counts)
+    near(trk.matmul_grouped(bx[:133, :64], one, c), want, BF, slack * 68 * U)
+
+
+@gpu_test
+def test_grouped_gradient_against_differences(trk, gpu):
+    g = gen_of(gpu, 31)
+    counts = [3, 0, 5]
+    x = torch.randn(9, 24, device=gpu, generator=g).to(BF).requires_grad_()
+    w = torch.randn(3, 20, 24, device=gpu, generator=g).to(BF).requires_grad_()
+    dy = torch.randn(9, 20, device=gpu, generator=g).to(BF)
+    got = torch.autograd.grad(trk.matmul_grouped(x, w, torch.tensor(counts, device=gpu, dtype=torch.int32)), (x, w), dy)
+    args = [x.detach().double(), w.detach().double()]
+    for k, i in ((0, 0), (0, 100), (0, 8 * 24 + 3), (1, 5), (1, 480 + 7), (1, 960 + 100)):
+        lo, hi = ([t.clone() for t in args] for _ in range(2))
+        lo[k].view(-1)[i] -= 0.5
+        hi[k].view(-1)[i] += 0.5
+        d = float(((grouped64(*hi, counts)[0] - grouped64(*lo, counts)[0]) * dy.double()).sum())  # linear: exact
+        assert abs(float(got[k].reshape(-1)[i]) - d) <= abs(d) * HALF[BF] * 1.001 + 1e-5
+
+
+# ---------------------------------------------------------------------------------------- as they are used
+def _chain(trk, x, res, w1, wq, ws, wg, wgs, counts):
+    """norm -> 8-bit layer -> norm with the residual -> each stream's own 8-bit layer"""
+    q, s, h = trk.rms_norm_fp8(x, w1, residual=res)
+    y = trk.matmul_fp8(q, s, wq, ws)
+    q2, s2, h2 = trk.rms_norm_fp8(y, w1, residual=h)
+    return h2, trk.matmul_grouped(q2, wg, counts, x_scale=s2, w_scale=wgs)
+
+
+def _chain_inputs(trk, gpu, seed, rows=300, D=512):
+    g = gen_of(gpu, 40, seed)
+    n = lambda *shape: torch.randn(*shape, device=gpu, generator=g)  # noqa: E731
+    wq, ws = trk.quantize_fp8((n(D, D) / D ** 0.5).to(BF), block_rows=128)
+    wg, wgs = trk.quantize_fp8((n(3, 100, D) / D ** 0.5).to(BF), block_rows=128)
+    return [n(rows, D).to(BF), n(rows, D).to(BF), (1 + 0.1 * n(D)).to(BF), wq, ws, wg, wgs,
+            torch.tensor([rows // 3, 0, rows - rows // 3 - 5], device=gpu, dtype=torch.int32)]
+
+
+@gpu_test
+def test_chain(trk, gpu):
+    a = _chain_inputs(trk, gpu, 0)
+    h2, y = _chain(trk, *a)
+    x, res, w1, wq, ws, wg, wgs, counts = a
+    h, _, n = norm64(x, w1, res, 1e-6)
+    t = n @ widen(wq, ws, 128).t()
+    _, _, n2 = norm64(t, w1, h, 1e-6)
+    want, _, end = grouped64(n2, widen(wg, wgs, 128), counts.tolist())
+    # codes are off by 2^-4 at most, about 2^-5.6 in the root mean square: of a sum of independent products as much
+    assert float((h2.double() - (t + h)).norm() / (t + h).norm()) < 2.0 ** -4
+    assert float((y[:end].double() - want[:end]).norm() / want.norm()) < 2.0 ** -3 and (y[end:] == 0).all()
+
+
+@gpu_test
+def test_chain_captured_and_on_streams(trk, gpu):
+    """captured once and replayed with other inputs and eager work between; two chains on two streams at once"""
+    a, b = _chain_inputs(trk, gpu, 1), _chain_inputs(trk, gpu, 2)
+    want = [[t.clone() for t in _chain(trk, *v)] for v in (a, b)]
+    static = [t.clone() for t in a]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _chain(trk, *static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _chain(trk, *static)
+    for k in (0, 1, 0, 1, 1):
+        for s, v in zip(static, (a, b)[k]):
+            s.copy_(v)
+        graph.replay()
+        eager = _chain(trk, *(a, b)[k])
+        torch.cuda.synchronize()
+        for p, q, e in zip(out, want[k], eager):
+            assert torch.equal(p, q) and torch.equal(e, q)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s, v, w in zip(streams, (a, b), want):
+            with torch.cuda.stream(s):
+                got.append((_chain(trk, *v), w))
+    torch.cuda.synchronize()
+    for g, w in got:
+        assert all(torch.equal(p, q) for p, q in zip(g, w))
+
+
+@gpu_test
+def test_gradients_captured(trk, gpu):
+    """forward and backward in one graph, replayed with other inputs"""
+    g = gen_of(gpu, 41)
+    counts = torch.tensor([20, 0, 45], device=gpu, dtype=torch.int32)
+    sets = [[torch.randn(*s, device=gpu, generator=g).to(BF) for s in ((70, 96), (96,), (3, 64, 96), (70, 64))]
+            for _ in range(2)]
+    static = [t.clone() for t in sets[0]]
+
+    def step(x, w, wg, dy):
+        x, w, wg = (t.detach().requires_grad_() for t in (x, w, wg))
+        y = trk.matmul_grouped(trk.rms_norm(x, w), wg, counts)
+        return (y,) + torch.autograd.grad(y, (x, w, wg), dy)
+
+    want = [[t.clone() for t in step(*v)] for v in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static)
+    for k in (1, 0, 1, 0):
+        for s, v in zip(static, sets[k]):
+            s.copy_(v)
+        graph.replay()
+        eager = step(*sets[k])
+        torch.cuda.synchronize()
+        for p, q, e in zip(out, want[k], eager):
+            assert torch.equal(p, q) and torch.equal(e, q)
+
+
+@gpu_test
+def test_long_offsets(trk, gpu):
+    """rows whose byte offsets pass 32 bits: the last rows of 5 GB of codes"""
+    M, K = 2_500_000, 2048
+    x = torch.zeros(M, K, device=gpu, dtype=torch.uint8).view(FP8)
+    sx = torch.ones(K // 128, M, device=gpu).t()
+    g = gen_of(gpu, 42)
+    tail, st = codes_of(g, 200, K, 1, gpu)
+    w, sw = codes_of(g, 16, K, 1, gpu)
+    x[-200:], sx[-200:] = tail, st
+    y = trk.matmul_fp8(x, sx, w, sw, out_dtype=F32)
+    want = widen(tail, st, 1) @ widen(w, sw, 1).t()
+    near(y[-200:], want, F32, product_slack(widen(tail, st, 1), widen(w, sw, 1), 16))
+    assert (y[:-200] == 0).all()
+    del x, sx, y
+    torch.cuda.empty_cache()
+    z = torch.zeros(1_200_000, 2048, device=gpu, dtype=BF)
+    z[-1] = torch.randn(2048, device=gpu, generator=g).to(BF)
+    y = trk.rms_norm(z)
+    q, s = trk.quantize_fp8(z)
+    _, _, y64 = norm64(z[-1:], None, None, 1e-6)
+    near(y[-1:], y64, BF, y64.abs() * 2.0 ** -18)
+    check_codes(q[-1:], s[-1:], z[-1:].double(), 1)
