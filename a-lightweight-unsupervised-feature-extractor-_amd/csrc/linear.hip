@@ -16,6 +16,14 @@
 
 using namespace trk;
 
+#ifndef TRK_TN
+#define TRK_TN 256
+#define TRK_TM 256
+#define TRK_WN 2
+#define TRK_WM 4
+#define TRK_NB 2
+#endif
+
 namespace {
 
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -318,6 +326,206 @@ __global__ __launch_bounds__(256) void mm_kernel(MmArgs A, int dt) {
   }
 }
 
+// ------------------------------------------------------------------ large tiles
+#define GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
+#define LPTR(p) ((__attribute__((address_space(3))) void*)(p))
+
+// work item `id` of `n` on the XCD that runs it (workgroup id % 8): each XCD gets a contiguous run
+__device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
+  const int64_t per = n / 8, more = n % 8, x = id % 8;
+  return x * per + min(x, more) + id / 8;
+}
+
+// TN x TM tile, WN x WM waves, operands copied straight to LDS (16 bytes a lane) NB - 1 steps
+// ahead in a ring of NB stages.  Rows start at multiples of 16 bytes.
+template <int IN, bool WROW, int TN, int TM, int WN, int WM, int NB>
+__global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt, int64_t ntiles, int64_t mtiles) {
+  constexpr int BT = WN * WM * 64, IT = TN / WN / 16, JT = TM / WM / 16;
+  constexpr int XB = TM * kStep, WB = TN * kStep, SB = is8(IN) ? (TM + TN) * 4 : 0, STAGE = XB + WB + SB;
+  constexpr int LX = TM * 8 / BT, LW = TN * 8 / BT, LS = is8(IN) ? (TM + TN) / BT : 0, LOADS = LX + LW + LS;
+  static_assert(TM * 8 % BT == 0 && TN * 8 % BT == 0 && (TM + TN) % BT == 0 && TM % 64 == 0, "whole loads");
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ int64_t scan[BT / 64][2];
+  __shared__ Tile found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t id = xcd_run(blockIdx.x, ntiles * mtiles);
+  // bands of 8 column tiles, row tiles inside a band one after the other: an XCD's share of the
+  // grid at any time is near square, so its L2 serves most operand reads
+  const int64_t band = id / (8 * mtiles), width = min((int64_t)8, ntiles - band * 8);
+  const int64_t in = id - band * 8 * mtiles, nt = band * 8 + in % width, mt = in / width;
+  Tile T;
+  if (A.counts) {
+    T = find_tile<TM, BT>(A, mt, scan, &found);
+  } else {
+    T.row0 = mt * TM;
+    T.rows = (int)min((int64_t)TM, A.M - T.row0);
+    T.g = 0;
+  }
+  if (T.rows <= 0) return;
+  const int64_t n0 = nt * TN;
+  const int cols = (int)min((int64_t)TN, A.N - n0);
+  const int wn = (wave % WN) * (TN / WN), wm = (wave / WN) * (TM / WM), lr = lane & 15, lg = lane >> 4;
+  const int64_t kbytes = T.g < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
+  const int64_t g = max(0, T.g);
+  const uint8_t* xb = A.x + T.row0 * A.ldx;
+  const uint8_t* wb = A.w + g * A.wg + n0 * A.ldw;
+  const float* sxp = A.sx + T.row0 * A.sx_row;
+  const float* swp = A.sw + g * A.sw_g;
+  const int steps = (int)(kbytes / kStep);
+
+  // a lane's source of each copy: LDS slot p of the operand holds row p / 8, chunk (p % 8) ^ (row % 8);
+  // rows past the end repeat the last one
+  const uint8_t* xsrc[LX];
+  const uint8_t* wsrc[LW];
+  const float* ssrc[LS > 0 ? LS : 1];
+#pragma unroll
+  for (int q = 0; q < LX; ++q) {
+    const int p = q * BT + tid, r = p >> 3;
+    xsrc[q] = xb + min(r, T.rows - 1) * A.ldx + (((p & 7) ^ (r & 7)) << 4);
+  }
+#pragma unroll
+  for (int q = 0; q < LW; ++q) {
+    const int p = q * BT + tid, r = p >> 3;
+    wsrc[q] = wb + min(r, cols - 1) * A.ldw + (((p & 7) ^ (r & 7)) << 4);
+  }
+#pragma unroll
+  for (int q = 0; q < LS; ++q) {  // scales: TM of the rows, then TN of the columns (whole waves of each)
+    const int p = q * BT + tid, r = p - TM;
+    ssrc[q] = p < TM ? sxp + min(p, T.rows - 1) * A.sx_row
+                     : swp + (WROW ? n0 + min(r, cols - 1) : (n0 + min(r, cols - 1)) / 128) * A.sw_row;
+  }
+  auto issue = [&](int kt, uint8_t* d) {
+#pragma unroll
+    for (int q = 0; q < LX; ++q)
+      __builtin_amdgcn_global_load_lds(GPTR(xsrc[q] + (int64_t)kt * kStep), LPTR(d + (q * BT + wave * 64) * 16), 16, 0, 0);
+#pragma unroll
+    for (int q = 0; q < LW; ++q)
+      __builtin_amdgcn_global_load_lds(GPTR(wsrc[q] + (int64_t)kt * kStep), LPTR(d + XB + (q * BT + wave * 64) * 16), 16,
+                                       0, 0);
+#pragma unroll
+    for (int q = 0; q < LS; ++q) {
+      const int64_t kb = (q * BT + wave * 64 < TM ? A.sx_kb : A.sw_kb) * (int64_t)kt;
+      __builtin_amdgcn_global_load_lds(GPTR(ssrc[q] + kb), LPTR(d + XB + WB + (q * BT + wave * 64) * 4), 4, 0, 0);
+    }
+  };
+
+  f4v acc[IT][JT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+#pragma unroll
+    for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
+
+  // One step of stage `st`, after the copies into `nx` (a different stage, so that the compiler lets
+  // them stay in flight across the reads) have been sent.  8 bits: the scaling of one row of tiles
+  // runs on the vector units under the matrix instructions of the next.
+  auto step = [&](const uint8_t* __restrict st, uint8_t* __restrict nx, int kn) __attribute__((always_inline)) {
+    const uint8_t *xs = st, *ws = st + XB;
+    const float* ss = (const float*)(st + XB + WB);
+    if (kn >= 0) issue(kn, nx);
+    Frag<IN> b[JT], a[2];
+    float s[JT];
+    f4v p[2][JT], wr[2];
+#pragma unroll
+    for (int j = 0; j < JT; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
+    a[0] = frag<IN>(ws, wn + lr, lg);
+    if constexpr (is8(IN)) {
+#pragma unroll
+      for (int j = 0; j < JT; ++j) {
+        s[j] = ss[wm + j * 16 + lr];
+        if constexpr (!WROW) s[j] *= ss[TM + wn];  // a wave's columns lie in one block of 128
+      }
+      if constexpr (WROW) wr[0] = *(const f4v*)(ss + TM + wn + lg * 4);
+    }
+    auto add = [&](int i) {
+      if constexpr (is8(IN)) {
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[i][j][e] = fmaf(p[i & 1][j][e], WROW ? s[j] * wr[i & 1][e] : s[j], acc[i][j][e]);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      if (i + 1 < IT) {
+        a[(i + 1) & 1] = frag<IN>(ws, wn + (i + 1) * 16 + lr, lg);
+      }
+#pragma unroll
+      for (int j = 0; j < JT; ++j) {
+        if constexpr (is8(IN)) p[i & 1][j] = mma<IN>(a[i & 1], b[j], f4v{0, 0, 0, 0});
+        else acc[i][j] = mma<IN>(a[i & 1], b[j], acc[i][j]);
+      }
+      if (i > 0) add(i - 1);
+      if constexpr (is8(IN) && WROW) {
+        if (i + 1 < IT) wr[(i + 1) & 1] = *(const f4v*)(ss + TM + wn + (i + 1) * 16 + lg * 4);
+      }
+      if constexpr (is8(IN)) {
+        // order of this part: the next row's reads, then a matrix instruction and the four operations
+        // (eight with scales by column) of the tile before it, in turn
+        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x008, IN == IN_E4M3 ? 1 : 4, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, WROW ? 8 : 4, 0);
+        }
+      }
+    }
+    add(IT - 1);
+  };
+  static_assert(WROW || 128 % (TN / WN) == 0, "a wave's columns lie in one block of 128");
+
+#pragma unroll
+  for (int k = 0; k < NB - 1; ++k)
+    if (k < steps) issue(k, smem + k * STAGE);
+  int at = 0;  // stage of step kt
+  for (int kt = 0; kt < steps; ++kt) {
+    // stage kt has landed (its copies are the oldest; younger stages stay in flight), and every wave is
+    // done with stage kt - 1, whose slot the next copies overwrite
+    if (kt + NB - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (NB - 2)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int last = at == 0 ? NB - 1 : at - 1;  // stage of step kt - 1
+    step(smem + at * STAGE, smem + last * STAGE, kt + NB - 1 < steps ? kt + NB - 1 : -1);
+    at = at + 1 == NB ? 0 : at + 1;
+  }
+  if (steps * kStep < kbytes) {  // the last, partial step: masked loads through registers
+    __syncthreads();
+    const int64_t k = (int64_t)steps * kStep;
+#pragma unroll
+    for (int q = 0; q < LX; ++q) {
+      const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
+      *(uint4*)(smem + p * 16) = load16(xsrc[q] + k, kbytes - k - c * 16);
+    }
+#pragma unroll
+    for (int q = 0; q < LW; ++q) {
+      const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
+      *(uint4*)(smem + XB + p * 16) = load16(wsrc[q] + k, kbytes - k - c * 16);
+    }
+#pragma unroll
+    for (int q = 0; q < LS; ++q) {
+      const int p = q * BT + tid;
+      *(float*)(smem + XB + WB + p * 4) = ssrc[q][(p < TM ? A.sx_kb : A.sw_kb) * steps];
+    }
+    __syncthreads();
+    step(smem, smem + STAGE, -1);
+  }
+#pragma unroll
+  for (int i = 0; i < IT; ++i) {
+    const int n = wn + i * 16 + lg * 4;
+    if (n >= cols) continue;
+    f4v b = {0, 0, 0, 0};
+    if (A.bias && T.g >= 0)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? A.bias[n0 + n + e] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < JT; ++j) {
+      const int m = wm + j * 16 + lr;
+      if (m < T.rows) put4(A.y, dt, (T.row0 + m) * A.ldy + n0 + n, cols - n, acc[i][j] + b);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ gradients (16 bits)
 // Both contract over an index that is not contiguous in memory, so their tiles are turned while
 // they are written to LDS: src is [64 k][128 cols] with row stride ld, LDS gets [col][k].
@@ -456,17 +664,42 @@ int check_mm(const char* what, const MmArgs& A, int64_t item, bool scaled) {
   return TRK_OK;
 }
 
-int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t mtiles, void* stream) {
-  TRK_REQUIRE(mtiles <= 65535, "%s: too many row tiles (%lld)", what, (long long)mtiles);
-  const dim3 grid((unsigned)((A.N + 127) / 128), (unsigned)mtiles);
-  hipStream_t st = (hipStream_t)stream;
-  if (in == IN_E4M3 && dt == TRK_F32 && wrow) mm_kernel<IN_E4M3X, true><<<grid, 256, 0, st>>>(A, dt);
-  else if (in == IN_E4M3 && dt == TRK_F32) mm_kernel<IN_E4M3X, false><<<grid, 256, 0, st>>>(A, dt);
-  else if (in == IN_E4M3 && wrow) mm_kernel<IN_E4M3, true><<<grid, 256, 0, st>>>(A, dt);
-  else if (in == IN_E4M3) mm_kernel<IN_E4M3, false><<<grid, 256, 0, st>>>(A, dt);
-  else if (in == IN_BF16) mm_kernel<IN_BF16, false><<<grid, 256, 0, st>>>(A, dt);
-  else mm_kernel<IN_F16, false><<<grid, 256, 0, st>>>(A, dt);
+// shared memory of a kernel above 64 KB has to be asked for, once for each device and kernel
+template <typename F>
+bool allow_lds(F* f, int bytes) {
+  return hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+}
+
+int row_tiles(const MmArgs& A, int tm) { return (int)(A.counts ? A.M / tm + A.G + 1 : (A.M + tm - 1) / tm); }
+
+template <int IN, bool WROW>
+int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStream_t st) {
+  if (aligned) {
+    constexpr bool small = IN == IN_E4M3X;
+    constexpr int TN = small ? 128 : TRK_TN, TM = small ? 128 : TRK_TM, WN = small ? 2 : TRK_WN, WM = small ? 2 : TRK_WM,
+                  NB = TRK_NB;
+    constexpr int lds = NB * ((TM + TN) * kStep + (is8(IN) ? (TM + TN) * 4 : 0));
+    auto* f = mm_tile_kernel<IN, WROW, TN, TM, WN, WM, NB>;
+    TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
+    const int64_t nt = (A.N + TN - 1) / TN, mt = row_tiles(A, TM);
+    TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
+    f<<<(unsigned)(nt * mt), WN * WM * 64, lds, st>>>(A, dt, nt, mt);
+  } else {
+    const int mt = row_tiles(A, 128);
+    TRK_REQUIRE(mt <= 65535, "%s: too many row tiles (%d)", what, mt);
+    mm_kernel<IN, WROW><<<dim3((unsigned)((A.N + 127) / 128), (unsigned)mt), 256, 0, st>>>(A, dt);
+  }
   return trk::check_launch(what);
+}
+
+int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  const bool al = A.K >= 128 && aligned16_ptr(A.x) && aligned16_ptr(A.w) && A.ldx % 16 == 0 && A.ldw % 16 == 0 && A.wg % 16 == 0;
+  if (in == IN_E4M3 && dt == TRK_F32)
+    return wrow ? launch_tiles<IN_E4M3X, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3X, false>(what, A, dt, al, st);
+  if (in == IN_E4M3) return wrow ? launch_tiles<IN_E4M3, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3, false>(what, A, dt, al, st);
+  if (in == IN_BF16) return launch_tiles<IN_BF16, false>(what, A, dt, al, st);
+  return launch_tiles<IN_F16, false>(what, A, dt, al, st);
 }
 
 }  // namespace
