@@ -47,24 +47,20 @@ _FLOAT = {torch.float32: _lib.TRK_F32, torch.bfloat16: _lib.TRK_BF16, torch.floa
 _HALF = {torch.bfloat16: _lib.TRK_BF16, torch.float16: _lib.TRK_F16}
 
 
-class _on:
-    """The device of the inputs made current for a launch (nothing where it already is)."""
+_device = torch._C._cuda_getDevice
 
-    __slots__ = ("idx", "before")
 
-    def __init__(self, dev: torch.device):
-        self.idx = dev.index
-
-    def __enter__(self):
-        self.before = torch._C._cuda_getDevice()
-        if self.before != self.idx:
-            torch._C._cuda_setDevice(self.idx)
-        return _raw_stream(self.idx)
-
-    def __exit__(self, *exc):
-        if self.before != self.idx:
-            torch._C._cuda_setDevice(self.before)
-        return False
+def _launch(what: str, fn: str, x: torch.Tensor, *args):
+    """lib().fn(*args, stream) on the current stream of x's device, which is made current for the launch"""
+    idx = x.get_device()
+    f = getattr(lib(), fn)
+    if idx == _device():
+        rc = f(*args, _raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = f(*args, _raw_stream(idx))
+    if rc:
+        check(rc, what)
 
 
 def _type(t: torch.Tensor, of: dict, what: str, name: str) -> int:
@@ -75,8 +71,8 @@ def _type(t: torch.Tensor, of: dict, what: str, name: str) -> int:
 
 
 def _same(x: torch.Tensor, t: torch.Tensor, what: str, name: str):
-    _need_gpu(t, what)
-    if t.device != x.device:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == x.get_device()):
+        _need_gpu(t, what)
         raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
 
 
@@ -87,24 +83,27 @@ def _no_grad(what: str, *ts):
                 raise NotImplementedError(f"{what}: the 8-bit form has no gradient; call it under torch.no_grad()")
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """t [.., D] as [R, D] with unit column stride and a row stride >= D (a view where t allows it)"""
+def _rows(t: torch.Tensor):
+    """(t [.., D] as [R, D] with unit column stride and a row stride >= D, that stride); a view where t allows it"""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
-    return t
+    R, D = t.shape
+    if not t.is_contiguous():
+        if (D > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < D):
+            t = t.contiguous()
+        elif R > 1:
+            return t, t.stride(0)
+    return t, D if D else 1
 
 
-def _ld(t: torch.Tensor) -> int:
-    """row stride of a [R, D] from _rows (a single row's is not meaningful)"""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
-def _codes(shape, device):
+def _codes(shape, x):
     """e4m3 codes of `shape`, rows padded to 16 bytes: (tensor, row stride)"""
     ld = (shape[-1] + 15) // 16 * 16
-    q = torch.empty((*shape[:-1], ld), device=device, dtype=FP8)
+    q = x.new_empty((*shape[:-1], ld), dtype=FP8)
     return (q if ld == shape[-1] else q[..., :shape[-1]]), ld
 
 
@@ -131,19 +130,20 @@ def _norm_inputs(what, x, weight, residual, eps):
     return dt
 
 
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 def _norm_forward(dt, x, weight, residual, eps, want_rstd):
-    x2 = _rows(x)
+    x2, ldx = _rows(x)
     R, D = x2.shape
-    r2 = _rows(residual) if residual is not None else None
-    w = weight.contiguous() if weight is not None else None
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
-    rstd = torch.empty(R, device=x.device, dtype=torch.float32) if want_rstd else None
-    with _on(x.device) as st:
-        check(lib().trk_rms_norm(
-            x2.data_ptr(), _ld(x2), r2.data_ptr() if r2 is not None else None, _ld(r2) if r2 is not None else 0,
-            w.data_ptr() if w is not None else None, eps, R, D, dt, y.data_ptr(), D,
-            h.data_ptr() if h is not None else None, D, rstd.data_ptr() if rstd is not None else None, st), "rms_norm")
+    r2, ldr = (None, 0) if residual is None else _rows(residual)
+    w = None if weight is None else weight.contiguous()
+    y = _like(x)
+    h = None if residual is None else _like(x)
+    rstd = x.new_empty(R, dtype=torch.float32) if want_rstd else None
+    _launch("rms_norm", "trk_rms_norm", x, x2.data_ptr(), ldx, _at(r2), ldr, _at(w), eps, R, D, dt, y.data_ptr(), D, _at(h),
+            D, _at(rstd))
     return y, h, rstd
 
 
@@ -163,23 +163,20 @@ class _RmsNorm(torch.autograd.Function):
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:  # only the sum was used
             return dh if need_x else None, None, dh if need_r else None, None, None
-        h2, y2 = _rows(h), _rows(dy)
+        h2, ldh = _rows(h)
+        y2, ldy = _rows(dy)
         R, D = h2.shape
-        e2 = _rows(dh) if dh is not None else None
-        w = weight.contiguous() if weight is not None else None
-        dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+        e2, lde = (None, 0) if dh is None else _rows(dh)
+        w = None if weight is None else weight.contiguous()
+        dx = _like(h)
         part = dw = None
         parts = 1
         if need_w:
             parts = lib().trk_rms_norm_bwd_parts(R, D)
-            part = torch.empty((parts, D), device=h.device, dtype=torch.float32)
-            dw = torch.empty(D, device=h.device, dtype=h.dtype)
-        with _on(h.device) as st:
-            check(lib().trk_rms_norm_bwd(
-                h2.data_ptr(), _ld(h2), w.data_ptr() if w is not None else None, rstd.data_ptr(), y2.data_ptr(), _ld(y2),
-                e2.data_ptr() if e2 is not None else None, _ld(e2) if e2 is not None else 0, R, D, ctx.dt, dx.data_ptr(), D,
-                part.data_ptr() if part is not None else None, parts, dw.data_ptr() if dw is not None else None, st),
-                "rms_norm backward")
+            part = h.new_empty((parts, D), dtype=torch.float32)
+            dw = h.new_empty(D)
+        _launch("rms_norm backward", "trk_rms_norm_bwd", h, h2.data_ptr(), ldh, _at(w), rstd.data_ptr(), y2.data_ptr(), ldy,
+                _at(e2), lde, R, D, ctx.dt, dx.data_ptr(), D, _at(part), parts, _at(dw))
         return dx if need_x else None, dw, dx if need_r else None, None, None
 
 
@@ -205,22 +202,19 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, resi
     what = "rms_norm_fp8"
     dt = _norm_inputs(what, x, weight, residual, eps)
     _no_grad(what, x, weight, residual)
-    x2 = _rows(x)
+    x2, ldx = _rows(x)
     R, D = x2.shape
-    r2 = _rows(residual) if residual is not None else None
-    w = weight.contiguous() if weight is not None else None
-    q, ldq = _codes((R, D), x.device)
-    kb = (D + 127) // 128
-    scale = torch.empty((kb, R), device=x.device, dtype=torch.float32)
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
-    with _on(x.device) as st:
-        check(lib().trk_rms_norm_fp8(
-            x2.data_ptr(), _ld(x2), r2.data_ptr() if r2 is not None else None, _ld(r2) if r2 is not None else 0,
-            w.data_ptr() if w is not None else None, eps, R, D, dt, q.data_ptr(), ldq, scale.data_ptr(), max(R, 1),
-            h.data_ptr() if h is not None else None, D, st), what)
-    s = scale.t()
-    if x.dim() != 2:
-        q, s = q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0], s.unflatten(0, x.shape[:-1]) if x.dim() > 2 else s[0]
+    r2, ldr = (None, 0) if residual is None else _rows(residual)
+    w = None if weight is None else weight.contiguous()
+    q, ldq = _codes((R, D), x)
+    s = torch.empty_strided((R, (D + 127) // 128), (1, max(R, 1)), dtype=torch.float32, device=x.device)
+    h = None if residual is None else _like(x)
+    _launch(what, "trk_rms_norm_fp8", x, x2.data_ptr(), ldx, _at(r2), ldr, _at(w), eps, R, D, dt, q.data_ptr(), ldq,
+            s.data_ptr(), max(R, 1), _at(h), D)
+    if x.dim() > 2:
+        q, s = q.unflatten(0, x.shape[:-1]), s.unflatten(0, x.shape[:-1])
+    elif x.dim() == 1:
+        q, s = q[0], s[0]
     return (q, s) if h is None else (q, s, h)
 
 
@@ -242,16 +236,17 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
     _no_grad(what, x)
     R, D = x.shape[-2:]
     B = x.shape[0] if x.dim() == 3 else 1
-    if (D > 1 and x.stride(-1) != 1) or (R > 1 and x.stride(-2) < D):
+    if not x.is_contiguous() and ((D > 1 and x.stride(-1) != 1) or (R > 1 and x.stride(-2) < D)):
         x = x.contiguous()
     ldx = x.stride(-2) if R > 1 else D
-    q, ldq = _codes(x.shape, x.device)
+    q, ldq = _codes(x.shape, x)
     rb, kb = (R if block_rows == 1 else (R + 127) // 128), (D + 127) // 128
-    scale = torch.empty((*x.shape[:-2], kb, rb), device=x.device, dtype=torch.float32)
-    with _on(x.device) as st:
-        check(lib().trk_quantize_fp8(x.data_ptr(), ldx, x.stride(0) if x.dim() == 3 else 0, B, R, D, block_rows, dt,
-                                     q.data_ptr(), ldq, R * ldq, scale.data_ptr(), max(rb, 1), kb * rb, st), what)
-    return q, scale.transpose(-1, -2)
+    one = (1, max(rb, 1))
+    s = torch.empty_strided((rb, kb) if x.dim() == 2 else (B, rb, kb), one if x.dim() == 2 else (kb * rb, *one),
+                            dtype=torch.float32, device=x.device)
+    _launch(what, "trk_quantize_fp8", x, x.data_ptr(), ldx, x.stride(0) if x.dim() == 3 else 0, B, R, D, block_rows, dt,
+            q.data_ptr(), ldq, R * ldq, s.data_ptr(), max(rb, 1), kb * rb)
+    return q, s
 
 
 # ---------------------------------------------------------------------------------------- products
@@ -263,9 +258,9 @@ def _scales(what, t, name, x, rows, kb, lead=()):
     if t.dtype != torch.float32:
         raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
     few = (rows + 127) // 128
-    if tuple(t.shape) == (*lead, rows, kb):
+    if t.shape == (*lead, rows, kb):
         return 1
-    if tuple(t.shape) == (*lead, few, kb):
+    if t.shape == (*lead, few, kb):
         return 128
     raise ValueError(f"{what}: {name} must be {[*lead, rows, kb]} or {[*lead, few, kb]}, got {list(t.shape)}")
 
@@ -275,7 +270,7 @@ def _out(what, out, out_dtype, x, M, N, default):
         dt = out_dtype or default
         if dt not in _FLOAT:
             raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {dt}")
-        return torch.empty((M, N), device=x.device, dtype=dt)
+        return x.new_empty((M, N), dtype=dt)
     _same(x, out, what, "out")
     _type(out, _FLOAT, what, "out")
     if out_dtype is not None and out.dtype != out_dtype:
@@ -316,33 +311,33 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
             raise ValueError(f"{what}: bias must be float32 [{N}]")
         bias = bias.contiguous()
     y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
-    x, w = _rows(x), _rows(w)
-    with _on(x.device) as st:
-        check(lib().trk_matmul_fp8(
-            x.data_ptr(), _ld(x), x_scale.data_ptr(), *x_scale.stride(), w.data_ptr(), _ld(w), w_scale.data_ptr(),
-            *w_scale.stride(), wb, bias.data_ptr() if bias is not None else None, M, N, K, y.data_ptr(),
-            y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype], st), what)
+    x, ldx = _rows(x)
+    w, ldw = _rows(w)
+    _launch(what, "trk_matmul_fp8", x, x.data_ptr(), ldx, x_scale.data_ptr(), *x_scale.stride(), w.data_ptr(), ldw,
+            w_scale.data_ptr(), *w_scale.stride(), wb, _at(bias), M, N, K, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1),
+            _FLOAT[y.dtype])
     return y
 
 
-def _weights(w: torch.Tensor) -> torch.Tensor:
-    if (w.shape[2] > 1 and w.stride(2) != 1) or (w.shape[1] > 1 and w.stride(1) < w.shape[2]):
-        return w.contiguous()
-    return w
+def _weights(w: torch.Tensor):
+    """(w [G, N, K] with unit column stride, its row stride)"""
+    if not w.is_contiguous() and ((w.shape[2] > 1 and w.stride(2) != 1) or (w.shape[1] > 1 and w.stride(1) < w.shape[2])):
+        w = w.contiguous()
+    return w, w.stride(1) if w.shape[1] > 1 else max(w.shape[2], 1)
 
 
 def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_tail):
-    x, w = _rows(x), _weights(w)
+    x, ldx = _rows(x)
+    w, ldw = _weights(w)
     M, K = x.shape
     G, N = w.shape[:2]
-    sx = (x_scale.data_ptr(), *x_scale.stride()) if x_scale is not None else (None, 0, 0)
-    sw = (w_scale.data_ptr(), w_scale.stride(1), w_scale.stride(2), w_scale.stride(0)) if x_scale is not None else \
-        (None, 0, 0, 0)
-    with _on(x.device) as st:
-        check(lib().trk_matmul_grouped(
-            x.data_ptr(), _ld(x), *sx, w.data_ptr(), w.stride(1) if N > 1 else max(K, 1), w.stride(0), *sw, wb,
-            counts.data_ptr(), G, M, N, K, in_dt, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype],
-            zero_tail, st), what)
+    if x_scale is None:
+        sx, sw = (None, 0, 0), (None, 0, 0, 0)
+    else:
+        sx = (x_scale.data_ptr(), *x_scale.stride())
+        sw = (w_scale.data_ptr(), w_scale.stride(1), w_scale.stride(2), w_scale.stride(0))
+    _launch(what, "trk_matmul_grouped", x, x.data_ptr(), ldx, *sx, w.data_ptr(), ldw, w.stride(0), *sw, wb, counts.data_ptr(),
+            G, M, N, K, in_dt, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype], zero_tail)
     return y
 
 
@@ -351,29 +346,27 @@ class _Grouped(torch.autograd.Function):
     def forward(ctx, x, w, counts, dt, out_dtype):
         ctx.save_for_backward(x, w, counts)
         ctx.dt = dt
-        y = torch.empty((x.shape[0], w.shape[1]), device=x.device, dtype=out_dtype)
+        y = x.new_empty((x.shape[0], w.shape[1]), dtype=out_dtype)
         return _grouped_forward("matmul_grouped", x, None, w, None, 128, counts, dt, y, 1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, w, counts = ctx.saved_tensors
-        x, w = _rows(x), _weights(w)
+        x, ldx = _rows(x)
+        w, ldw = _weights(w)
         M, K = x.shape
         G, N = w.shape[:2]
-        dy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        dy, ldy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
         dx = dw = None
-        with _on(x.device) as st:
-            if ctx.needs_input_grad[0]:
-                dx = torch.empty((M, K), device=x.device, dtype=x.dtype)
-                check(lib().trk_matmul_grouped_dx(
-                    dy.data_ptr(), _ld(dy), w.data_ptr(), w.stride(1) if N > 1 else max(K, 1), w.stride(0),
-                    counts.data_ptr(), G, M, N, K, ctx.dt, dx.data_ptr(), max(K, 1), st), "matmul_grouped backward")
-            if ctx.needs_input_grad[1]:
-                dw = torch.empty((G, N, K), device=x.device, dtype=x.dtype)
-                check(lib().trk_matmul_grouped_dw(
-                    dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), counts.data_ptr(), G, M, N, K, ctx.dt, dw.data_ptr(),
-                    max(K, 1), N * K, st), "matmul_grouped backward")
+        if ctx.needs_input_grad[0]:
+            dx = x.new_empty((M, K))
+            _launch("matmul_grouped backward", "trk_matmul_grouped_dx", x, dy.data_ptr(), ldy, w.data_ptr(), ldw, w.stride(0),
+                    counts.data_ptr(), G, M, N, K, ctx.dt, dx.data_ptr(), max(K, 1))
+        if ctx.needs_input_grad[1]:
+            dw = x.new_empty((G, N, K))
+            _launch("matmul_grouped backward", "trk_matmul_grouped_dw", x, dy.data_ptr(), ldy, x.data_ptr(), ldx,
+                    counts.data_ptr(), G, M, N, K, ctx.dt, dw.data_ptr(), max(K, 1), N * K)
         return dx, dw, None, None, None
 
 
