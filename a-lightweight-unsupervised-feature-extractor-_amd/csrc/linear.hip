@@ -12,6 +12,8 @@
 // two 16x16x32 16-bit matrix instructions a tile).  Which k a lane's bytes hold does not matter
 // as long as both operands agree: a lane of group g = lane / 16 takes the 16-byte chunks g and
 // g + 4 of its row.
+#include <type_traits>
+
 #include "trk_common.h"
 
 using namespace trk;
@@ -125,20 +127,30 @@ __device__ Tile find_tile(const MmArgs& A, int64_t t, int64_t (*scan)[2], Tile* 
 }
 
 // ------------------------------------------------------------------ stores of four columns
-__device__ __forceinline__ void put(void* y, int dt, int64_t at, float v) {
-  if (dt == TRK_F32) ((float*)y)[at] = v;
-  else if (dt == TRK_BF16) ((uint16_t*)y)[at] = f32_to_bf16(v);
+// f(integral_constant) for the output type `dt`
+template <typename F>
+__device__ __forceinline__ void by_type(int dt, F f) {
+  if (dt == TRK_F32) f(std::integral_constant<int, TRK_F32>());
+  else if (dt == TRK_BF16) f(std::integral_constant<int, TRK_BF16>());
+  else f(std::integral_constant<int, TRK_F16>());
+}
+
+template <int DT>
+__device__ __forceinline__ void put(void* y, int64_t at, float v) {
+  if constexpr (DT == TRK_F32) ((float*)y)[at] = v;
+  else if constexpr (DT == TRK_BF16) ((uint16_t*)y)[at] = f32_to_bf16(v);
   else ((_Float16*)y)[at] = (_Float16)v;
 }
 
 // y[at .. at + 3] (`left` of them exist); gfx950 takes the wide store at any alignment
-__device__ __forceinline__ void put4(void* y, int dt, int64_t at, int64_t left, f4v v) {
+template <int DT>
+__device__ __forceinline__ void put4(void* y, int64_t at, int left, f4v v) {
   if (left >= 4) {
-    if (dt == TRK_F32) {
+    if constexpr (DT == TRK_F32) {
       __builtin_memcpy((float*)y + at, &v, 16);
     } else {
       uint2 p;
-      if (dt == TRK_BF16) {
+      if constexpr (DT == TRK_BF16) {
         p = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
       } else {
         p = make_uint2(__builtin_bit_cast(uint32_t, h2v{(_Float16)v[0], (_Float16)v[1]}),
@@ -148,9 +160,33 @@ __device__ __forceinline__ void put4(void* y, int dt, int64_t at, int64_t left, 
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < left) put(y, dt, at + j, v[j]);
+    for (int j = 0; j < 3; ++j)
+      if (j < left) put<DT>(y, at + j, v[j]);
   }
+}
+
+// A wave's IT x JT tiles of 16 x 16: columns wn + 16 i + 4 lg .. + 3 of rows wm + 16 j + lr, of a tile with
+// `rows` rows and `cols` columns at y (row stride ld).  bias: of the tile's columns, or null.
+template <int IT, int JT>
+__device__ __forceinline__ void store_tiles(const f4v (&acc)[IT][JT], void* y, int dt, int64_t at, int64_t ld, int rows,
+                                            int cols, int wn, int wm, int lr, int lg, const float* bias) {
+  by_type(dt, [&](auto t) {
+    constexpr int DT = decltype(t)::value;
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      const int n = wn + i * 16 + lg * 4;
+      if (n >= cols) continue;
+      f4v b = {0, 0, 0, 0};
+      if (bias)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? bias[n + e] : 0.0f;
+#pragma unroll
+      for (int j = 0; j < JT; ++j) {
+        const int m = wm + j * 16 + lr;
+        if (m < rows) put4<DT>(y, at + m * ld + n, cols - n, acc[i][j] + b);
+      }
+    }
+  });
 }
 
 // ------------------------------------------------------------------ one K step of one tile
@@ -310,20 +346,8 @@ __global__ __launch_bounds__(256) void mm_kernel(MmArgs A, int dt) {
       }
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = wn + i * 16 + lg * 4;
-    if (n >= cols) continue;
-    f4v b = {0, 0, 0, 0};
-    if (A.bias && T.g >= 0)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? A.bias[n0 + n + e] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = wm + j * 16 + lr;
-      if (m < T.rows) put4(A.y, dt, (T.row0 + m) * A.ldy + n0 + n, cols - n, acc[i][j] + b);
-    }
-  }
+  store_tiles(acc, A.y, dt, T.row0 * A.ldy + n0, A.ldy, T.rows, cols, wn, wm, lr, lg,
+              A.bias && T.g >= 0 ? A.bias + n0 : nullptr);
 }
 
 // ------------------------------------------------------------------ large tiles
@@ -510,20 +534,8 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
     __syncthreads();
     step(smem, smem + STAGE, -1);
   }
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int n = wn + i * 16 + lg * 4;
-    if (n >= cols) continue;
-    f4v b = {0, 0, 0, 0};
-    if (A.bias && T.g >= 0)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? A.bias[n0 + n + e] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < JT; ++j) {
-      const int m = wm + j * 16 + lr;
-      if (m < T.rows) put4(A.y, dt, (T.row0 + m) * A.ldy + n0 + n, cols - n, acc[i][j] + b);
-    }
-  }
+  store_tiles(acc, A.y, dt, T.row0 * A.ldy + n0, A.ldy, T.rows, cols, wn, wm, lr, lg,
+              A.bias && T.g >= 0 ? A.bias + n0 : nullptr);
 }
 
 // ------------------------------------------------------------------ gradients (16 bits)
@@ -550,20 +562,6 @@ struct GradArgs {
   int64_t ldy, ldx, ldw, wg, ldo, og;  // elements
   int64_t M, N, K, G;
 };
-
-__device__ __forceinline__ void store_tile(const f4v (&acc)[4][4], void* out, int dt, int64_t row0, int rows, int64_t ldo,
-                                           int64_t n0, int cols, int wn, int wm, int lr, int lg) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int n = wn + i * 16 + lg * 4;
-    if (n >= cols) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = wm + j * 16 + lr;
-      if (m < rows) put4(out, dt, (row0 + m) * ldo + n0 + n, cols - n, acc[i][j]);
-    }
-  }
-}
 
 template <int IN>
 __device__ __forceinline__ void mm_tile16(const uint8_t* ws, const uint8_t* xs, f4v (&acc)[4][4], int wn, int wm, int lr,
@@ -615,7 +613,7 @@ __global__ __launch_bounds__(256) void grouped_dx_kernel(GradArgs A, int dt) {
     __syncthreads();
     mm_tile16<IN>(ws, xs, acc, wn, wm, lr, lg);
   }
-  store_tile(acc, A.out, dt, T.row0, T.rows, A.ldo, c0, cols, wn, wm, lr, lg);
+  store_tiles(acc, A.out, dt, T.row0 * A.ldo + c0, A.ldo, T.rows, cols, wn, wm, lr, lg, nullptr);
 }
 
 // dw[g][n][k] = sum over the rows m of group g of dy[m][n] x[m][k]
@@ -646,7 +644,159 @@ __global__ __launch_bounds__(256) void grouped_dw_kernel(GradArgs A, int dt) {
     __syncthreads();
     mm_tile16<IN>(ws, xs, acc, wn, wm, lr, lg);
   }
-  store_tile(acc, (uint16_t*)A.out + g * A.og, dt, n0, nr, A.ldo, k0, kc, wn, wm, lr, lg);
+  store_tiles(acc, A.out, dt, g * A.og + n0 * A.ldo + k0, A.ldo, nr, kc, wn, wm, lr, lg, nullptr);
+}
+
+// ------------------------------------------------------------------ gradients on large tiles
+typedef short s4v __attribute__((ext_vector_type(4)));
+
+// A turned tile keeps its source's order, [64 k][T cols], and is turned while it is read: for 16
+// lanes that name 4 rows x 16 columns (4 lanes of 8 bytes a row) the transposing read returns to
+// lane i the four rows' values of column i.  32-byte pieces of a row are rotated by XOR with
+// the row, so that the 16 rows a wave's read touches spread over the banks.
+__device__ __forceinline__ int turn_of(int row) { return (row & 3) | ((row >> 1) & 4); }
+
+template <int IN, int T>
+__device__ __forceinline__ Frag<IN> frag_turned(const uint8_t* tile, int col0, int lane) {
+  const int j = lane & 15, g = lane >> 4;
+  uint2 h[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = 32 * (q >> 1) + 8 * g + 4 * (q & 1) + (j >> 2);
+    const uint8_t* p = tile + row * (T * 2) + ((((col0 >> 4) ^ turn_of(row))) << 5) + (j & 3) * 8;
+    h[q] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) s4v*)p));
+  }
+  Frag<IN> f;
+  f.set(make_uint4(h[0].x, h[0].y, h[1].x, h[1].y), make_uint4(h[2].x, h[2].y, h[3].x, h[3].y));
+  return f;
+}
+
+// T x T tile of dx (DW false: rows m of one group, columns k, contracted over n) or of dw[g] (rows n,
+// columns k, contracted over the group's rows), 8 waves, copies one step of 64 ahead.
+template <int IN, bool DW>
+__global__ __launch_bounds__(512) void grad_tile_kernel(GradArgs A, int dt, int64_t ctiles, int64_t rtiles) {
+  constexpr int T = 256, BT = 512, WN = 2, WM = 4, IT = T / WN / 16, JT = T / WM / 16;
+  constexpr int XB = T * kStep, STAGE = 2 * XB, L = T * 8 / BT;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  __shared__ int64_t scan[BT / 64][2];
+  __shared__ Tile found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lg = lane >> 4, wn = (wave % WN) * (T / WN), wm = (wave / WN) * (T / WM);
+  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  const int64_t ct = id % ctiles, rt = id / ctiles;
+  const int64_t c0 = ct * T;
+  const int cols = (int)min((int64_t)T, A.K - c0);
+  int64_t row0, steps_of;  // first output row; length of the contraction
+  int rows;
+  const uint16_t *wsrc0, *xsrc0;
+  int64_t wld, xld;
+  uint16_t* out = (uint16_t*)A.out;
+  if constexpr (DW) {
+    const int64_t g = rt / rtiles;
+    int64_t before = 0;
+    for (int64_t i = tid; i < g; i += BT) before += max(0, A.counts[i]);
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
+    if (lane == 0) scan[wave][0] = before;
+    __syncthreads();
+    int64_t first = 0;
+    for (int w = 0; w < BT / 64; ++w) first += scan[w][0];
+    first = min(first, A.M);
+    steps_of = min((int64_t)max(0, A.counts[g]), A.M - first);
+    row0 = (rt % rtiles) * T;
+    rows = (int)min((int64_t)T, A.N - row0);
+    wsrc0 = A.x + first * A.ldx + c0;
+    wld = A.ldx;
+    xsrc0 = A.dy + first * A.ldy + row0;
+    xld = A.ldy;
+    out += g * A.og;
+  } else {
+    MmArgs F{};
+    F.counts = A.counts;
+    F.G = A.G;
+    F.M = A.M;
+    F.zero_tail = 1;
+    const Tile t = find_tile<T, BT>(F, rt, scan, &found);
+    if (t.rows <= 0) return;
+    row0 = t.row0;
+    rows = t.rows;
+    steps_of = t.g < 0 ? 0 : A.N;
+    wsrc0 = A.w + max(0, t.g) * A.wg + c0;
+    wld = A.ldw;
+    xsrc0 = A.dy + row0 * A.ldy;
+    xld = A.ldy;
+  }
+  const int steps = (int)(steps_of / 64);
+  // turned: slot p holds 8 values of row p / 32; columns past the end repeat the last whole-or-part piece
+  const uint16_t *wsrc[L], *xsrc[L];
+#pragma unroll
+  for (int q = 0; q < L; ++q) {
+    const int p = q * BT + tid, r = p >> 5, c = ((((p >> 1) & 15) ^ turn_of(r)) << 4) + (p & 1) * 8;
+    wsrc[q] = wsrc0 + r * wld + min(c, (cols - 1) & ~7);
+    if constexpr (DW) {
+      xsrc[q] = xsrc0 + r * xld + min(c, (rows - 1) & ~7);
+    } else {
+      const int xr = p >> 3;
+      xsrc[q] = xsrc0 + min(xr, rows - 1) * xld + (((p & 7) ^ (xr & 7)) << 3);
+    }
+  }
+  const int64_t wstep = 64 * wld, xstep = DW ? 64 * xld : 64;
+  auto issue = [&](int kt, uint8_t* d) {
+#pragma unroll
+    for (int q = 0; q < L; ++q)
+      __builtin_amdgcn_global_load_lds(GPTR(xsrc[q] + kt * xstep), LPTR(d + (q * BT + wave * 64) * 16), 16, 0, 0);
+#pragma unroll
+    for (int q = 0; q < L; ++q)
+      __builtin_amdgcn_global_load_lds(GPTR(wsrc[q] + kt * wstep), LPTR(d + XB + (q * BT + wave * 64) * 16), 16, 0, 0);
+  };
+  f4v acc[IT][JT];
+#pragma unroll
+  for (int i = 0; i < IT; ++i)
+#pragma unroll
+    for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
+  auto step = [&](const uint8_t* __restrict st, uint8_t* __restrict nx, int kn) __attribute__((always_inline)) {
+    if (kn >= 0) issue(kn, nx);
+    Frag<IN> b[JT], a[2];
+#pragma unroll
+    for (int j = 0; j < JT; ++j) {
+      if constexpr (DW) b[j] = frag_turned<IN, T>(st, wm + j * 16, lane);
+      else b[j] = frag<IN>(st, wm + j * 16 + lr, lg);
+    }
+    a[0] = frag_turned<IN, T>(st + XB, wn, lane);
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+      if (i + 1 < IT) a[(i + 1) & 1] = frag_turned<IN, T>(st + XB, wn + (i + 1) * 16, lane);
+#pragma unroll
+      for (int j = 0; j < JT; ++j) acc[i][j] = mma<IN>(a[i & 1], b[j], acc[i][j]);
+    }
+  };
+  if (steps > 0) issue(0, smem);
+  for (int kt = 0; kt < steps; ++kt) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    step(smem + (kt & 1) * STAGE, smem + (~kt & 1) * STAGE, kt + 1 < steps ? kt + 1 : -1);
+  }
+  const int64_t left = steps_of - (int64_t)steps * 64;
+  if (left > 0) {  // the last, partial step: rows (or columns) of the contraction past the end are zeros
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < L; ++q) {
+      const int p = q * BT + tid;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      *(uint4*)(smem + XB + p * 16) = (p >> 5) < left ? *(const uint4*)(wsrc[q] + steps * wstep) : zero;
+      if constexpr (DW) {
+        *(uint4*)(smem + p * 16) = (p >> 5) < left ? *(const uint4*)(xsrc[q] + steps * xstep) : zero;
+      } else {
+        const int c = (p & 7) ^ ((p >> 3) & 7);
+        *(uint4*)(smem + p * 16) = load16((const uint8_t*)(xsrc[q] + steps * xstep), 2 * (left - c * 8));
+      }
+    }
+    __syncthreads();
+    step(smem, smem + STAGE, -1);
+  }
+  store_tiles(acc, out, dt, row0 * A.ldo + c0, A.ldo, rows, cols, wn, wm, lr, lg, nullptr);
 }
 
 int check_out(const char* what, int dt) {
@@ -664,6 +814,11 @@ int check_mm(const char* what, const MmArgs& A, int64_t item, bool scaled) {
   return TRK_OK;
 }
 
+// gradients: whole 16-byte pieces of every row at multiples of 16 bytes
+bool grad_aligned(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t bg) {
+  return aligned16_ptr(a) && aligned16_ptr(b) && lda % 8 == 0 && ldb % 8 == 0 && bg % 8 == 0;
+}
+
 // shared memory of a kernel above 64 KB has to be asked for, once for each device and kernel
 template <typename F>
 bool allow_lds(F* f, int bytes) {
@@ -671,6 +826,17 @@ bool allow_lds(F* f, int bytes) {
 }
 
 int row_tiles(const MmArgs& A, int tm) { return (int)(A.counts ? A.M / tm + A.G + 1 : (A.M + tm - 1) / tm); }
+
+template <int IN, bool DW>
+int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
+  constexpr int T = 256, lds = 4 * T * kStep;
+  auto* f = grad_tile_kernel<IN, DW>;
+  TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
+  const int64_t ct = (A.K + T - 1) / T, rt = DW ? (A.N + T - 1) / T : 1, n = ct * (DW ? rt * A.G : A.M / T + A.G + 1);
+  TRK_REQUIRE(n < ((int64_t)1 << 31), "%s: too many tiles", what);
+  f<<<(unsigned)n, 512, lds, st>>>(A, dt, ct, rt);
+  return trk::check_launch(what);
+}
 
 template <int IN, bool WROW>
 int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStream_t st) {
@@ -753,6 +919,8 @@ int trk_matmul_grouped_dx(const void* dy, int64_t ldy, const void* w, int64_t ld
   const GradArgs A{(const uint16_t*)dy, nullptr, (const uint16_t*)w, dx, counts, ldy, 0, ldw, wg, ldx, 0, M, N, K, G};
   const dim3 grid((unsigned)((K + 127) / 128), (unsigned)(M / 128 + G + 1));
   hipStream_t st = (hipStream_t)stream;
+  if (grad_aligned(dy, ldy, w, ldw, wg))
+    return dtype == TRK_BF16 ? launch_grad<IN_BF16, false>(what, A, dtype, st) : launch_grad<IN_F16, false>(what, A, dtype, st);
   if (dtype == TRK_BF16) grouped_dx_kernel<IN_BF16><<<grid, 256, 0, st>>>(A, dtype);
   else grouped_dx_kernel<IN_F16><<<grid, 256, 0, st>>>(A, dtype);
   return trk::check_launch(what);
@@ -771,6 +939,8 @@ int trk_matmul_grouped_dw(const void* dy, int64_t ldy, const void* x, int64_t ld
   const GradArgs A{(const uint16_t*)dy, (const uint16_t*)x, nullptr, dw, counts, ldy, ldx, 0, 0, ldw, wg, M, N, K, G};
   const dim3 grid((unsigned)((K + 127) / 128), (unsigned)((N + 127) / 128), (unsigned)G);
   hipStream_t st = (hipStream_t)stream;
+  if (grad_aligned(dy, ldy, x, ldx, 0))
+    return dtype == TRK_BF16 ? launch_grad<IN_BF16, true>(what, A, dtype, st) : launch_grad<IN_F16, true>(what, A, dtype, st);
   if (dtype == TRK_BF16) grouped_dw_kernel<IN_BF16><<<grid, 256, 0, st>>>(A, dtype);
   else grouped_dw_kernel<IN_F16><<<grid, 256, 0, st>>>(A, dtype);
   return trk::check_launch(what);
