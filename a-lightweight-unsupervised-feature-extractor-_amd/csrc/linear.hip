@@ -354,6 +354,17 @@ __global__ __launch_bounds__(256) void mm_kernel(MmArgs A, int dt) {
 #define GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define LPTR(p) ((__attribute__((address_space(3))) void*)(p))
 
+// 16 bytes a lane from base + voff + soff to LDS (lane l of the wave at lds + 16 l)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const uint8_t* base, int64_t bytes) {
+  const uint64_t u = reinterpret_cast<uint64_t>(base);  // the same in every lane
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  const uint32_t n = __builtin_amdgcn_readfirstlane((uint32_t)min(bytes, (int64_t)0xffffffff));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>((uint64_t)hi << 32 | lo), 0, n, 0x00020000);
+}
+__device__ __forceinline__ void to_lds(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t voff, uint32_t soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, LPTR(lds), 16, voff, soff, 0, 0);
+}
+
 // work item `id` of `n` on the XCD that runs it (workgroup id % 8): each XCD gets a contiguous run
 __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
   const int64_t per = n / 8, more = n % 8, x = id % 8;
@@ -365,9 +376,9 @@ __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
 template <int IN, bool WROW, int TN, int TM, int WN, int WM, int NB>
 __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt, int64_t ntiles, int64_t mtiles) {
   constexpr int BT = WN * WM * 64, IT = TN / WN / 16, JT = TM / WM / 16;
-  constexpr int XB = TM * kStep, WB = TN * kStep, SB = is8(IN) ? (TM + TN) * 4 : 0, STAGE = XB + WB + SB;
-  constexpr int LX = TM * 8 / BT, LW = TN * 8 / BT, LS = is8(IN) ? (TM + TN) / BT : 0, LOADS = LX + LW + LS;
-  static_assert(TM * 8 % BT == 0 && TN * 8 % BT == 0 && (TM + TN) % BT == 0 && TM % 64 == 0, "whole loads");
+  constexpr int XB = TM * kStep, WB = TN * kStep, LS = is8(IN) ? (TM + TN + BT - 1) / BT : 0, STAGE = XB + WB + LS * BT * 4;
+  constexpr int LX = TM * 8 / BT, LW = TN * 8 / BT, LOADS = LX + LW + LS;
+  static_assert(TM * 8 % BT == 0 && TN * 8 % BT == 0 && TM % 64 == 0, "whole loads");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int64_t scan[BT / 64][2];
   __shared__ Tile found;
@@ -397,20 +408,20 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
   const float* swp = A.sw + g * A.sw_g;
   const int steps = (int)(kbytes / kStep);
 
-  // a lane's source of each copy: LDS slot p of the operand holds row p / 8, chunk (p % 8) ^ (row % 8);
-  // rows past the end repeat the last one
-  const uint8_t* xsrc[LX];
-  const uint8_t* wsrc[LW];
+  // a lane's source of each copy, from the tile's first row on: LDS slot p of an operand holds row
+  // p / 8, chunk (p % 8) ^ (row % 8); rows past the end repeat the last one
+  const __amdgpu_buffer_rsrc_t xr = rows_at(xb, (T.rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
+  uint32_t xoff[LX], woff[LW];
   const float* ssrc[LS > 0 ? LS : 1];
 #pragma unroll
   for (int q = 0; q < LX; ++q) {
     const int p = q * BT + tid, r = p >> 3;
-    xsrc[q] = xb + min(r, T.rows - 1) * A.ldx + (((p & 7) ^ (r & 7)) << 4);
+    xoff[q] = (uint32_t)(min(r, T.rows - 1) * A.ldx) + (((p & 7) ^ (r & 7)) << 4);
   }
 #pragma unroll
   for (int q = 0; q < LW; ++q) {
     const int p = q * BT + tid, r = p >> 3;
-    wsrc[q] = wb + min(r, cols - 1) * A.ldw + (((p & 7) ^ (r & 7)) << 4);
+    woff[q] = (uint32_t)(min(r, cols - 1) * A.ldw) + (((p & 7) ^ (r & 7)) << 4);
   }
 #pragma unroll
   for (int q = 0; q < LS; ++q) {  // scales: TM of the rows, then TN of the columns (whole waves of each)
@@ -418,18 +429,16 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
     ssrc[q] = p < TM ? sxp + min(p, T.rows - 1) * A.sx_row
                      : swp + (WROW ? n0 + min(r, cols - 1) : (n0 + min(r, cols - 1)) / 128) * A.sw_row;
   }
-  auto issue = [&](int kt, uint8_t* d) {
-#pragma unroll
-    for (int q = 0; q < LX; ++q)
-      __builtin_amdgcn_global_load_lds(GPTR(xsrc[q] + (int64_t)kt * kStep), LPTR(d + (q * BT + wave * 64) * 16), 16, 0, 0);
-#pragma unroll
-    for (int q = 0; q < LW; ++q)
-      __builtin_amdgcn_global_load_lds(GPTR(wsrc[q] + (int64_t)kt * kStep), LPTR(d + XB + (q * BT + wave * 64) * 16), 16,
-                                       0, 0);
-#pragma unroll
-    for (int q = 0; q < LS; ++q) {
-      const int64_t kb = (q * BT + wave * 64 < TM ? A.sx_kb : A.sw_kb) * (int64_t)kt;
-      __builtin_amdgcn_global_load_lds(GPTR(ssrc[q] + kb), LPTR(d + XB + WB + (q * BT + wave * 64) * 4), 4, 0, 0);
+  // copy q of LOADS of step kt into its stage
+  auto copy = [&](int q, int kt, uint8_t* d) __attribute__((always_inline)) {
+    if (q < LX) {
+      to_lds(xr, d + (q * BT + wave * 64) * 16, xoff[q], kt * kStep);
+    } else if (q < LX + LW) {
+      to_lds(wr, d + XB + ((q - LX) * BT + wave * 64) * 16, woff[q - LX], kt * kStep);
+    } else {
+      const int p = q - LX - LW;
+      const int64_t kb = (p * BT + wave * 64 < TM ? A.sx_kb : A.sw_kb) * (int64_t)kt;
+      __builtin_amdgcn_global_load_lds(GPTR(ssrc[p] + kb), LPTR(d + XB + WB + (p * BT + wave * 64) * 4), 4, 0, 0);
     }
   };
 
@@ -439,16 +448,16 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
 #pragma unroll
     for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
 
+  constexpr int PER = (LOADS + IT - 1) / IT;
   // One step of stage `st`, after the copies into `nx` (a different stage, so that the compiler lets
   // them stay in flight across the reads) have been sent.  8 bits: the scaling of one row of tiles
   // runs on the vector units under the matrix instructions of the next.
-  auto step = [&](const uint8_t* __restrict st, uint8_t* __restrict nx, int kn) __attribute__((always_inline)) {
+  auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx, int kn) __attribute__((always_inline)) {
     const uint8_t *xs = st, *ws = st + XB;
     const float* ss = (const float*)(st + XB + WB);
-    if (kn >= 0) issue(kn, nx);
     Frag<IN> b[JT], a[2];
     float s[JT];
-    f4v p[2][JT], wr[2];
+    f4v p[2][JT], sc[2];
 #pragma unroll
     for (int j = 0; j < JT; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
     a[0] = frag<IN>(ws, wn + lr, lg);
@@ -458,7 +467,7 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
         s[j] = ss[wm + j * 16 + lr];
         if constexpr (!WROW) s[j] *= ss[TM + wn];  // a wave's columns lie in one block of 128
       }
-      if constexpr (WROW) wr[0] = *(const f4v*)(ss + TM + wn + lg * 4);
+      if constexpr (WROW) sc[0] = *(const f4v*)(ss + TM + wn + lg * 4);
     }
     auto add = [&](int i) {
       if constexpr (is8(IN)) {
@@ -466,7 +475,7 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
         for (int j = 0; j < JT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            acc[i][j][e] = fmaf(p[i & 1][j][e], WROW ? s[j] * wr[i & 1][e] : s[j], acc[i][j][e]);
+            acc[i][j][e] = fmaf(p[i & 1][j][e], WROW ? s[j] * sc[i & 1][e] : s[j], acc[i][j][e]);
       }
     };
 #pragma unroll
@@ -480,8 +489,15 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
         else acc[i][j] = mma<IN>(a[i & 1], b[j], acc[i][j]);
       }
       if (i > 0) add(i - 1);
+      // the next step's copies, a share with each row of tiles: sent all at once they hold up the
+      // wave's first reads while the memory pipe is full
+      if constexpr (decltype(more)::value) {
+#pragma unroll
+        for (int q = i * PER; q < (i + 1) * PER; ++q)
+          if (q < LOADS) copy(q, kn, nx);
+      }
       if constexpr (is8(IN) && WROW) {
-        if (i + 1 < IT) wr[(i + 1) & 1] = *(const f4v*)(ss + TM + wn + (i + 1) * 16 + lg * 4);
+        if (i + 1 < IT) sc[(i + 1) & 1] = *(const f4v*)(ss + TM + wn + (i + 1) * 16 + lg * 4);
       }
       if constexpr (is8(IN)) {
         // order of this part: the next row's reads, then a matrix instruction and the four operations
@@ -492,6 +508,7 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
           __builtin_amdgcn_sched_group_barrier(0x008, IN == IN_E4M3 ? 1 : 4, 0);
           __builtin_amdgcn_sched_group_barrier(0x002, WROW ? 8 : 4, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(0x010, PER, 0);
       }
     }
     add(IT - 1);
@@ -500,39 +517,46 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
 
 #pragma unroll
   for (int k = 0; k < NB - 1; ++k)
-    if (k < steps) issue(k, smem + k * STAGE);
+    if (k < steps)
+#pragma unroll
+      for (int q = 0; q < LOADS; ++q) copy(q, k, smem + k * STAGE);
   int at = 0;  // stage of step kt
-  for (int kt = 0; kt < steps; ++kt) {
+  const int rest = steps * kStep < kbytes;  // a last, partial step: masked loads through registers
+  for (int kt = 0; kt < steps - (NB - 1); ++kt) {
     // stage kt has landed (its copies are the oldest; younger stages stay in flight), and every wave is
     // done with stage kt - 1, whose slot the next copies overwrite
-    if (kt + NB - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (NB - 2)) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (NB - 2)) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int last = at == 0 ? NB - 1 : at - 1;  // stage of step kt - 1
-    step(smem + at * STAGE, smem + last * STAGE, kt + NB - 1 < steps ? kt + NB - 1 : -1);
+    step(std::true_type(), smem + at * STAGE, smem + (at == 0 ? NB - 1 : at - 1) * STAGE, kt + NB - 1);
     at = at + 1 == NB ? 0 : at + 1;
   }
-  if (steps * kStep < kbytes) {  // the last, partial step: masked loads through registers
-    __syncthreads();
-    const int64_t k = (int64_t)steps * kStep;
+  for (int kt = max(0, steps - (NB - 1)); kt < steps + rest; ++kt) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (kt == steps) {
+      const int64_t k = (int64_t)steps * kStep;
+      uint8_t* d = smem + at * STAGE;
 #pragma unroll
-    for (int q = 0; q < LX; ++q) {
-      const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
-      *(uint4*)(smem + p * 16) = load16(xsrc[q] + k, kbytes - k - c * 16);
-    }
+      for (int q = 0; q < LX; ++q) {
+        const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
+        *(uint4*)(d + p * 16) = load16(xb + xoff[q] + k, kbytes - k - c * 16);
+      }
 #pragma unroll
-    for (int q = 0; q < LW; ++q) {
-      const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
-      *(uint4*)(smem + XB + p * 16) = load16(wsrc[q] + k, kbytes - k - c * 16);
-    }
+      for (int q = 0; q < LW; ++q) {
+        const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
+        *(uint4*)(d + XB + p * 16) = load16(wb + woff[q] + k, kbytes - k - c * 16);
+      }
 #pragma unroll
-    for (int q = 0; q < LS; ++q) {
-      const int p = q * BT + tid;
-      *(float*)(smem + XB + WB + p * 4) = ssrc[q][(p < TM ? A.sx_kb : A.sw_kb) * steps];
+      for (int q = 0; q < LS; ++q) {
+        const int p = q * BT + tid;
+        *(float*)(d + XB + WB + p * 4) = ssrc[q][(p < TM ? A.sx_kb : A.sw_kb) * steps];
+      }
+      __syncthreads();
     }
-    __syncthreads();
-    step(smem, smem + STAGE, -1);
+    step(std::false_type(), smem + at * STAGE, smem, 0);
+    at = at + 1 == NB ? 0 : at + 1;
   }
   store_tiles(acc, A.y, dt, T.row0 * A.ldy + n0, A.ldy, T.rows, cols, wn, wm, lr, lg,
               A.bias && T.g >= 0 ? A.bias + n0 : nullptr);
@@ -844,7 +868,8 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
     constexpr bool small = IN == IN_E4M3X;
     constexpr int TN = small ? 128 : TRK_TN, TM = small ? 128 : TRK_TM, WN = small ? 2 : TRK_WN, WM = small ? 2 : TRK_WM,
                   NB = TRK_NB;
-    constexpr int lds = NB * ((TM + TN) * kStep + (is8(IN) ? (TM + TN) * 4 : 0));
+    constexpr int BT = WN * WM * 64;
+    constexpr int lds = NB * ((TM + TN) * kStep + (is8(IN) ? (TM + TN + BT - 1) / BT * BT * 4 : 0));
     auto* f = mm_tile_kernel<IN, WROW, TN, TM, WN, WM, NB>;
     TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
     const int64_t nt = (A.N + TN - 1) / TN, mt = row_tiles(A, TM);
@@ -860,7 +885,8 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
 
 int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const bool al = A.K >= 128 && aligned16_ptr(A.x) && aligned16_ptr(A.w) && A.ldx % 16 == 0 && A.ldw % 16 == 0 && A.wg % 16 == 0;
+  const bool al = A.K >= 128 && aligned16_ptr(A.x) && aligned16_ptr(A.w) && A.ldx % 16 == 0 && A.ldw % 16 == 0 && A.wg % 16 == 0 &&
+                  A.ldx < (1 << 23) && A.ldw < (1 << 23);  // offsets inside a tile are 32 bits
   if (in == IN_E4M3 && dt == TRK_F32)
     return wrow ? launch_tiles<IN_E4M3X, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3X, false>(what, A, dt, al, st);
   if (in == IN_E4M3) return wrow ? launch_tiles<IN_E4M3, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3, false>(what, A, dt, al, st);
