@@ -509,6 +509,10 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
           __builtin_amdgcn_sched_group_barrier(0x002, WROW ? 8 : 4, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x010, PER, 0);
+      } else {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * JT, 0);
+        __builtin_amdgcn_sched_group_barrier(0x010, PER, 0);
       }
     }
     add(IT - 1);
@@ -680,17 +684,21 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 // the row, so that the 16 rows a wave's read touches spread over the banks.
 __device__ __forceinline__ int turn_of(int row) { return (row & 3) | ((row >> 1) & 4); }
 
+// byte of a turned tile that a lane reads for the 16 columns from col0 on (a multiple of 16) and rows 0 .. 3;
+// the other columns of a wave are at this XOR 32 i, the other rows at constant distances
+template <int T>
+__device__ __forceinline__ uint32_t turned_at(int col0, int lane) {
+  const int j = lane & 15, row = 8 * (lane >> 4) + (j >> 2);
+  return row * (T * 2) + (((col0 >> 4) ^ turn_of(row)) << 5) + (j & 3) * 8;
+}
+
 template <int IN, int T>
-__device__ __forceinline__ Frag<IN> frag_turned(const uint8_t* tile, int col0, int lane) {
-  const int j = lane & 15, g = lane >> 4;
+__device__ __forceinline__ Frag<IN> frag_turned(const uint8_t* tile, uint32_t at) {
   uint2 h[4];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int row = 32 * (q >> 1) + 8 * g + 4 * (q & 1) + (j >> 2);
-    const uint8_t* p = tile + row * (T * 2) + ((((col0 >> 4) ^ turn_of(row))) << 5) + (j & 3) * 8;
-    h[q] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                         (__attribute__((address_space(3))) s4v*)p));
-  }
+  for (int q = 0; q < 4; ++q)
+    h[q] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(
+                                         tile + at + (32 * (q >> 1) + 4 * (q & 1)) * T * 2)));
   Frag<IN> f;
   f.set(make_uint4(h[0].x, h[0].y, h[1].x, h[1].y), make_uint4(h[2].x, h[2].y, h[3].x, h[3].y));
   return f;
@@ -753,72 +761,88 @@ __global__ __launch_bounds__(512) void grad_tile_kernel(GradArgs A, int dt, int6
   }
   const int steps = (int)(steps_of / 64);
   // turned: slot p holds 8 values of row p / 32; columns past the end repeat the last whole-or-part piece
-  const uint16_t *wsrc[L], *xsrc[L];
+  const int64_t wstep = 64 * wld * 2, xstep = DW ? 64 * xld * 2 : kStep;  // bytes a step
+  uint32_t woff[L], xoff[L];
 #pragma unroll
   for (int q = 0; q < L; ++q) {
     const int p = q * BT + tid, r = p >> 5, c = ((((p >> 1) & 15) ^ turn_of(r)) << 4) + (p & 1) * 8;
-    wsrc[q] = wsrc0 + r * wld + min(c, (cols - 1) & ~7);
-    if constexpr (DW) {
-      xsrc[q] = xsrc0 + r * xld + min(c, (rows - 1) & ~7);
-    } else {
-      const int xr = p >> 3;
-      xsrc[q] = xsrc0 + min(xr, rows - 1) * xld + (((p & 7) ^ (xr & 7)) << 3);
-    }
+    woff[q] = (uint32_t)(r * wld + min(c, (cols - 1) & ~7)) * 2;
+    const int xrow = p >> 3;
+    xoff[q] = DW ? (uint32_t)(r * xld + min(c, (rows - 1) & ~7)) * 2
+                 : (uint32_t)(min(xrow, rows - 1) * xld) * 2 + (((p & 7) ^ (xrow & 7)) << 4);
   }
-  const int64_t wstep = 64 * wld, xstep = DW ? 64 * xld : 64;
-  auto issue = [&](int kt, uint8_t* d) {
-#pragma unroll
-    for (int q = 0; q < L; ++q)
-      __builtin_amdgcn_global_load_lds(GPTR(xsrc[q] + kt * xstep), LPTR(d + (q * BT + wave * 64) * 16), 16, 0, 0);
-#pragma unroll
-    for (int q = 0; q < L; ++q)
-      __builtin_amdgcn_global_load_lds(GPTR(wsrc[q] + kt * wstep), LPTR(d + XB + (q * BT + wave * 64) * 16), 16, 0, 0);
+  // copies q and q + L of a step; the bases move with the steps (a group's rows may span more than 4 GB)
+  const uint32_t wat = turned_at<T>(wn, lane), xat = turned_at<T>(wm, lane);
+  const uint8_t *xp = (const uint8_t*)xsrc0, *wp = (const uint8_t*)wsrc0;
+  auto copy = [&](int q, __amdgpu_buffer_rsrc_t xr, __amdgpu_buffer_rsrc_t wr, uint8_t* d) __attribute__((always_inline)) {
+    to_lds(xr, d + (q * BT + wave * 64) * 16, xoff[q], 0);
+    to_lds(wr, d + XB + (q * BT + wave * 64) * 16, woff[q], 0);
   };
   f4v acc[IT][JT];
 #pragma unroll
   for (int i = 0; i < IT; ++i)
 #pragma unroll
     for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
-  auto step = [&](const uint8_t* __restrict st, uint8_t* __restrict nx, int kn) __attribute__((always_inline)) {
-    if (kn >= 0) issue(kn, nx);
+  auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t xr = rows_at(xp, 0x7fffffff), wr = rows_at(wp, 0x7fffffff);
+    uint32_t at = wat, bt = xat;
+    asm volatile("" : "+v"(at), "+v"(bt));  // the addresses are made in the step, not kept across it
     Frag<IN> b[JT], a[2];
 #pragma unroll
     for (int j = 0; j < JT; ++j) {
-      if constexpr (DW) b[j] = frag_turned<IN, T>(st, wm + j * 16, lane);
+      if constexpr (DW) b[j] = frag_turned<IN, T>(st, bt ^ (j << 5));
       else b[j] = frag<IN>(st, wm + j * 16 + lr, lg);
     }
-    a[0] = frag_turned<IN, T>(st + XB, wn, lane);
+    a[0] = frag_turned<IN, T>(st + XB, at);
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if (i + 1 < IT) a[(i + 1) & 1] = frag_turned<IN, T>(st + XB, wn + (i + 1) * 16, lane);
+      if (i + 1 < IT) a[(i + 1) & 1] = frag_turned<IN, T>(st + XB, at ^ ((i + 1) << 5));
 #pragma unroll
       for (int j = 0; j < JT; ++j) acc[i][j] = mma<IN>(a[i & 1], b[j], acc[i][j]);
+      if constexpr (decltype(more)::value) {
+        if (i < L) copy(i, xr, wr, nx);
+      }
     }
   };
-  if (steps > 0) issue(0, smem);
-  for (int kt = 0; kt < steps; ++kt) {
+  static_assert(L <= IT, "two copies with each row of tiles");
+  if (steps > 0) {
+    const __amdgpu_buffer_rsrc_t xr = rows_at(xp, 0x7fffffff), wr = rows_at(wp, 0x7fffffff);
+#pragma unroll
+    for (int q = 0; q < L; ++q) copy(q, xr, wr, smem);
+  }
+  const int64_t left = steps_of - (int64_t)steps * 64;
+  for (int kt = 0; kt < steps - 1; ++kt) {
+    // step kt has landed, and every wave is done with step kt - 1, whose slot the next copies overwrite
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    step(smem + (kt & 1) * STAGE, smem + (~kt & 1) * STAGE, kt + 1 < steps ? kt + 1 : -1);
+    xp += xstep;
+    wp += wstep;
+    step(std::true_type(), smem + (kt & 1) * STAGE, smem + (~kt & 1) * STAGE);
   }
-  const int64_t left = steps_of - (int64_t)steps * 64;
-  if (left > 0) {  // the last, partial step: rows (or columns) of the contraction past the end are zeros
-    __syncthreads();
+  for (int kt = max(0, steps - 1); kt < steps + (left > 0); ++kt) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    uint8_t* d = smem + (kt & 1) * STAGE;
+    if (kt == steps) {  // the last, partial step: rows (or columns) of the contraction past the end are zeros
 #pragma unroll
-    for (int q = 0; q < L; ++q) {
-      const int p = q * BT + tid;
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      *(uint4*)(smem + XB + p * 16) = (p >> 5) < left ? *(const uint4*)(wsrc[q] + steps * wstep) : zero;
-      if constexpr (DW) {
-        *(uint4*)(smem + p * 16) = (p >> 5) < left ? *(const uint4*)(xsrc[q] + steps * xstep) : zero;
-      } else {
-        const int c = (p & 7) ^ ((p >> 3) & 7);
-        *(uint4*)(smem + p * 16) = load16((const uint8_t*)(xsrc[q] + steps * xstep), 2 * (left - c * 8));
+      for (int q = 0; q < L; ++q) {
+        const int p = q * BT + tid;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        *(uint4*)(d + XB + p * 16) = (p >> 5) < left ? *(const uint4*)(wp + woff[q]) : zero;
+        if constexpr (DW) {
+          *(uint4*)(d + p * 16) = (p >> 5) < left ? *(const uint4*)(xp + xoff[q]) : zero;
+        } else {
+          const int c = (p & 7) ^ ((p >> 3) & 7);
+          *(uint4*)(d + p * 16) = load16(xp + xoff[q], 2 * (left - c * 8));
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
-    step(smem, smem + STAGE, -1);
+    step(std::false_type(), d, smem);
+    xp += xstep;
+    wp += wstep;
   }
   store_tiles(acc, out, dt, row0 * A.ldo + c0, A.ldo, rows, cols, wn, wm, lr, lg, nullptr);
 }
@@ -840,7 +864,8 @@ int check_mm(const char* what, const MmArgs& A, int64_t item, bool scaled) {
 
 // gradients: whole 16-byte pieces of every row at multiples of 16 bytes
 bool grad_aligned(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t bg) {
-  return aligned16_ptr(a) && aligned16_ptr(b) && lda % 8 == 0 && ldb % 8 == 0 && bg % 8 == 0;
+  return aligned16_ptr(a) && aligned16_ptr(b) && lda % 8 == 0 && ldb % 8 == 0 && bg % 8 == 0 &&
+         lda < (1 << 22) && ldb < (1 << 22);  // offsets inside a tile are 32 bits
 }
 
 // shared memory of a kernel above 64 KB has to be asked for, once for each device and kernel
