@@ -57,74 +57,107 @@ struct Tile {
   int g;      // group, or -1: rows behind the last group
 };
 
-// The rows of tile `t` (TM rows each, a group's last one shorter), found by all BT threads from
-// the counts: each thread sums a run of groups, the sums are scanned, the thread whose run
-// holds tile t walks it.  Negative counts are 0 and the sum stops at M, so no count reaches
-// past the rows.
+// Which rows a tile (TM rows, a group's last one shorter) has, found by all BT threads from the counts:
+// each thread owns a run of groups; its rows and tiles are summed and scanned once, and the thread
+// whose run holds a tile walks it.  Negative counts are 0 and the sum stops at M, so no count
+// reaches past the rows.
+struct Runs {                 // of a thread: the first row of its groups, their first tile, how many tiles
+  int first, t0, tiles;
+};
+
 template <int TM, int BT>
-__device__ Tile find_tile(const MmArgs& A, int64_t t, int64_t (*scan)[2], Tile* found) {
-  const int tid = threadIdx.x;
-  const int64_t run = (A.G + BT - 1) / BT, g0 = tid * run, g1 = min(A.G, g0 + run);
-  if (tid == 0) *found = Tile{0, 0, 0};
-  int64_t rows = 0;
-  for (int64_t g = g0; g < g1; ++g) rows += max(0, A.counts[g]);
-  // exclusive scan of the rows over the threads
-  const int lane = tid & 63, wave = tid >> 6;
-  int64_t incl = rows;
+struct Finder {
+  int live, end;             // tiles of all groups; rows of all groups
+  int all;                   // tiles, with those of the rows behind the last group
+
+  __device__ __forceinline__ static int scan(int v, int* sums, int& total) {  // exclusive, over the workgroup
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = v;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += o;
-  }
-  if (lane == 63) scan[wave][0] = incl;
-  __syncthreads();
-  int64_t first = incl - rows, total = 0;
-  for (int w = 0; w < BT / 64; ++w) {
-    if (w < wave) first += scan[w][0];
-    total += scan[w][0];
-  }
-  // tiles of this thread's groups, with the rows cut at M
-  int64_t tiles = 0, at = min(first, A.M);
-  for (int64_t g = g0; g < g1; ++g) {
-    const int64_t c = min((int64_t)max(0, A.counts[g]), A.M - at);
-    tiles += (c + TM - 1) / TM;
-    at += c;
-  }
-  incl = tiles;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += o;
+    }
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int before = incl - v;
+    total = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(incl, d, 64);
-    if (lane >= d) incl += o;
+    for (int w = 0; w < BT / 64; ++w) {
+      if (w < wave) before += sums[w];
+      total += sums[w];
+    }
+    __syncthreads();
+    return before;
   }
-  if (lane == 63) scan[wave][1] = incl;
-  __syncthreads();
-  int64_t t0 = incl - tiles, all = 0;
-  for (int w = 0; w < BT / 64; ++w) {
-    if (w < wave) t0 += scan[w][1];
-    all += scan[w][1];
+
+  // saturating: sums of rows stop at M < 2^31 in every step
+  __device__ __forceinline__ static int scan_rows(int v, int* sums, int M, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl = (int)min((int64_t)incl + o, (int64_t)M);
+    }
+    const int excl = __shfl_up(incl, 1, 64);
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int64_t before = lane > 0 ? excl : 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < BT / 64; ++w) {
+      if (w < wave) before += sums[w];
+      all += sums[w];
+    }
+    total = (int)min(all, (int64_t)M);
+    __syncthreads();
+    return (int)min(before, (int64_t)M);
   }
-  if (t >= t0 && t < t0 + tiles) {
-    at = min(first, A.M);
-    int64_t k = t0;
-    for (int64_t g = g0; g < g1; ++g) {
-      const int64_t c = min((int64_t)max(0, A.counts[g]), A.M - at);
-      const int64_t n = (c + TM - 1) / TM;
-      if (t < k + n) {
-        const int64_t o = (t - k) * TM;
-        *found = Tile{at + o, (int)min((int64_t)TM, c - o), (int)g};
-        break;
-      }
-      k += n;
+
+  // groups are fewer than 2^16, rows fewer than 2^31
+  __device__ void init(const int32_t* counts, int G, int64_t M, bool tail, int* sums, Runs* runs) {
+    const int run = (G + BT - 1) / BT, g0 = min(G, (int)threadIdx.x * run), g1 = min(G, g0 + run);
+    int64_t rows = 0;
+    for (int g = g0; g < g1; ++g) rows = min(rows + max(0, counts[g]), M);
+    Runs r;
+    r.first = scan_rows((int)rows, sums, (int)M, end);
+    r.tiles = 0;
+    int64_t at = r.first;
+    for (int g = g0; g < g1; ++g) {
+      const int64_t c = min((int64_t)max(0, counts[g]), M - at);
+      r.tiles += (int)((c + TM - 1) / TM);
       at += c;
     }
+    r.t0 = scan(r.tiles, sums, live);
+    runs[threadIdx.x] = r;
+    all = live + (tail ? (int)((M - end + TM - 1) / TM) : 0);
   }
-  if (tid == 0 && t >= all && A.zero_tail) {
-    const int64_t end = min(total, A.M), o = end + (t - all) * TM;
-    if (o < A.M) *found = Tile{o, (int)min((int64_t)TM, A.M - o), -1};
+
+  // one thread writes the rows of tile t < all
+  __device__ void find(const int32_t* counts, int G, int64_t M, int t, const Runs* runs, Tile* found) const {
+    const Runs r = runs[threadIdx.x];
+    if (t >= r.t0 && t < r.t0 + r.tiles) {
+      const int run = (G + BT - 1) / BT, g0 = (int)threadIdx.x * run, g1 = min(G, g0 + run);
+      int64_t at = r.first;
+      int k = r.t0;
+      for (int g = g0; g < g1; ++g) {
+        const int64_t c = min((int64_t)max(0, counts[g]), M - at);
+        const int n = (int)((c + TM - 1) / TM);
+        if (t < k + n) {
+          const int64_t o = (int64_t)(t - k) * TM;
+          *found = Tile{at + o, (int)min((int64_t)TM, c - o), g};
+          break;
+        }
+        k += n;
+        at += c;
+      }
+    }
+    if (threadIdx.x == 0 && t >= live) {
+      const int64_t o = end + (int64_t)(t - live) * TM;
+      *found = Tile{o, (int)min((int64_t)TM, M - o), -1};
+    }
   }
-  __syncthreads();
-  return *found;
-}
+};
 
 // ------------------------------------------------------------------ stores of four columns
 // f(integral_constant) for the output type `dt`
@@ -142,6 +175,14 @@ __device__ __forceinline__ void put(void* y, int64_t at, float v) {
   else ((_Float16*)y)[at] = (_Float16)v;
 }
 
+template <int DT>
+__device__ __forceinline__ uint2 pack4(f4v v) {
+  if constexpr (DT == TRK_BF16) return make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+  else
+    return make_uint2(__builtin_bit_cast(uint32_t, h2v{(_Float16)v[0], (_Float16)v[1]}),
+                      __builtin_bit_cast(uint32_t, h2v{(_Float16)v[2], (_Float16)v[3]}));
+}
+
 // y[at .. at + 3] (`left` of them exist); gfx950 takes the wide store at any alignment
 template <int DT>
 __device__ __forceinline__ void put4(void* y, int64_t at, int left, f4v v) {
@@ -149,13 +190,7 @@ __device__ __forceinline__ void put4(void* y, int64_t at, int left, f4v v) {
     if constexpr (DT == TRK_F32) {
       __builtin_memcpy((float*)y + at, &v, 16);
     } else {
-      uint2 p;
-      if constexpr (DT == TRK_BF16) {
-        p = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
-      } else {
-        p = make_uint2(__builtin_bit_cast(uint32_t, h2v{(_Float16)v[0], (_Float16)v[1]}),
-                       __builtin_bit_cast(uint32_t, h2v{(_Float16)v[2], (_Float16)v[3]}));
-      }
+      const uint2 p = pack4<DT>(v);
       __builtin_memcpy((uint16_t*)y + at, &p, 8);
     }
   } else {
@@ -167,23 +202,52 @@ __device__ __forceinline__ void put4(void* y, int64_t at, int left, f4v v) {
 
 // A wave's IT x JT tiles of 16 x 16: columns wn + 16 i + 4 lg .. + 3 of rows wm + 16 j + lr, of a tile with
 // `rows` rows and `cols` columns at y (row stride ld).  bias: of the tile's columns, or null.
+// 16-bit rows: lanes of odd and even lg swap halves of two neighbouring column tiles, so that a lane
+// stores 8 columns (16 bytes) and a row of the pair is one run of 64 bytes.
 template <int IT, int JT>
 __device__ __forceinline__ void store_tiles(const f4v (&acc)[IT][JT], void* y, int dt, int64_t at, int64_t ld, int rows,
                                             int cols, int wn, int wm, int lr, int lg, const float* bias) {
+  asm volatile("" : "+v"(lr), "+v"(lg));  // addresses are made here, not kept through the loops before
   by_type(dt, [&](auto t) {
     constexpr int DT = decltype(t)::value;
-#pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int n = wn + i * 16 + lg * 4;
-      if (n >= cols) continue;
+    typedef std::conditional_t<DT == TRK_F32, float, uint16_t> E;
+    E* tile = (E*)y + at;
+    auto column_bias = [&](int i) {
       f4v b = {0, 0, 0, 0};
+      const int n = wn + i * 16 + lg * 4;
       if (bias)
 #pragma unroll
         for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? bias[n + e] : 0.0f;
+      return b;
+    };
+    if (DT != TRK_F32 && wn + IT * 16 <= cols) {  // the wave's columns are all there
+      if constexpr (DT != TRK_F32) {
 #pragma unroll
-      for (int j = 0; j < JT; ++j) {
-        const int m = wm + j * 16 + lr;
-        if (m < rows) put4<DT>(y, at + m * ld + n, cols - n, acc[i][j] + b);
+        for (int i = 0; i < IT; i += 2) {
+          const f4v b0 = column_bias(i), b1 = column_bias(i + 1);
+#pragma unroll
+          for (int j = 0; j < JT; ++j) {
+            const uint2 p = pack4<DT>(acc[i][j] + b0), q = pack4<DT>(acc[i + 1][j] + b1);
+            typedef unsigned u2 __attribute__((ext_vector_type(2)));
+            const u2 x = __builtin_amdgcn_permlane16_swap(p.x, q.x, false, false);
+            const u2 z = __builtin_amdgcn_permlane16_swap(p.y, q.y, false, false);
+            const uint4 o = make_uint4(x[0], z[0], x[1], z[1]);
+            const int m = wm + j * 16 + lr;
+            if (m < rows) __builtin_memcpy(tile + m * ld + wn + (i + (lg & 1)) * 16 + (lg >> 1) * 8, &o, 16);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int n = wn + i * 16 + lg * 4;
+        if (n >= cols) continue;
+        const f4v b = column_bias(i);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          const int m = wm + j * 16 + lr;
+          if (m < rows) put4<DT>(tile, m * ld + n, cols - n, acc[i][j] + b);
+        }
       }
     }
   });
@@ -276,20 +340,25 @@ template <int IN, bool WROW>
 __global__ __launch_bounds__(256) void mm_kernel(MmArgs A, int dt) {
   constexpr int TM = 128, TN = 128;
   __shared__ uint4 smem[(TM + TN) * kStep / 16];
-  __shared__ int64_t scan[4][2];
+  __shared__ int sums[4];
+  __shared__ Runs runs[256];
   __shared__ Tile found;
   uint8_t* xs = (uint8_t*)smem;
   uint8_t* ws = xs + TM * kStep;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Tile T;
   if (A.counts) {
-    T = find_tile<TM, 256>(A, blockIdx.y, scan, &found);
+    Finder<TM, 256> F;
+    F.init(A.counts, (int)A.G, A.M, A.zero_tail, sums, runs);
+    if (blockIdx.y >= F.all) return;
+    F.find(A.counts, (int)A.G, A.M, blockIdx.y, runs, &found);
+    __syncthreads();
+    T = found;
   } else {
     T.row0 = (int64_t)blockIdx.y * TM;
     T.rows = (int)min((int64_t)TM, A.M - T.row0);
     T.g = 0;
   }
-  if (T.rows <= 0) return;
   const int64_t n0 = (int64_t)blockIdx.x * TN;
   const int cols = (int)min((int64_t)TN, A.N - n0);
   const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
@@ -371,70 +440,87 @@ __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
   return x * per + min(x, more) + id / 8;
 }
 
-// TN x TM tile, WN x WM waves, operands copied straight to LDS (16 bytes a lane) NB - 1 steps
-// ahead in a ring of NB stages.  Rows start at multiples of 16 bytes.
+// TN x TM tiles, WN x WM waves, operands copied straight to LDS (16 bytes a lane) NB - 1 steps ahead in
+// a ring of NB stages.  Rows start at multiples of 16 bytes.  A workgroup runs several tiles: the
+// next tile's first copies are sent before a tile's stores.
 template <int IN, bool WROW, int TN, int TM, int WN, int WM, int NB>
-__global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt, int64_t ntiles, int64_t mtiles) {
+__global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int dt, int ntiles, int mtiles) {
   constexpr int BT = WN * WM * 64, IT = TN / WN / 16, JT = TM / WM / 16;
   constexpr int XB = TM * kStep, WB = TN * kStep, LS = is8(IN) ? (TM + TN + BT - 1) / BT : 0, STAGE = XB + WB + LS * BT * 4;
-  constexpr int LX = TM * 8 / BT, LW = TN * 8 / BT, LOADS = LX + LW + LS;
+  constexpr int LX = TM * 8 / BT, LW = TN * 8 / BT, LOADS = LX + LW + LS, PER = (LOADS + IT - 1) / IT;
   static_assert(TM * 8 % BT == 0 && TN * 8 % BT == 0 && TM % 64 == 0, "whole loads");
+  static_assert(WROW || 128 % (TN / WN) == 0, "a wave's columns lie in one block of 128");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  __shared__ int64_t scan[BT / 64][2];
+  __shared__ int sums[BT / 64];
+  __shared__ Runs runs[BT];
   __shared__ Tile found;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t id = xcd_run(blockIdx.x, ntiles * mtiles);
-  // bands of 8 column tiles, row tiles inside a band one after the other: an XCD's share of the
-  // grid at any time is near square, so its L2 serves most operand reads
-  const int64_t band = id / (8 * mtiles), width = min((int64_t)8, ntiles - band * 8);
-  const int64_t in = id - band * 8 * mtiles, nt = band * 8 + in % width, mt = in / width;
-  Tile T;
-  if (A.counts) {
-    T = find_tile<TM, BT>(A, mt, scan, &found);
-  } else {
-    T.row0 = mt * TM;
-    T.rows = (int)min((int64_t)TM, A.M - T.row0);
-    T.g = 0;
-  }
-  if (T.rows <= 0) return;
-  const int64_t n0 = nt * TN;
-  const int cols = (int)min((int64_t)TN, A.N - n0);
   const int wn = (wave % WN) * (TN / WN), wm = (wave / WN) * (TM / WM), lr = lane & 15, lg = lane >> 4;
-  const int64_t kbytes = T.g < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
-  const int64_t g = max(0, T.g);
-  const uint8_t* xb = A.x + T.row0 * A.ldx;
-  const uint8_t* wb = A.w + g * A.wg + n0 * A.ldw;
-  const float* sxp = A.sx + T.row0 * A.sx_row;
-  const float* swp = A.sw + g * A.sw_g;
-  const int steps = (int)(kbytes / kStep);
+  Finder<TM, BT> F;
+  if (A.counts) {
+    F.init(A.counts, (int)A.G, A.M, A.zero_tail, sums, runs);
+    mtiles = __builtin_amdgcn_readfirstlane(F.all);
+  }
+  const int64_t total = (int64_t)ntiles * mtiles;
 
-  // a lane's source of each copy, from the tile's first row on: LDS slot p of an operand holds row
-  // p / 8, chunk (p % 8) ^ (row % 8); rows past the end repeat the last one
-  const __amdgpu_buffer_rsrc_t xr = rows_at(xb, (T.rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
-  uint32_t xoff[LX], woff[LW];
+  // the tile that is worked on: its rows, columns and sources
+  int64_t row0, n0;
+  int rows, cols, grp, steps, rest;
+  int64_t kbytes;
+  const uint8_t *xb, *wb;
+  uint32_t x0, w0, xend, wend;  // a lane's first piece of its operand's rows, and its piece of the last row
   const float* ssrc[LS > 0 ? LS : 1];
+  auto tile_at = [&](int64_t idx, int& nt, int& mt) {
+    // bands of 8 column tiles, row tiles inside a band one after the other: an XCD's share of the
+    // grid at any time is near square, so its L2 serves most operand reads
+    const int id = (int)xcd_run(idx, total), bsize = 8 * mtiles, band = id / bsize, in = id - band * bsize;
+    const int width = min(8, ntiles - band * 8);
+    nt = band * 8 + in % width;
+    mt = in / width;
+  };
+  auto setup = [&](int nt, int mt) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (as in store_tiles)
+    if (A.counts) {
+      row0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)found.row0);  // rows are below 2^31
+      rows = __builtin_amdgcn_readfirstlane(found.rows);
+      grp = __builtin_amdgcn_readfirstlane(found.g);
+    } else {
+      row0 = (int64_t)mt * TM;
+      rows = (int)min((int64_t)TM, A.M - row0);
+      grp = 0;
+    }
+    n0 = (int64_t)nt * TN;
+    cols = (int)min((int64_t)TN, A.N - n0);
+    kbytes = grp < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
+    steps = (int)(kbytes / kStep);
+    rest = steps * kStep < kbytes;  // a last, partial step: masked loads through registers
+    const int64_t g = max(0, grp);
+    xb = A.x + row0 * A.ldx;
+    wb = A.w + g * A.wg + n0 * A.ldw;
+    // LDS slot p of an operand holds row p / 8, chunk (p % 8) ^ (row % 8): a lane's q-th copy is of row
+    // tid / 8 + q BT / 8; rows past the end repeat the last one
+    const uint32_t c = ((tid & 7) ^ ((tid >> 3) & 7)) << 4;
+    x0 = (uint32_t)(tid >> 3) * (uint32_t)A.ldx + c;
+    w0 = (uint32_t)(tid >> 3) * (uint32_t)A.ldw + c;
+    xend = (uint32_t)(rows - 1) * (uint32_t)A.ldx + c;
+    wend = (uint32_t)(cols - 1) * (uint32_t)A.ldw + c;
 #pragma unroll
-  for (int q = 0; q < LX; ++q) {
-    const int p = q * BT + tid, r = p >> 3;
-    xoff[q] = (uint32_t)(min(r, T.rows - 1) * A.ldx) + (((p & 7) ^ (r & 7)) << 4);
-  }
-#pragma unroll
-  for (int q = 0; q < LW; ++q) {
-    const int p = q * BT + tid, r = p >> 3;
-    woff[q] = (uint32_t)(min(r, cols - 1) * A.ldw) + (((p & 7) ^ (r & 7)) << 4);
-  }
-#pragma unroll
-  for (int q = 0; q < LS; ++q) {  // scales: TM of the rows, then TN of the columns (whole waves of each)
-    const int p = q * BT + tid, r = p - TM;
-    ssrc[q] = p < TM ? sxp + min(p, T.rows - 1) * A.sx_row
-                     : swp + (WROW ? n0 + min(r, cols - 1) : (n0 + min(r, cols - 1)) / 128) * A.sw_row;
-  }
+    for (int q = 0; q < LS; ++q) {  // scales: TM of the rows, then TN of the columns (whole waves of each)
+      const int p = q * BT + tid, r = p - TM;
+      ssrc[q] = p < TM ? A.sx + (row0 + min(p, rows - 1)) * A.sx_row
+                       : A.sw + g * A.sw_g + (WROW ? n0 + min(r, cols - 1) : (n0 + min(r, cols - 1)) / 128) * A.sw_row;
+    }
+  };
+  auto xoff = [&](int q) { return min(x0 + (uint32_t)(q * (BT / 8)) * (uint32_t)A.ldx, xend); };
+  auto woff = [&](int q) { return min(w0 + (uint32_t)(q * (BT / 8)) * (uint32_t)A.ldw, wend); };
   // copy q of LOADS of step kt into its stage
-  auto copy = [&](int q, int kt, uint8_t* d) __attribute__((always_inline)) {
+  auto copy = [&](int q, int kt, uint8_t* d, __amdgpu_buffer_rsrc_t xr, __amdgpu_buffer_rsrc_t wr)
+      __attribute__((always_inline)) {
     if (q < LX) {
-      to_lds(xr, d + (q * BT + wave * 64) * 16, xoff[q], kt * kStep);
+      to_lds(xr, d + (q * BT + wave * 64) * 16, xoff(q), kt * kStep);
     } else if (q < LX + LW) {
-      to_lds(wr, d + XB + ((q - LX) * BT + wave * 64) * 16, woff[q - LX], kt * kStep);
+      to_lds(wr, d + XB + ((q - LX) * BT + wave * 64) * 16, woff(q - LX), kt * kStep);
     } else {
       const int p = q - LX - LW;
       const int64_t kb = (p * BT + wave * 64 < TM ? A.sx_kb : A.sw_kb) * (int64_t)kt;
@@ -443,16 +529,11 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
   };
 
   f4v acc[IT][JT];
-#pragma unroll
-  for (int i = 0; i < IT; ++i)
-#pragma unroll
-    for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
-
-  constexpr int PER = (LOADS + IT - 1) / IT;
-  // One step of stage `st`, after the copies into `nx` (a different stage, so that the compiler lets
-  // them stay in flight across the reads) have been sent.  8 bits: the scaling of one row of tiles
-  // runs on the vector units under the matrix instructions of the next.
-  auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx, int kn) __attribute__((always_inline)) {
+  // One step of stage `st`; the copies go into `nx` (a different stage, so that the compiler lets
+  // them stay in flight across the reads).  8 bits: the scaling of one row of tiles runs on the
+  // vector units under the matrix instructions of the next.
+  auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx, int kn, __amdgpu_buffer_rsrc_t xr,
+                  __amdgpu_buffer_rsrc_t wr) __attribute__((always_inline)) {
     const uint8_t *xs = st, *ws = st + XB;
     const float* ss = (const float*)(st + XB + WB);
     Frag<IN> b[JT], a[2];
@@ -480,9 +561,7 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
     };
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
-      if (i + 1 < IT) {
-        a[(i + 1) & 1] = frag<IN>(ws, wn + (i + 1) * 16 + lr, lg);
-      }
+      if (i + 1 < IT) a[(i + 1) & 1] = frag<IN>(ws, wn + (i + 1) * 16 + lr, lg);
 #pragma unroll
       for (int j = 0; j < JT; ++j) {
         if constexpr (is8(IN)) p[i & 1][j] = mma<IN>(a[i & 1], b[j], f4v{0, 0, 0, 0});
@@ -494,7 +573,7 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
       if constexpr (decltype(more)::value) {
 #pragma unroll
         for (int q = i * PER; q < (i + 1) * PER; ++q)
-          if (q < LOADS) copy(q, kn, nx);
+          if (q < LOADS) copy(q, kn, nx, xr, wr);
       }
       if constexpr (is8(IN) && WROW) {
         if (i + 1 < IT) sc[(i + 1) & 1] = *(const f4v*)(ss + TM + wn + (i + 1) * 16 + lg * 4);
@@ -517,53 +596,90 @@ __global__ __launch_bounds__(WN * WM * 64) void mm_tile_kernel(MmArgs A, int dt,
     }
     add(IT - 1);
   };
-  static_assert(WROW || 128 % (TN / WN) == 0, "a wave's columns lie in one block of 128");
-
+  auto first_copies = [&](int at) {
+    const __amdgpu_buffer_rsrc_t xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
 #pragma unroll
-  for (int k = 0; k < NB - 1; ++k)
-    if (k < steps)
+    for (int k = 0; k < NB - 1; ++k) {
+      if (k < steps)
 #pragma unroll
-      for (int q = 0; q < LOADS; ++q) copy(q, k, smem + k * STAGE);
-  int at = 0;  // stage of step kt
-  const int rest = steps * kStep < kbytes;  // a last, partial step: masked loads through registers
-  for (int kt = 0; kt < steps - (NB - 1); ++kt) {
-    // stage kt has landed (its copies are the oldest; younger stages stay in flight), and every wave is
-    // done with stage kt - 1, whose slot the next copies overwrite
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (NB - 2)) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    step(std::true_type(), smem + at * STAGE, smem + (at == 0 ? NB - 1 : at - 1) * STAGE, kt + NB - 1);
-    at = at + 1 == NB ? 0 : at + 1;
-  }
-  for (int kt = max(0, steps - (NB - 1)); kt < steps + rest; ++kt) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    if (kt == steps) {
-      const int64_t k = (int64_t)steps * kStep;
-      uint8_t* d = smem + at * STAGE;
-#pragma unroll
-      for (int q = 0; q < LX; ++q) {
-        const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
-        *(uint4*)(d + p * 16) = load16(xb + xoff[q] + k, kbytes - k - c * 16);
-      }
-#pragma unroll
-      for (int q = 0; q < LW; ++q) {
-        const int p = q * BT + tid, c = (p & 7) ^ ((p >> 3) & 7);
-        *(uint4*)(d + XB + p * 16) = load16(wb + woff[q] + k, kbytes - k - c * 16);
-      }
-#pragma unroll
-      for (int q = 0; q < LS; ++q) {
-        const int p = q * BT + tid;
-        *(float*)(d + XB + WB + p * 4) = ssrc[q][(p < TM ? A.sx_kb : A.sw_kb) * steps];
-      }
-      __syncthreads();
+        for (int q = 0; q < LOADS; ++q) copy(q, k, smem + (at + k >= NB ? at + k - NB : at + k) * STAGE, xr, wr);
     }
-    step(std::false_type(), smem + at * STAGE, smem, 0);
-    at = at + 1 == NB ? 0 : at + 1;
+  };
+
+  int64_t idx = blockIdx.x;
+  if (idx >= total) return;
+  int nt, mt, at = 0;  // at: the stage of the step
+  tile_at(idx, nt, mt);
+  if (A.counts) {
+    F.find(A.counts, (int)A.G, A.M, mt, runs, &found);
+    __syncthreads();
   }
-  store_tiles(acc, A.y, dt, T.row0 * A.ldy + n0, A.ldy, T.rows, cols, wn, wm, lr, lg,
-              A.bias && T.g >= 0 ? A.bias + n0 : nullptr);
+  setup(nt, mt);
+  first_copies(at);
+  while (true) {
+    {
+      const __amdgpu_buffer_rsrc_t xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+#pragma unroll
+        for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
+      for (int kt = 0; kt < steps - (NB - 1); ++kt) {
+        // stage kt has landed (its copies are the oldest; younger stages stay in flight), and every wave
+        // is done with stage kt - 1, whose slot the next copies overwrite
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (NB - 2)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        step(std::true_type(), smem + at * STAGE, smem + (at == 0 ? NB - 1 : at - 1) * STAGE, kt + NB - 1, xr, wr);
+        at = at + 1 == NB ? 0 : at + 1;
+      }
+      for (int kt = max(0, steps - (NB - 1)); kt < steps + rest; ++kt) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (kt == steps) {
+          int t = tid;
+          asm volatile("" : "+v"(t));  // (as in store_tiles)
+          const int64_t k = (int64_t)steps * kStep;
+          uint8_t* d = smem + at * STAGE;
+#pragma unroll
+          for (int q = 0; q < LX; ++q) {
+            const int p = q * BT + t, c = (p & 7) ^ ((p >> 3) & 7);
+            *(uint4*)(d + p * 16) = load16(xb + xoff(q) + k, kbytes - k - c * 16);
+          }
+#pragma unroll
+          for (int q = 0; q < LW; ++q) {
+            const int p = q * BT + t, c = (p & 7) ^ ((p >> 3) & 7);
+            *(uint4*)(d + XB + p * 16) = load16(wb + woff(q) + k, kbytes - k - c * 16);
+          }
+#pragma unroll
+          for (int q = 0; q < LS; ++q) {
+            const int p = q * BT + t;
+            *(float*)(d + XB + WB + p * 4) = ssrc[q][(p < TM ? A.sx_kb : A.sw_kb) * steps];
+          }
+          __syncthreads();
+        }
+        step(std::false_type(), smem + at * STAGE, smem, 0, xr, wr);
+        at = at + 1 == NB ? 0 : at + 1;
+      }
+    }
+    const int64_t y0 = row0 * A.ldy + n0;
+    const float* bias = A.bias && grp >= 0 ? A.bias + n0 : nullptr;
+    const int yrows = rows, ycols = cols;
+    idx += gridDim.x;
+    const bool more = idx < total;
+    if (more) {
+      tile_at(idx, nt, mt);
+      if (A.counts) F.find(A.counts, (int)A.G, A.M, mt, runs, &found);
+      // every wave is done with the last step's stage (and `found` is written)
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      setup(nt, mt);
+      first_copies(at);
+    }
+    store_tiles(acc, A.y, dt, y0, A.ldy, yrows, ycols, wn, wm, lr, lg, bias);
+    if (!more) break;
+  }
 }
 
 // ------------------------------------------------------------------ gradients (16 bits)
@@ -610,18 +726,18 @@ template <int IN>
 __global__ __launch_bounds__(256) void grouped_dx_kernel(GradArgs A, int dt) {
   constexpr int TM = 128;
   __shared__ uint4 smem[2 * 128 * kStep / 16];
-  __shared__ int64_t scan[4][2];
+  __shared__ int sums[4];
+  __shared__ Runs runs[256];
   __shared__ Tile found;
   uint8_t* xs = (uint8_t*)smem;
   uint8_t* ws = xs + 128 * kStep;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  MmArgs F{};
-  F.counts = A.counts;
-  F.G = A.G;
-  F.M = A.M;
-  F.zero_tail = 1;
-  const Tile T = find_tile<TM, 256>(F, blockIdx.y, scan, &found);
-  if (T.rows <= 0) return;
+  Finder<TM, 256> F;
+  F.init(A.counts, (int)A.G, A.M, true, sums, runs);
+  if (blockIdx.y >= F.all) return;
+  F.find(A.counts, (int)A.G, A.M, blockIdx.y, runs, &found);
+  __syncthreads();
+  const Tile T = found;
   const int64_t c0 = (int64_t)blockIdx.x * 128;
   const int cols = (int)min((int64_t)128, A.K - c0);
   const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
@@ -711,11 +827,19 @@ __global__ __launch_bounds__(512) void grad_tile_kernel(GradArgs A, int dt, int6
   constexpr int T = 256, BT = 512, WN = 2, WM = 4, IT = T / WN / 16, JT = T / WM / 16;
   constexpr int XB = T * kStep, STAGE = 2 * XB, L = T * 8 / BT;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  __shared__ int64_t scan[BT / 64][2];
+  __shared__ int sums[BT / 64];
+  __shared__ Runs runs[BT];
   __shared__ Tile found;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4, wn = (wave % WN) * (T / WN), wm = (wave / WN) * (T / WM);
-  const int64_t id = xcd_run(blockIdx.x, gridDim.x);
+  Finder<T, BT> F;
+  if constexpr (!DW) {
+    F.init(A.counts, (int)A.G, A.M, true, sums, runs);
+    rtiles = F.all;
+  }
+  const int64_t total = ctiles * rtiles * (DW ? A.G : 1);
+  if (blockIdx.x >= total) return;
+  const int64_t id = xcd_run(blockIdx.x, total);
   const int64_t ct = id % ctiles, rt = id / ctiles;
   const int64_t c0 = ct * T;
   const int cols = (int)min((int64_t)T, A.K - c0);
@@ -727,14 +851,10 @@ __global__ __launch_bounds__(512) void grad_tile_kernel(GradArgs A, int dt, int6
   if constexpr (DW) {
     const int64_t g = rt / rtiles;
     int64_t before = 0;
-    for (int64_t i = tid; i < g; i += BT) before += max(0, A.counts[i]);
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
-    if (lane == 0) scan[wave][0] = before;
-    __syncthreads();
-    int64_t first = 0;
-    for (int w = 0; w < BT / 64; ++w) first += scan[w][0];
-    first = min(first, A.M);
+    for (int64_t i = tid; i < g; i += BT) before = min(before + max(0, A.counts[i]), A.M);
+    int end;
+    Finder<T, BT>::scan_rows((int)before, sums, (int)A.M, end);
+    const int64_t first = end;
     steps_of = min((int64_t)max(0, A.counts[g]), A.M - first);
     row0 = (rt % rtiles) * T;
     rows = (int)min((int64_t)T, A.N - row0);
@@ -744,13 +864,9 @@ __global__ __launch_bounds__(512) void grad_tile_kernel(GradArgs A, int dt, int6
     xld = A.ldy;
     out += g * A.og;
   } else {
-    MmArgs F{};
-    F.counts = A.counts;
-    F.G = A.G;
-    F.M = A.M;
-    F.zero_tail = 1;
-    const Tile t = find_tile<T, BT>(F, rt, scan, &found);
-    if (t.rows <= 0) return;
+    F.find(A.counts, (int)A.G, A.M, (int)rt, runs, &found);
+    __syncthreads();
+    const Tile t = found;
     row0 = t.row0;
     rows = t.rows;
     steps_of = t.g < 0 ? 0 : A.N;
@@ -899,7 +1015,11 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
     TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
     const int64_t nt = (A.N + TN - 1) / TN, mt = row_tiles(A, TM);
     TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
-    f<<<(unsigned)(nt * mt), WN * WM * 64, lds, st>>>(A, dt, nt, mt);
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+      cus = 256;
+    const int64_t grid = std::min<int64_t>(nt * mt, (int64_t)cus * (small ? 2 : 1) / 8 * 8);
+    f<<<(unsigned)grid, WN * WM * 64, lds, st>>>(A, dt, (int)nt, (int)mt);
   } else {
     const int mt = row_tiles(A, 128);
     TRK_REQUIRE(mt <= 65535, "%s: too many row tiles (%d)", what, mt);
