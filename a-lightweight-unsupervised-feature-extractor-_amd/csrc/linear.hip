@@ -588,11 +588,8 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
           __builtin_amdgcn_sched_group_barrier(0x002, WROW ? 8 : 4, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x010, PER, 0);
-      } else {
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * JT, 0);
-        __builtin_amdgcn_sched_group_barrier(0x010, PER, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);  // rows of tiles stay in this order
     }
     add(IT - 1);
   };
@@ -918,6 +915,7 @@ __global__ __launch_bounds__(512) void grad_tile_kernel(GradArgs A, int dt, int6
       if constexpr (decltype(more)::value) {
         if (i < L) copy(i, xr, wr, nx);
       }
+      __builtin_amdgcn_sched_barrier(0);  // rows of tiles stay in this order
     }
   };
   static_assert(L <= IT, "two copies with each row of tiles");
