@@ -136,6 +136,19 @@ struct NormArgs {
   float eps;
 };
 
+// 448 / top as a sum of two f32, so that v * (448 / top) is rounded once (to within 2^-40): values that
+// lie halfway between two codes, common among 16-bit inputs, stay there and go to the even one.  An
+// infinite top gives 0 (and NaN for the infinity itself).
+struct Ratio {
+  float hi, lo;
+  __device__ __forceinline__ explicit Ratio(float top) {
+    hi = kTop / top;
+    const float rest = fmaf(-hi, top, kTop);  // exact
+    lo = top < INFINITY ? rest / top : 0.0f;
+  }
+  __device__ __forceinline__ float operator*(float v) const { return fmaf(v, hi, v * lo); }
+};
+
 // quantise the 8 values a lane holds of its 128-column block (16 consecutive lanes)
 __device__ __forceinline__ void quant8(const float (&v)[kV], uint8_t* q, int64_t col, int64_t D, int64_t ldq,
                                        float* scale) {
@@ -143,10 +156,10 @@ __device__ __forceinline__ void quant8(const float (&v)[kV], uint8_t* q, int64_t
 #pragma unroll
   for (int j = 0; j < kV; ++j) top = fmaxf(top, fabsf(v[j]));
   top = fmaxf(max_lanes<16>(top), kLeast);
-  const float inv = kTop / top;
+  const Ratio inv(top);
   float t[kV];
 #pragma unroll
-  for (int j = 0; j < kV; ++j) t[j] = v[j] * inv;
+  for (int j = 0; j < kV; ++j) t[j] = inv * v[j];
   const int64_t pad = (D + 15) / 16 * 16;
   const int64_t room = (ldq >= pad ? pad : D) - col;  // the row's padding (to 16 bytes) is written as zeros
   if (room > 0) store8_e4m3(q + col, D - col, room, pack8_e4m3(t));
@@ -307,19 +320,24 @@ __global__ __launch_bounds__(BT) void rms_norm_bwd_kernel(BwdArgs A) {
   }
 }
 
-// dw[c] = sum over parts of part[p][c]: 64 columns x 4 part slices a workgroup, joined in order
+// dw[c] = sum over parts of part[p][c]: 16 columns x 16 slices of the parts a workgroup, joined in
+// order.  (64 columns x 4 slices took 63 us for 1024 parts of 512 columns: 8 workgroups, 256 loads
+// one after the other.)
 template <int DT>
 __global__ __launch_bounds__(256) void dw_sum_kernel(const float* part, int64_t parts, int64_t D, void* dw) {
-  __shared__ float s[4][64];
-  const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int k = threadIdx.x >> 6;
+  __shared__ float s[16][17];
+  const int x = threadIdx.x & 15, k = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + x;
   float a = 0.0f;
-  if (c < D)
-    for (int64_t p = k; p < parts; p += 4) a += part[p * D + c];
-  s[k][threadIdx.x & 63] = a;
+  if (c < D) {
+#pragma unroll 8
+    for (int64_t p = k; p < parts; p += 16) a += part[p * D + c];
+  }
+  s[k][x] = a;
   __syncthreads();
   if (k == 0 && c < D) {
-    for (int o = 1; o < 4; ++o) a += s[o][threadIdx.x];
+#pragma unroll
+    for (int o = 1; o < 16; ++o) a += s[o][x];
     ((typename El<DT>::T*)dw)[c] = from_f<DT>(a);
   }
 }
@@ -367,7 +385,7 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(QuantArgs A) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
   __syncthreads();
   top = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), kLeast);
-  const float inv = kTop / top;
+  const Ratio inv(top);
   const int64_t pad = (A.D + 15) / 16 * 16;
   const int64_t room = (A.ldq >= pad ? pad : A.D) - c;
 #pragma unroll
@@ -375,7 +393,7 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(QuantArgs A) {
     const int64_t row = rb * 128 + i * 16 + (threadIdx.x >> 4);
     if (row >= A.R || room <= 0) continue;
 #pragma unroll
-    for (int j = 0; j < kV; ++j) v[i][j] *= inv;
+    for (int j = 0; j < kV; ++j) v[i][j] = inv * v[i][j];
     store8_e4m3(A.q + b * A.qb + row * A.ldq + c, A.D - c, room, pack8_e4m3(v[i]));
   }
   if (threadIdx.x == 0) A.scale[b * A.sb + blk * A.sld + rb] = top / kTop;
@@ -415,7 +433,7 @@ void launch_bwd(const BwdArgs& A, hipStream_t st) {
   else if (D <= 8192) TRK_BWD(256, 4, false);
   else TRK_BWD(256, 4, true);
 #undef TRK_BWD
-  if (A.dw) dw_sum_kernel<DT><<<(unsigned)((D + 63) / 64), 256, 0, st>>>(A.part, A.parts, D, A.dw);
+  if (A.dw) dw_sum_kernel<DT><<<(unsigned)((D + 15) / 16), 256, 0, st>>>(A.part, A.parts, D, A.dw);
 }
 
 bool float_type(int dt) { return dt == TRK_F32 || dt == TRK_BF16 || dt == TRK_F16; }
@@ -486,7 +504,7 @@ int trk_rms_norm_bwd(const void* h, int64_t ldh, const void* weight, const float
                   R > 0 ? bwd_parts(R, D) : 0};
   if (R == 0) {
     if (!dw) return TRK_OK;
-#define CALL(DT) dw_sum_kernel<DT><<<(unsigned)((D + 63) / 64), 256, 0, st>>>(part, 0, D, dw)
+#define CALL(DT) dw_sum_kernel<DT><<<(unsigned)((D + 15) / 16), 256, 0, st>>>(part, 0, D, dw)
     TRK_BY_TYPE(dtype, CALL);
 #undef CALL
   } else {
