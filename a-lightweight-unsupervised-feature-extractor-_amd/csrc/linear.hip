@@ -679,6 +679,123 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   }
 }
 
+// ------------------------------------------------------------------ few rows
+// 16 JT rows by 16 columns a wave, the operands straight from memory to registers: with few rows the
+// weights are read once and that is what counts.  KW waves of the 8 share 16 columns, each with
+// every KW-th step, and are joined in order through LDS; the others take the next columns.
+// U steps are loaded before they are multiplied.  Any alignment.
+template <int IN, bool WROW, int JT, int KW>
+__global__ __launch_bounds__(512) void mm_few_kernel(MmArgs A, int dt) {
+  constexpr int TM = 16 * JT, NW = 8 / KW, U = JT >= 4 || IN == IN_E4M3X ? 2 : 4;
+  __shared__ f4v part[8][JT][64];
+  __shared__ int sums[8];
+  __shared__ Runs runs[512];
+  __shared__ Tile found;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lg = lane >> 4, kw = wave % KW;
+  const int64_t n0 = ((int64_t)blockIdx.x * NW + wave / KW) * 16;
+  int64_t row0 = (int64_t)blockIdx.y * TM;
+  int rows, g = 0;
+  if (A.counts) {
+    Finder<TM, 512> F;
+    F.init(A.counts, (int)A.G, A.M, A.zero_tail, sums, runs);
+    if (blockIdx.y >= F.all) return;
+    F.find(A.counts, (int)A.G, A.M, blockIdx.y, runs, &found);
+    __syncthreads();
+    row0 = found.row0;
+    rows = __builtin_amdgcn_readfirstlane(found.rows);
+    g = __builtin_amdgcn_readfirstlane(found.g);
+  } else {
+    rows = (int)min((int64_t)TM, A.M - row0);
+  }
+  const int cols = (int)min((int64_t)16, A.N - n0);  // may be <= 0: this wave only takes part in the barrier
+  const int64_t kbytes = g < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
+  const int steps = (int)((kbytes + kStep - 1) / kStep);
+  f4v acc[JT];
+#pragma unroll
+  for (int j = 0; j < JT; ++j) acc[j] = f4v{0, 0, 0, 0};
+  if (cols > 0) {
+    const int64_t gw = max(0, g);
+    const uint8_t* wp = A.w + gw * A.wg + (n0 + min(lr, cols - 1)) * A.ldw + lg * 16;
+    const uint8_t* xp[JT];
+    const float* sx[JT];
+#pragma unroll
+    for (int j = 0; j < JT; ++j) {
+      const int64_t r = row0 + min(j * 16 + lr, rows - 1);
+      xp[j] = A.x + r * A.ldx + lg * 16;
+      sx[j] = A.sx + r * A.sx_row;
+    }
+    const float* sw = A.sw + gw * A.sw_g;
+    const float* swr[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) swr[e] = sw + (WROW ? n0 + min(lg * 4 + e, cols - 1) : n0 / 128) * A.sw_row;
+    for (int k0 = kw; k0 < steps; k0 += KW * U) {
+      uint4 a[U][2], b[U][JT][2];
+      float s[U][JT], w[U][WROW ? 4 : 1];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int kt = k0 + u * KW;
+        if (kt >= steps) break;
+        const int64_t k = (int64_t)kt * kStep, left = kbytes - k - lg * 16;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) a[u][h] = load16(wp + k + h * 64, left - h * 64);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) b[u][j][h] = load16(xp[j] + k + h * 64, left - h * 64);
+          if constexpr (is8(IN)) s[u][j] = sx[j][kt * A.sx_kb];
+        }
+        if constexpr (is8(IN)) {
+#pragma unroll
+          for (int e = 0; e < (WROW ? 4 : 1); ++e) w[u][e] = swr[e][kt * A.sw_kb];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k0 + u * KW >= steps) break;
+        Frag<IN> fa;
+        fa.set(a[u][0], a[u][1]);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          Frag<IN> fb;
+          fb.set(b[u][j][0], b[u][j][1]);
+          if constexpr (is8(IN)) {
+            const f4v p = mma<IN>(fa, fb, f4v{0, 0, 0, 0});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(p[e], s[u][j] * w[u][WROW ? e : 0], acc[j][e]);
+          } else {
+            acc[j] = mma<IN>(fa, fb, acc[j]);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (KW > 1) {
+    if (kw > 0)
+#pragma unroll
+      for (int j = 0; j < JT; ++j) part[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int o = 1; o < KW; ++o)
+#pragma unroll
+      for (int j = 0; j < JT; ++j) acc[j] += part[wave + o][j][lane];
+  }
+  const int n = lg * 4;
+  if (n >= cols) return;
+  f4v bias = {0, 0, 0, 0};
+  if (A.bias && g >= 0)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bias[e] = n + e < cols ? A.bias[n0 + n + e] : 0.0f;
+  by_type(dt, [&](auto t) {
+#pragma unroll
+    for (int j = 0; j < JT; ++j) {
+      const int m = j * 16 + lr;
+      if (m < rows) put4<decltype(t)::value>(A.y, (row0 + m) * A.ldy + n0 + n, cols - n, acc[j] + bias);
+    }
+  });
+}
+
 // ------------------------------------------------------------------ gradients (16 bits)
 // Both contract over an index that is not contiguous in memory, so their tiles are turned while
 // they are written to LDS: src is [64 k][128 cols] with row stride ld, LDS gets [col][k].
@@ -1001,9 +1118,26 @@ int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
   return trk::check_launch(what);
 }
 
+template <int IN, bool WROW, int JT>
+void launch_few(const MmArgs& A, int dt, hipStream_t st) {
+  const int64_t strips = (A.N + 15) / 16, mt = row_tiles(A, 16 * JT), steps = (A.K * (is8(IN) ? 1 : 2) + kStep - 1) / kStep;
+  int kw = 8;  // waves that share 16 columns: enough for 2048 waves in all, no more than there are steps
+  while (kw > 1 && (strips * mt * (kw / 2) >= 2048 || kw > steps)) kw /= 2;
+  const dim3 grid((unsigned)((strips + 8 / kw - 1) / (8 / kw)), (unsigned)mt);
+  if (kw == 8) mm_few_kernel<IN, WROW, JT, 8><<<grid, 512, 0, st>>>(A, dt);
+  else if (kw == 4) mm_few_kernel<IN, WROW, JT, 4><<<grid, 512, 0, st>>>(A, dt);
+  else if (kw == 2) mm_few_kernel<IN, WROW, JT, 2><<<grid, 512, 0, st>>>(A, dt);
+  else mm_few_kernel<IN, WROW, JT, 1><<<grid, 512, 0, st>>>(A, dt);
+}
+
 template <int IN, bool WROW>
 int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStream_t st) {
-  if (aligned) {
+  const int64_t each = A.counts ? (A.M + A.G - 1) / A.G : A.M;  // rows of a group
+  if (each <= 64 && row_tiles(A, 16) <= 65535) {
+    if (each <= 16) launch_few<IN, WROW, 1>(A, dt, st);
+    else if (each <= 32) launch_few<IN, WROW, 2>(A, dt, st);
+    else launch_few<IN, WROW, 4>(A, dt, st);
+  } else if (aligned) {
     constexpr bool small = IN == IN_E4M3X;
     constexpr int TN = small ? 128 : TRK_TN, TM = small ? 128 : TRK_TM, WN = small ? 2 : TRK_WN, WM = small ? 2 : TRK_WM,
                   NB = TRK_NB;
