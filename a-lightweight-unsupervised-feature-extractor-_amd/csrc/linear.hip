@@ -200,10 +200,26 @@ __device__ __forceinline__ void put4(void* y, int64_t at, int left, f4v v) {
   }
 }
 
+// A wave's 16-byte pieces of two 64-byte runs of its 16 rows, a of columns 0 .. and b of the columns
+// behind them: rows 8 .. 15 of a and 0 .. 7 of b change places, so that a holds rows 0 .. 7 of both
+// runs and b rows 8 .. 15.  One store then writes 8 whole 128-byte lines and not 16 halves.
+__device__ __forceinline__ void pair_lines(uint4& a, uint4& b, bool low) {
+  auto turn = [&](uint32_t& u, uint32_t& v) {
+    const uint32_t t = low ? v : u;  // what the other half needs
+    const uint32_t r = __builtin_amdgcn_mov_dpp(t, 0x128, 0xf, 0xf, false);  // from the lane 8 further in its 16
+    (low ? v : u) = r;
+  };
+  turn(a.x, b.x);
+  turn(a.y, b.y);
+  turn(a.z, b.z);
+  turn(a.w, b.w);
+}
+
 // A wave's IT x JT tiles of 16 x 16: columns wn + 16 i + 4 lg .. + 3 of rows wm + 16 j + lr, of a tile with
 // `rows` rows and `cols` columns at y (row stride ld).  bias: of the tile's columns, or null.
 // 16-bit rows: lanes of odd and even lg swap halves of two neighbouring column tiles, so that a lane
-// stores 8 columns (16 bytes) and a row of the pair is one run of 64 bytes.
+// has 8 columns (16 bytes) and the pair a run of 64 bytes a row, as one tile has in 32 bits; two such
+// runs are then paired to lines.
 template <int IT, int JT>
 __device__ __forceinline__ void store_tiles(const f4v (&acc)[IT][JT], void* y, int dt, int64_t at, int64_t ld, int rows,
                                             int cols, int wn, int wm, int lr, int lg, const float* bias) {
@@ -220,21 +236,35 @@ __device__ __forceinline__ void store_tiles(const f4v (&acc)[IT][JT], void* y, i
         for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? bias[n + e] : 0.0f;
       return b;
     };
-    if (DT != TRK_F32 && wn + IT * 16 <= cols) {  // the wave's columns are all there
-      if constexpr (DT != TRK_F32) {
+    if (wn + IT * 16 <= cols) {  // the wave's columns are all there
+      constexpr int RUN = DT == TRK_F32 ? 1 : 2;  // column tiles of a 64-byte run
+      const bool low = lr < 8;
+      auto run = [&](int i, int j, const f4v* b) {
+        if constexpr (DT == TRK_F32) {
+          return __builtin_bit_cast(uint4, acc[i][j] + b[0]);
+        } else {
+          typedef unsigned u2 __attribute__((ext_vector_type(2)));
+          const uint2 p = pack4<DT>(acc[i][j] + b[0]), q = pack4<DT>(acc[i + 1][j] + b[1]);
+          const u2 x = __builtin_amdgcn_permlane16_swap(p.x, q.x, false, false);
+          const u2 z = __builtin_amdgcn_permlane16_swap(p.y, q.y, false, false);
+          return make_uint4(x[0], z[0], x[1], z[1]);
+        }
+      };
+      // a lane's column in a run; lanes of the upper rows hold the second run
+      const int n = wn + (DT == TRK_F32 ? lg * 4 : (lg & 1) * 16 + (lg >> 1) * 8) + (low ? 0 : RUN * 16);
 #pragma unroll
-        for (int i = 0; i < IT; i += 2) {
-          const f4v b0 = column_bias(i), b1 = column_bias(i + 1);
+      for (int i = 0; i < IT; i += 2 * RUN) {
+        f4v b[2 * RUN];
 #pragma unroll
-          for (int j = 0; j < JT; ++j) {
-            const uint2 p = pack4<DT>(acc[i][j] + b0), q = pack4<DT>(acc[i + 1][j] + b1);
-            typedef unsigned u2 __attribute__((ext_vector_type(2)));
-            const u2 x = __builtin_amdgcn_permlane16_swap(p.x, q.x, false, false);
-            const u2 z = __builtin_amdgcn_permlane16_swap(p.y, q.y, false, false);
-            const uint4 o = make_uint4(x[0], z[0], x[1], z[1]);
-            const int m = wm + j * 16 + lr;
-            if (m < rows) __builtin_memcpy(tile + m * ld + wn + (i + (lg & 1)) * 16 + (lg >> 1) * 8, &o, 16);
-          }
+        for (int h = 0; h < 2 * RUN; ++h) b[h] = column_bias(i + h);
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          uint4 u = run(i, j, b), v = run(i + RUN, j, b + RUN);
+          pair_lines(u, v, low);
+          const int m = wm + j * 16 + (lr & 7);
+          E* to = tile + m * ld + n + i * 16;
+          if (m < rows) __builtin_memcpy(to, &u, 16);
+          if (m + 8 < rows) __builtin_memcpy(to + 8 * ld, &v, 16);
         }
       }
     } else {
