@@ -38,8 +38,8 @@ _lib.register({
                        _I),
     "trk_matmul_grouped": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I64,
                             _I64, _I, _P, _I64, _I, _I, _P], _I),
-    "trk_matmul_grouped_dx": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P], _I),
-    "trk_matmul_grouped_dw": ([_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _P], _I),
+    "trk_matmul_grouped_bwd": ([_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _I64,
+                                _I64, _P], _I),
 })
 
 FP8 = torch.float8_e4m3fn
@@ -358,15 +358,10 @@ class _Grouped(torch.autograd.Function):
         M, K = x.shape
         G, N = w.shape[:2]
         dy, ldy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = x.new_empty((M, K))
-            _launch("matmul_grouped backward", "trk_matmul_grouped_dx", x, dy.data_ptr(), ldy, w.data_ptr(), ldw, w.stride(0),
-                    counts.data_ptr(), G, M, N, K, ctx.dt, dx.data_ptr(), max(K, 1))
-        if ctx.needs_input_grad[1]:
-            dw = x.new_empty((G, N, K))
-            _launch("matmul_grouped backward", "trk_matmul_grouped_dw", x, dy.data_ptr(), ldy, x.data_ptr(), ldx,
-                    counts.data_ptr(), G, M, N, K, ctx.dt, dw.data_ptr(), max(K, 1), N * K)
+        dx = x.new_empty((M, K)) if ctx.needs_input_grad[0] else None
+        dw = x.new_empty((G, N, K)) if ctx.needs_input_grad[1] else None
+        _launch("matmul_grouped backward", "trk_matmul_grouped_bwd", x, dy.data_ptr(), ldy, x.data_ptr(), ldx, w.data_ptr(), ldw,
+                w.stride(0), counts.data_ptr(), G, M, N, K, ctx.dt, _at(dx), max(K, 1), _at(dw), max(K, 1), N * K)
         return dx, dw, None, None, None
 
 
