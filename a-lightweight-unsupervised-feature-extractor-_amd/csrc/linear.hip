@@ -18,14 +18,6 @@
 
 using namespace trk;
 
-#ifndef TRK_TN
-#define TRK_TN 256
-#define TRK_TM 256
-#define TRK_WN 2
-#define TRK_WM 4
-#define TRK_NB 2
-#endif
-
 namespace {
 
 typedef float f4v __attribute__((ext_vector_type(4)));
@@ -1176,45 +1168,75 @@ int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
   return trk::check_launch(what);
 }
 
+// row tiles that have rows, as far as the host knows: groups have at least a tile each
+int64_t live_tiles(const MmArgs& A, int tm) {
+  const int64_t full = (A.M + tm - 1) / tm;
+  return A.counts ? std::max(full, std::min(A.G, A.M)) : full;
+}
+
 template <int IN, bool WROW, int JT>
-void launch_few(const MmArgs& A, int dt, hipStream_t st) {
-  const int64_t strips = (A.N + 15) / 16, mt = row_tiles(A, 16 * JT), steps = (A.K * (is8(IN) ? 1 : 2) + kStep - 1) / kStep;
-  int kw = 8;  // waves that share 16 columns: enough for 2048 waves in all, no more than there are steps
-  while (kw > 1 && (strips * mt * (kw / 2) >= 2048 || kw > steps)) kw /= 2;
-  const dim3 grid((unsigned)((strips + 8 / kw - 1) / (8 / kw)), (unsigned)mt);
+int launch_few(const char* what, const MmArgs& A, int dt, hipStream_t st) {
+  const int64_t strips = (A.N + 15) / 16, live = live_tiles(A, 16 * JT), steps = (A.K * (is8(IN) ? 1 : 2) + kStep - 1) / kStep;
+  // waves that share 16 columns: enough for 2048 waves in all, no more than there are steps (16 x 4096 x
+  // 4096 in 8 bits: 7.0 us with 8, 10.5 with 4; 64 groups of 1 row x 1024 x 1024: 15.2 with 1, 23.5 with 4)
+  int kw = 8;
+  while (kw > 1 && (strips * live * (kw / 2) >= 2048 || kw > steps)) kw /= 2;
+  const dim3 grid((unsigned)((strips + 8 / kw - 1) / (8 / kw)), (unsigned)row_tiles(A, 16 * JT));
   if (kw == 8) mm_few_kernel<IN, WROW, JT, 8><<<grid, 512, 0, st>>>(A, dt);
   else if (kw == 4) mm_few_kernel<IN, WROW, JT, 4><<<grid, 512, 0, st>>>(A, dt);
   else if (kw == 2) mm_few_kernel<IN, WROW, JT, 2><<<grid, 512, 0, st>>>(A, dt);
   else mm_few_kernel<IN, WROW, JT, 1><<<grid, 512, 0, st>>>(A, dt);
+  return trk::check_launch(what);
+}
+
+int cu_count() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+    cus = 256;
+  return cus;
+}
+
+template <int IN, bool WROW, int T, int WN, int WM>
+int launch_tile(const char* what, const MmArgs& A, int dt, int cus, hipStream_t st) {
+  constexpr int BT = WN * WM * 64, NB = 2;
+  constexpr int lds = NB * (2 * T * kStep + (is8(IN) ? (2 * T + BT - 1) / BT * BT * 4 : 0));
+  auto* f = mm_tile_kernel<IN, WROW, T, T, WN, WM, NB>;
+  TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
+  const int64_t nt = (A.N + T - 1) / T, mt = row_tiles(A, T);
+  TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
+  const int64_t grid = std::min<int64_t>(nt * mt, (int64_t)cus * (BT == 256 ? 2 : 1) / 8 * 8);
+  f<<<(unsigned)grid, BT, lds, st>>>(A, dt, (int)nt, (int)mt);
+  return trk::check_launch(what);
 }
 
 template <int IN, bool WROW>
 int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStream_t st) {
-  const int64_t each = A.counts ? (A.M + A.G - 1) / A.G : A.M;  // rows of a group
-  if (each <= 64 && row_tiles(A, 16) <= 65535) {
-    if (each <= 16) launch_few<IN, WROW, 1>(A, dt, st);
-    else if (each <= 32) launch_few<IN, WROW, 2>(A, dt, st);
-    else launch_few<IN, WROW, 4>(A, dt, st);
-  } else if (aligned) {
-    constexpr bool small = IN == IN_E4M3X;
-    constexpr int TN = small ? 128 : TRK_TN, TM = small ? 128 : TRK_TM, WN = small ? 2 : TRK_WN, WM = small ? 2 : TRK_WM,
-                  NB = TRK_NB;
-    constexpr int BT = WN * WM * 64;
-    constexpr int lds = NB * ((TM + TN) * kStep + (is8(IN) ? (TM + TN + BT - 1) / BT * BT * 4 : 0));
-    auto* f = mm_tile_kernel<IN, WROW, TN, TM, WN, WM, NB>;
-    TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
-    const int64_t nt = (A.N + TN - 1) / TN, mt = row_tiles(A, TM);
-    TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
-    int dev = 0, cus = 0;
-    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-      cus = 256;
-    const int64_t grid = std::min<int64_t>(nt * mt, (int64_t)cus * (small ? 2 : 1) / 8 * 8);
-    f<<<(unsigned)grid, WN * WM * 64, lds, st>>>(A, dt, (int)nt, (int)mt);
-  } else {
-    const int mt = row_tiles(A, 128);
-    TRK_REQUIRE(mt <= 65535, "%s: too many row tiles (%d)", what, mt);
-    mm_kernel<IN, WROW><<<dim3((unsigned)((A.N + 127) / 128), (unsigned)mt), 256, 0, st>>>(A, dt);
+  const int cus = cu_count();
+  // CHOICE
+  // Few strips of 16 JT rows x 16 columns: straight from memory to registers, 16 rows a strip while there
+  // are at most 256, else the fewest strips by the work of one (1, 1.4 and 2.2 for 16, 32 and 64 rows).
+  // In 8 bits, us, strips / 128-tiles: 16 x 4096 x 4096 7.0 / 20.9, 64 x 4096 x 4096 13.9 / 21.0, 256 x
+  // 1024 x 1024 6.2 / 8.6, 32 x 16384 x 4096 26.5 / 28.5; past the limits 128 x 4096 x 4096 22.8 / 21.2,
+  // 16 x 50000 x 1024 18.0 / 12.7, 512 x 8192 x 1024 40.7 / 10.5.
+  const int64_t strips = (A.N + 15) / 16, s16 = strips * live_tiles(A, 16), s32 = strips * live_tiles(A, 32),
+                s64 = strips * live_tiles(A, 64);
+  if (row_tiles(A, 16) <= 65535) {
+    if (s16 <= 256 || (s16 <= 1024 && 5 * s16 <= 7 * s32 && 5 * s16 <= 11 * s64)) return launch_few<IN, WROW, 1>(what, A, dt, st);
+    if (s32 <= 1024 && 7 * s32 <= 11 * s64) return launch_few<IN, WROW, 2>(what, A, dt, st);
+    if (s64 <= 512) return launch_few<IN, WROW, 4>(what, A, dt, st);
   }
+  if (aligned) {
+    // 256-tiles where whole ones alone fill the CUs (2048 x 8192 x 1024 in 8 bits 23.2 us against 25.8 with 128-tiles;
+    // 1024 x 8192 x 1024 20.2 against 15.2; 64 groups of 8 rows x 2048 x 2048 70 against 48).  f32
+    // outputs have wider fragments, which only leave room for 128-tiles.
+    if constexpr (IN != IN_E4M3X) {
+      if ((A.N + 255) / 256 * (A.M / 256) >= cus) return launch_tile<IN, WROW, 256, 2, 4>(what, A, dt, cus, st);
+    }
+    return launch_tile<IN, WROW, 128, 2, 2>(what, A, dt, cus, st);
+  }
+  const int mt = row_tiles(A, 128);
+  TRK_REQUIRE(mt <= 65535, "%s: too many row tiles (%d)", what, mt);
+  mm_kernel<IN, WROW><<<dim3((unsigned)((A.N + 127) / 128), (unsigned)mt), 256, 0, st>>>(A, dt);
   return trk::check_launch(what);
 }
 
