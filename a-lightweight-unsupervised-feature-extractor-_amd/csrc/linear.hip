@@ -356,91 +356,6 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p, int64_t left) {
   return v;
 }
 
-// 128 x 128 tile, 4 waves of 64 x 64.  Rows of the tile past their end are read from the last
-// row and never stored; columns of w likewise.
-template <int IN, bool WROW>
-__global__ __launch_bounds__(256) void mm_kernel(MmArgs A, int dt) {
-  constexpr int TM = 128, TN = 128;
-  __shared__ uint4 smem[(TM + TN) * kStep / 16];
-  __shared__ int sums[4];
-  __shared__ Runs runs[256];
-  __shared__ Tile found;
-  uint8_t* xs = (uint8_t*)smem;
-  uint8_t* ws = xs + TM * kStep;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Tile T;
-  if (A.counts) {
-    Finder<TM, 256> F;
-    F.init(A.counts, (int)A.G, A.M, A.zero_tail, sums, runs);
-    if (blockIdx.y >= F.all) return;
-    F.find(A.counts, (int)A.G, A.M, blockIdx.y, runs, &found);
-    __syncthreads();
-    T = found;
-  } else {
-    T.row0 = (int64_t)blockIdx.y * TM;
-    T.rows = (int)min((int64_t)TM, A.M - T.row0);
-    T.g = 0;
-  }
-  const int64_t n0 = (int64_t)blockIdx.x * TN;
-  const int cols = (int)min((int64_t)TN, A.N - n0);
-  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
-  const int64_t kbytes = T.g < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
-  const int64_t g = max(0, T.g);
-  const uint8_t* xb = A.x + T.row0 * A.ldx;
-  const uint8_t* wb = A.w + g * A.wg + n0 * A.ldw;
-  const float* sw = A.sw + g * A.sw_g;
-  f4v acc[4][4];  // [n tile][m tile]
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = f4v{0, 0, 0, 0};
-  for (int64_t k = 0; k < kbytes; k += kStep) {
-    const int c = tid & 7;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (tid >> 3) + 32 * i;
-      *(uint4*)(xs + lds_at(r, c)) = load16(xb + min(r, T.rows - 1) * A.ldx + k + c * 16, kbytes - k - c * 16);
-      *(uint4*)(ws + lds_at(r, c)) = load16(wb + min(r, cols - 1) * A.ldw + k + c * 16, kbytes - k - c * 16);
-    }
-    __syncthreads();
-    Frag<IN> b[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
-    float s[4];
-    const int64_t kb = k / kBK;  // e4m3: one block of columns a step
-    if constexpr (is8(IN)) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j] = A.sx[(T.row0 + min(wm + j * 16 + lr, T.rows - 1)) * A.sx_row + kb * A.sx_kb];
-        if constexpr (!WROW) s[j] *= sw[(n0 / 128) * A.sw_row + kb * A.sw_kb];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const Frag<IN> a = frag<IN>(ws, wn + i * 16 + lr, lg);
-      float wr[4];
-      if constexpr (is8(IN) && WROW) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          wr[e] = sw[(n0 + min(wn + i * 16 + lg * 4 + e, cols - 1)) * A.sw_row + kb * A.sw_kb];
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (is8(IN)) {
-          const f4v p = mma<IN>(a, b[j], f4v{0, 0, 0, 0});
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(p[e], WROW ? s[j] * wr[e] : s[j], acc[i][j][e]);
-        } else {
-          acc[i][j] = mma<IN>(a, b[j], acc[i][j]);
-        }
-      }
-    }
-  }
-  store_tiles(acc, A.y, dt, T.row0 * A.ldy + n0, A.ldy, T.rows, cols, wn, wm, lr, lg,
-              A.bias && T.g >= 0 ? A.bias + n0 : nullptr);
-}
-
 // ------------------------------------------------------------------ large tiles
 #define GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define LPTR(p) ((__attribute__((address_space(3))) void*)(p))
@@ -462,10 +377,10 @@ __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
   return x * per + min(x, more) + id / 8;
 }
 
-// TN x TM tiles, WN x WM waves, operands copied straight to LDS (16 bytes a lane) NB - 1 steps ahead in
-// a ring of NB stages.  Rows start at multiples of 16 bytes.  A workgroup runs several tiles: the
-// next tile's first copies are sent before a tile's stores.
-template <int IN, bool WROW, int TN, int TM, int WN, int WM, int NB>
+// TN x TM tiles, WN x WM waves, operands copied to LDS one step ahead.  DMA: straight, 16 bytes a lane;
+// every row starts at a multiple of 16 bytes.  Else through registers, at any alignment.  A
+// workgroup runs several tiles: the next tile's first copies are sent before a tile's stores.
+template <int IN, bool WROW, bool DMA, int TN, int TM, int WN, int WM>
 __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int dt, int ntiles, int mtiles) {
   constexpr int BT = WN * WM * 64, IT = TN / WN / 16, JT = TM / WM / 16;
   constexpr int XB = TM * kStep, WB = TN * kStep, LS = is8(IN) ? (TM + TN + BT - 1) / BT : 0, STAGE = XB + WB + LS * BT * 4;
@@ -536,17 +451,25 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   };
   auto xoff = [&](int q) { return min(x0 + (uint32_t)(q * (BT / 8)) * (uint32_t)A.ldx, xend); };
   auto woff = [&](int q) { return min(w0 + (uint32_t)(q * (BT / 8)) * (uint32_t)A.ldw, wend); };
-  // copy q of LOADS of step kt into its stage
-  auto copy = [&](int q, int kt, uint8_t* d, __amdgpu_buffer_rsrc_t xr, __amdgpu_buffer_rsrc_t wr)
-      __attribute__((always_inline)) {
+  // copy q of LOADS of step kt into its stage; without DMA, into `hold`, which keep() writes there
+  typedef __amdgpu_buffer_rsrc_t Rsrc;
+  auto copy = [&](int q, int kt, uint8_t* d, Rsrc xr, Rsrc wr, uint4* hold) __attribute__((always_inline)) {
     if (q < LX) {
-      to_lds(xr, d + (q * BT + wave * 64) * 16, xoff(q), kt * kStep);
+      if constexpr (DMA) to_lds(xr, d + (q * BT + wave * 64) * 16, xoff(q), kt * kStep);
+      else __builtin_memcpy(hold + q, xb + xoff(q) + (int64_t)kt * kStep, 16);
     } else if (q < LX + LW) {
-      to_lds(wr, d + XB + ((q - LX) * BT + wave * 64) * 16, woff(q - LX), kt * kStep);
+      if constexpr (DMA) to_lds(wr, d + XB + ((q - LX) * BT + wave * 64) * 16, woff(q - LX), kt * kStep);
+      else __builtin_memcpy(hold + q, wb + woff(q - LX) + (int64_t)kt * kStep, 16);
     } else {
       const int p = q - LX - LW;
       const int64_t kb = (p * BT + wave * 64 < TM ? A.sx_kb : A.sw_kb) * (int64_t)kt;
       __builtin_amdgcn_global_load_lds(GPTR(ssrc[p] + kb), LPTR(d + XB + WB + (p * BT + wave * 64) * 4), 4, 0, 0);
+    }
+  };
+  auto keep = [&](uint8_t* d, const uint4* hold) __attribute__((always_inline)) {
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int q = 0; q < LX + LW; ++q) *(uint4*)(d + (q * BT + tid) * 16) = hold[q];  // (XB is LX BT 16)
     }
   };
 
@@ -554,13 +477,14 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   // One step of stage `st`; the copies go into `nx` (a different stage, so that the compiler lets
   // them stay in flight across the reads).  8 bits: the scaling of one row of tiles runs on the
   // vector units under the matrix instructions of the next.
-  auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx, int kn, __amdgpu_buffer_rsrc_t xr,
-                  __amdgpu_buffer_rsrc_t wr) __attribute__((always_inline)) {
+  auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx, int kn, Rsrc xr, Rsrc wr)
+      __attribute__((always_inline)) {
     const uint8_t *xs = st, *ws = st + XB;
     const float* ss = (const float*)(st + XB + WB);
     Frag<IN> b[JT], a[2];
     float s[JT];
     f4v p[2][JT], sc[2];
+    uint4 hold[LX + LW];
 #pragma unroll
     for (int j = 0; j < JT; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
     a[0] = frag<IN>(ws, wn + lr, lg);
@@ -595,7 +519,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
       if constexpr (decltype(more)::value) {
 #pragma unroll
         for (int q = i * PER; q < (i + 1) * PER; ++q)
-          if (q < LOADS) copy(q, kn, nx, xr, wr);
+          if (q < LOADS) copy(q, kn, nx, xr, wr, hold);
       }
       if constexpr (is8(IN) && WROW) {
         if (i + 1 < IT) sc[(i + 1) & 1] = *(const f4v*)(ss + TM + wn + (i + 1) * 16 + lg * 4);
@@ -614,20 +538,20 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
       __builtin_amdgcn_sched_barrier(0);  // rows of tiles stay in this order
     }
     add(IT - 1);
+    if constexpr (decltype(more)::value) keep(nx, hold);
   };
   auto first_copies = [&](int at) {
-    const __amdgpu_buffer_rsrc_t xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
+    if (steps == 0) return;
+    const Rsrc xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
+    uint4 hold[LX + LW];
 #pragma unroll
-    for (int k = 0; k < NB - 1; ++k) {
-      if (k < steps)
-#pragma unroll
-        for (int q = 0; q < LOADS; ++q) copy(q, k, smem + (at + k >= NB ? at + k - NB : at + k) * STAGE, xr, wr);
-    }
+    for (int q = 0; q < LOADS; ++q) copy(q, 0, smem + at * STAGE, xr, wr, hold);
+    keep(smem + at * STAGE, hold);
   };
 
   int64_t idx = blockIdx.x;
   if (idx >= total) return;
-  int nt, mt, at = 0;  // at: the stage of the step
+  int nt, mt, at = 0;  // at: the stage of the step, 0 or 1
   tile_at(idx, nt, mt);
   if (A.counts) {
     F.find(A.counts, (int)A.G, A.M, mt, runs, &found);
@@ -637,21 +561,20 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   first_copies(at);
   while (true) {
     {
-      const __amdgpu_buffer_rsrc_t xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
+      const Rsrc xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
 #pragma unroll
       for (int i = 0; i < IT; ++i)
 #pragma unroll
         for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
-      for (int kt = 0; kt < steps - (NB - 1); ++kt) {
-        // stage kt has landed (its copies are the oldest; younger stages stay in flight), and every wave
-        // is done with stage kt - 1, whose slot the next copies overwrite
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS * (NB - 2)) : "memory");
+      for (int kt = 0; kt < steps - 1; ++kt) {
+        // step kt has landed, and every wave is done with step kt - 1, whose stage the next copies overwrite
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        step(std::true_type(), smem + at * STAGE, smem + (at == 0 ? NB - 1 : at - 1) * STAGE, kt + NB - 1, xr, wr);
-        at = at + 1 == NB ? 0 : at + 1;
+        step(std::true_type(), smem + at * STAGE, smem + (at ^ 1) * STAGE, kt + 1, xr, wr);
+        at ^= 1;
       }
-      for (int kt = max(0, steps - (NB - 1)); kt < steps + rest; ++kt) {
+      for (int kt = max(0, steps - 1); kt < steps + rest; ++kt) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -678,7 +601,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
           __syncthreads();
         }
         step(std::false_type(), smem + at * STAGE, smem, 0, xr, wr);
-        at = at + 1 == NB ? 0 : at + 1;
+        at ^= 1;
       }
     }
     const int64_t y0 = row0 * A.ldy + n0;
@@ -819,22 +742,6 @@ __global__ __launch_bounds__(512) void mm_few_kernel(MmArgs A, int dt) {
 }
 
 // ------------------------------------------------------------------ gradients (16 bits)
-// Both contract over an index that is not contiguous in memory, so their tiles are turned while
-// they are written to LDS: src is [64 k][128 cols] with row stride ld, LDS gets [col][k].
-__device__ __forceinline__ void stage_turned(uint8_t* lds, const uint16_t* src, int64_t ld, int64_t ks, int cols) {
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int k = (tid >> 4) + 16 * i, c0 = (tid & 15) * 8;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (k < ks) v = load16((const uint8_t*)(src + k * ld + c0), 2 * (int64_t)(cols - c0));
-    uint16_t t[8];
-    __builtin_memcpy(t, &v, 16);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) *(uint16_t*)(lds + lds_at(c0 + j, k >> 3) + (k & 7) * 2) = t[j];
-  }
-}
-
 struct GradArgs {
   const uint16_t *dy, *x, *w;
   void *dx, *dw;                                   // null: not wanted
@@ -843,91 +750,6 @@ struct GradArgs {
   int64_t M, N, K, G;
 };
 
-template <int IN>
-__device__ __forceinline__ void mm_tile16(const uint8_t* ws, const uint8_t* xs, f4v (&acc)[4][4], int wn, int wm, int lr,
-                                          int lg) {
-  Frag<IN> b[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = frag<IN>(xs, wm + j * 16 + lr, lg);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const Frag<IN> a = frag<IN>(ws, wn + i * 16 + lr, lg);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = mma<IN>(a, b[j], acc[i][j]);
-  }
-}
-
-// dx[m][k] = sum_n dy[m][n] w[g][n][k]
-template <int IN>
-__global__ __launch_bounds__(256) void grouped_dx_kernel(GradArgs A, int dt) {
-  constexpr int TM = 128;
-  __shared__ uint4 smem[2 * 128 * kStep / 16];
-  __shared__ int sums[4];
-  __shared__ Runs runs[256];
-  __shared__ Tile found;
-  uint8_t* xs = (uint8_t*)smem;
-  uint8_t* ws = xs + 128 * kStep;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Finder<TM, 256> F;
-  F.init(A.counts, (int)A.G, A.M, true, sums, runs);
-  if (blockIdx.y >= F.all) return;
-  F.find(A.counts, (int)A.G, A.M, blockIdx.y, runs, &found);
-  __syncthreads();
-  const Tile T = found;
-  const int64_t c0 = (int64_t)blockIdx.x * 128;
-  const int cols = (int)min((int64_t)128, A.K - c0);
-  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
-  const uint8_t* xb = (const uint8_t*)(A.dy + T.row0 * A.ldy);
-  const uint16_t* wb = A.w + max(0, T.g) * A.wg + c0;
-  f4v acc[4][4] = {};
-  for (int64_t k = 0; k < (T.g < 0 ? 0 : A.N); k += 64) {
-    __syncthreads();
-    const int c = tid & 7;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = (tid >> 3) + 32 * i;
-      *(uint4*)(xs + lds_at(r, c)) =
-          load16(xb + (min(r, T.rows - 1) * A.ldy + k + c * 8) * 2, 2 * (A.N - k - c * 8));
-    }
-    stage_turned(ws, wb + k * A.ldw, A.ldw, A.N - k, cols);
-    __syncthreads();
-    mm_tile16<IN>(ws, xs, acc, wn, wm, lr, lg);
-  }
-  store_tiles(acc, A.dx, dt, T.row0 * A.lddx + c0, A.lddx, T.rows, cols, wn, wm, lr, lg, nullptr);
-}
-
-// dw[g][n][k] = sum over the rows m of group g of dy[m][n] x[m][k]
-template <int IN>
-__global__ __launch_bounds__(256) void grouped_dw_kernel(GradArgs A, int dt) {
-  __shared__ uint4 smem[2 * 128 * kStep / 16];
-  __shared__ int64_t red[4][2];
-  uint8_t* xs = (uint8_t*)smem;
-  uint8_t* ws = xs + 128 * kStep;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t g = blockIdx.z;
-  int64_t before = 0;
-  for (int64_t i = tid; i < g; i += 256) before += max(0, A.counts[i]);
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) before += __shfl_xor(before, m, 64);
-  if (lane == 0) red[wave][0] = before;
-  __syncthreads();
-  const int64_t row0 = min(A.M, red[0][0] + red[1][0] + red[2][0] + red[3][0]);
-  const int64_t rows = min((int64_t)max(0, A.counts[g]), A.M - row0);
-  const int64_t n0 = (int64_t)blockIdx.y * 128, k0 = (int64_t)blockIdx.x * 128;
-  const int nr = (int)min((int64_t)128, A.N - n0), kc = (int)min((int64_t)128, A.K - k0);
-  const int wn = (wave & 1) * 64, wm = (wave >> 1) * 64, lr = lane & 15, lg = lane >> 4;
-  f4v acc[4][4] = {};
-  for (int64_t r = 0; r < rows; r += 64) {
-    __syncthreads();
-    stage_turned(xs, A.dy + (row0 + r) * A.ldy + n0, A.ldy, rows - r, nr);
-    stage_turned(ws, A.x + (row0 + r) * A.ldx + k0, A.ldx, rows - r, kc);
-    __syncthreads();
-    mm_tile16<IN>(ws, xs, acc, wn, wm, lr, lg);
-  }
-  store_tiles(acc, A.dw, dt, g * A.og + n0 * A.ldo + k0, A.ldo, nr, kc, wn, wm, lr, lg, nullptr);
-}
-
-// ------------------------------------------------------------------ gradients on large tiles
 typedef short s4v __attribute__((ext_vector_type(4)));
 
 // A turned tile keeps its source's order, [64 k][T cols], and is turned while it is read: for 16
@@ -958,7 +780,7 @@ __device__ __forceinline__ Frag<IN> frag_turned(const uint8_t* tile, uint32_t at
 
 // T x T tile `block` of dx (DW false: rows m of one group, columns k, contracted over n) or of dw[g] (rows n,
 // columns k, contracted over the group's rows), 8 waves, copies one step of 64 ahead.
-template <int IN, bool DW>
+template <int IN, bool DW, bool DMA>
 __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t block, int64_t ctiles, int64_t rtiles, uint8_t* smem,
                                           int* sums, Runs* runs, Tile* found) {
   constexpr int T = 256, BT = 512, WN = 2, WM = 4, IT = T / WN / 16, JT = T / WM / 16;
@@ -1024,17 +846,35 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
 #pragma unroll
   for (int q = 0; q < L; ++q) {
     const int p = q * BT + tid, r = p >> 5, c = ((((p >> 1) & 15) ^ turn_of(r)) << 4) + (p & 1) * 8;
-    woff[q] = (uint32_t)(r * wld + min(c, (cols - 1) & ~7)) * 2;
+    woff[q] = (uint32_t)(r * wld + (DMA ? min(c, (cols - 1) & ~7) : min(c, cols))) * 2;
     const int xrow = p >> 3;
-    xoff[q] = DW ? (uint32_t)(r * xld + min(c, (rows - 1) & ~7)) * 2
+    xoff[q] = DW ? (uint32_t)(r * xld + (DMA ? min(c, (rows - 1) & ~7) : min(c, rows))) * 2
                  : (uint32_t)(min(xrow, rows - 1) * xld) * 2 + (((p & 7) ^ (xrow & 7)) << 4);
   }
   // copies q and q + L of a step; the bases move with the steps (a group's rows may span more than 4 GB)
   const uint32_t wat = turned_at<T>(wn, lane), xat = turned_at<T>(wm, lane);
   const uint8_t *xp = (const uint8_t*)xsrc0, *wp = (const uint8_t*)wsrc0;
-  auto copy = [&](int q, __amdgpu_buffer_rsrc_t xr, __amdgpu_buffer_rsrc_t wr, uint8_t* d) __attribute__((always_inline)) {
-    to_lds(xr, d + (q * BT + wave * 64) * 16, xoff[q], 0);
-    to_lds(wr, d + XB + (q * BT + wave * 64) * 16, woff[q], 0);
+  // piece q of a turned operand, whose row has `n` columns (without DMA: any alignment, nothing read behind them)
+  auto turned_piece = [&](const uint8_t* p, uint32_t off, int q, int n) {
+    const int slot = q * BT + tid, c = ((((slot >> 1) & 15) ^ turn_of(slot >> 5)) << 4) + (slot & 1) * 8;
+    return load16(p + off, 2 * (n - c));
+  };
+  auto copy = [&](int q, __amdgpu_buffer_rsrc_t xr, __amdgpu_buffer_rsrc_t wr, uint8_t* d, uint4* hold)
+      __attribute__((always_inline)) {
+    if constexpr (DMA) {
+      to_lds(xr, d + (q * BT + wave * 64) * 16, xoff[q], 0);
+      to_lds(wr, d + XB + (q * BT + wave * 64) * 16, woff[q], 0);
+    } else {
+      if constexpr (DW) hold[q] = turned_piece(xp, xoff[q], q, rows);
+      else __builtin_memcpy(hold + q, xp + xoff[q], 16);
+      hold[L + q] = turned_piece(wp, woff[q], q, cols);
+    }
+  };
+  auto keep = [&](uint8_t* d, const uint4* hold) __attribute__((always_inline)) {
+    if constexpr (!DMA) {
+#pragma unroll
+      for (int q = 0; q < 2 * L; ++q) *(uint4*)(d + (q * BT + tid) * 16) = hold[q];
+    }
   };
   f4v acc[IT][JT];
 #pragma unroll
@@ -1042,10 +882,11 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
 #pragma unroll
     for (int j = 0; j < JT; ++j) acc[i][j] = f4v{0, 0, 0, 0};
   auto step = [&](auto more, const uint8_t* __restrict st, uint8_t* __restrict nx) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t xr = rows_at(xp, 0x7fffffff), wr = rows_at(wp, 0x7fffffff);
+    const __amdgpu_buffer_rsrc_t xr = rows_at(xp, 0xffffffff), wr = rows_at(wp, 0xffffffff);
     uint32_t at = wat, bt = xat;
     asm volatile("" : "+v"(at), "+v"(bt));  // the addresses are made in the step, not kept across it
     Frag<IN> b[JT], a[2];
+    uint4 hold[2 * L];
 #pragma unroll
     for (int j = 0; j < JT; ++j) {
       if constexpr (DW) b[j] = frag_turned<IN, T>(st, bt ^ (j << 5));
@@ -1058,16 +899,19 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
 #pragma unroll
       for (int j = 0; j < JT; ++j) acc[i][j] = mma<IN>(a[i & 1], b[j], acc[i][j]);
       if constexpr (decltype(more)::value) {
-        if (i < L) copy(i, xr, wr, nx);
+        if (i < L) copy(i, xr, wr, nx, hold);
       }
       __builtin_amdgcn_sched_barrier(0);  // rows of tiles stay in this order
     }
+    if constexpr (decltype(more)::value) keep(nx, hold);
   };
   static_assert(L <= IT, "two copies with each row of tiles");
   if (steps > 0) {
-    const __amdgpu_buffer_rsrc_t xr = rows_at(xp, 0x7fffffff), wr = rows_at(wp, 0x7fffffff);
+    const __amdgpu_buffer_rsrc_t xr = rows_at(xp, 0xffffffff), wr = rows_at(wp, 0xffffffff);
+    uint4 hold[2 * L];
 #pragma unroll
-    for (int q = 0; q < L; ++q) copy(q, xr, wr, smem);
+    for (int q = 0; q < L; ++q) copy(q, xr, wr, smem, hold);
+    keep(smem, hold);
   }
   const int64_t left = steps_of - (int64_t)steps * 64;
   for (int kt = 0; kt < steps - 1; ++kt) {
@@ -1089,9 +933,9 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
       for (int q = 0; q < L; ++q) {
         const int p = q * BT + tid;
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        *(uint4*)(d + XB + p * 16) = (p >> 5) < left ? *(const uint4*)(wp + woff[q]) : zero;
+        *(uint4*)(d + XB + p * 16) = (p >> 5) >= left ? zero : DMA ? *(const uint4*)(wp + woff[q]) : turned_piece(wp, woff[q], q, cols);
         if constexpr (DW) {
-          *(uint4*)(d + p * 16) = (p >> 5) < left ? *(const uint4*)(xp + xoff[q]) : zero;
+          *(uint4*)(d + p * 16) = (p >> 5) >= left ? zero : DMA ? *(const uint4*)(xp + xoff[q]) : turned_piece(xp, xoff[q], q, rows);
         } else {
           const int c = (p & 7) ^ ((p >> 3) & 7);
           *(uint4*)(d + p * 16) = load16(xp + xoff[q], 2 * (left - c * 8));
@@ -1108,14 +952,14 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
 
 // Both gradients in one grid (dw's tiles first): the workgroups that find no more tiles of the one
 // take those of the other, where two launches leave part of the CUs idle at the end of each.
-template <int IN>
+template <int IN, bool DMA>
 __global__ __launch_bounds__(512, 2) void grad_kernel(GradArgs A, int dt, int64_t ctiles, int64_t rtiles, int64_t dw_tiles) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int sums[8];
   __shared__ Runs runs[512];
   __shared__ Tile found;
-  if (blockIdx.x < dw_tiles) grad_tile<IN, true>(A, dt, blockIdx.x, ctiles, rtiles, smem, sums, runs, &found);
-  else grad_tile<IN, false>(A, dt, blockIdx.x - dw_tiles, ctiles, 0, smem, sums, runs, &found);
+  if (blockIdx.x < dw_tiles) grad_tile<IN, true, DMA>(A, dt, blockIdx.x, ctiles, rtiles, smem, sums, runs, &found);
+  else grad_tile<IN, false, DMA>(A, dt, blockIdx.x - dw_tiles, ctiles, 0, smem, sums, runs, &found);
 }
 
 int check_out(const char* what, int dt) {
@@ -1130,13 +974,19 @@ int check_mm(const char* what, const MmArgs& A, int64_t item, bool scaled) {
   if (A.M == 0 || A.N == 0) return TRK_OK;
   TRK_REQUIRE(A.y && (A.K == 0 || (A.x && A.w)) && (!scaled || A.K == 0 || (A.sx && A.sw)), "%s: null pointer", what);
   TRK_REQUIRE(A.ldx >= A.K * item && A.ldw >= A.K * item && A.ldy >= A.N, "%s: row stride below the row's length", what);
+  // offsets inside a tile of 256 rows are 32 bits
+  if (A.ldx >= (1 << 24) || A.ldw >= (1 << 24)) {
+    set_error("%s: row strides of 16 MiB and more are not supported", what);
+    return TRK_EUNSUPPORTED;
+  }
   return TRK_OK;
 }
 
-// gradients: whole 16-byte pieces of every row at multiples of 16 bytes
-bool grad_aligned(const void* a, int64_t lda, const void* b, int64_t ldb, int64_t bg) {
-  return aligned16_ptr(a) && aligned16_ptr(b) && lda % 8 == 0 && ldb % 8 == 0 && bg % 8 == 0 &&
-         lda < (1 << 22) && ldb < (1 << 22);  // offsets inside a tile are 32 bits
+// whole 16-byte pieces of every row at multiples of 16 bytes (offsets inside a tile are 32 bits)
+bool rows_aligned(const void* p, int64_t ld) { return aligned16_ptr(p) && ld % 8 == 0; }
+bool grad_aligned(const GradArgs& A) {
+  return rows_aligned(A.dy, A.ldy) && (!A.dw || rows_aligned(A.x, A.ldx)) &&
+         (!A.dx || (rows_aligned(A.w, A.ldw) && A.wg % 8 == 0));
 }
 
 // shared memory of a kernel above 64 KB has to be asked for, once for each device and kernel
@@ -1149,22 +999,14 @@ int row_tiles(const MmArgs& A, int tm) { return (int)(A.counts ? A.M / tm + A.G 
 
 template <int IN>
 int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
-  if (grad_aligned(A.dy, A.ldy, A.x, A.dw ? A.ldx : 0, 0) && grad_aligned(A.dy, A.ldy, A.w, A.dx ? A.ldw : 0, A.dx ? A.wg : 0)) {
-    constexpr int T = 256, lds = 4 * T * kStep;
-    auto* f = grad_kernel<IN>;
-    TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
-    const int64_t ct = (A.K + T - 1) / T, rt = (A.N + T - 1) / T;
-    // (whole rounds over the XCDs, so that both lists of tiles start at the first one)
-    const int64_t dw = A.dw ? (ct * rt * A.G + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + A.G + 1) : 0;
-    TRK_REQUIRE(dw + dx < ((int64_t)1 << 31), "%s: too many tiles", what);
-    f<<<(unsigned)(dw + dx), 512, lds, st>>>(A, dt, ct, rt, dw);
-    return trk::check_launch(what);
-  }
-  const unsigned ct = (unsigned)((A.K + 127) / 128);
-  const int64_t mt = A.M / 128 + A.G + 1, nt = (A.N + 127) / 128;
-  TRK_REQUIRE((!A.dx || mt <= 65535) && (!A.dw || nt <= 65535), "%s: too many row tiles", what);
-  if (A.dx) grouped_dx_kernel<IN><<<dim3(ct, (unsigned)mt), 256, 0, st>>>(A, dt);
-  if (A.dw) grouped_dw_kernel<IN><<<dim3(ct, (unsigned)nt, (unsigned)A.G), 256, 0, st>>>(A, dt);
+  constexpr int T = 256, lds = 4 * T * kStep;
+  auto* f = grad_aligned(A) ? grad_kernel<IN, true> : grad_kernel<IN, false>;
+  TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
+  const int64_t ct = (A.K + T - 1) / T, rt = (A.N + T - 1) / T;
+  // (whole rounds over the XCDs, so that both lists of tiles start at the first one)
+  const int64_t dw = A.dw ? (ct * rt * A.G + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + A.G + 1) : 0;
+  TRK_REQUIRE(dw + dx < ((int64_t)1 << 31), "%s: too many tiles", what);
+  f<<<(unsigned)(dw + dx), 512, lds, st>>>(A, dt, ct, rt, dw);
   return trk::check_launch(what);
 }
 
@@ -1196,11 +1038,11 @@ int cu_count() {
   return cus;
 }
 
-template <int IN, bool WROW, int T, int WN, int WM>
+template <int IN, bool WROW, bool DMA, int T, int WN, int WM>
 int launch_tile(const char* what, const MmArgs& A, int dt, int cus, hipStream_t st) {
-  constexpr int BT = WN * WM * 64, NB = 2;
-  constexpr int lds = NB * (2 * T * kStep + (is8(IN) ? (2 * T + BT - 1) / BT * BT * 4 : 0));
-  auto* f = mm_tile_kernel<IN, WROW, T, T, WN, WM, NB>;
+  constexpr int BT = WN * WM * 64;
+  constexpr int lds = 2 * (2 * T * kStep + (is8(IN) ? (2 * T + BT - 1) / BT * BT * 4 : 0));
+  auto* f = mm_tile_kernel<IN, WROW, DMA, T, T, WN, WM>;
   TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
   const int64_t nt = (A.N + T - 1) / T, mt = row_tiles(A, T);
   TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
@@ -1225,25 +1067,23 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
     if (s32 <= 1024 && 7 * s32 <= 11 * s64) return launch_few<IN, WROW, 2>(what, A, dt, st);
     if (s64 <= 512) return launch_few<IN, WROW, 4>(what, A, dt, st);
   }
-  if (aligned) {
-    // 256-tiles where whole ones alone fill the CUs (2048 x 8192 x 1024 in 8 bits 23.2 us against 25.8 with 128-tiles;
-    // 1024 x 8192 x 1024 20.2 against 15.2; 64 groups of 8 rows x 2048 x 2048 70 against 48).  f32
-    // outputs have wider fragments, which only leave room for 128-tiles.
-    if constexpr (IN != IN_E4M3X) {
-      if ((A.N + 255) / 256 * (A.M / 256) >= cus) return launch_tile<IN, WROW, 256, 2, 4>(what, A, dt, cus, st);
+  // 256-tiles where whole ones alone fill the CUs (2048 x 8192 x 1024 in 8 bits 23.2 us against 25.8 with 128-tiles;
+  // 1024 x 8192 x 1024 20.2 against 15.2; 64 groups of 8 rows x 2048 x 2048 70 against 48).  f32 outputs
+  // have wider fragments, and unaligned 8-bit rows are held in registers on their way: both leave room
+  // for 128-tiles only.
+  if constexpr (IN != IN_E4M3X) {
+    if ((A.N + 255) / 256 * (A.M / 256) >= cus) {
+      if (aligned) return launch_tile<IN, WROW, true, 256, 2, 4>(what, A, dt, cus, st);
+      if constexpr (!is8(IN)) return launch_tile<IN, WROW, false, 256, 2, 4>(what, A, dt, cus, st);
     }
-    return launch_tile<IN, WROW, 128, 2, 2>(what, A, dt, cus, st);
   }
-  const int mt = row_tiles(A, 128);
-  TRK_REQUIRE(mt <= 65535, "%s: too many row tiles (%d)", what, mt);
-  mm_kernel<IN, WROW><<<dim3((unsigned)((A.N + 127) / 128), (unsigned)mt), 256, 0, st>>>(A, dt);
-  return trk::check_launch(what);
+  return aligned ? launch_tile<IN, WROW, true, 128, 2, 2>(what, A, dt, cus, st)
+                 : launch_tile<IN, WROW, false, 128, 2, 2>(what, A, dt, cus, st);
 }
 
 int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const bool al = A.K >= 128 && aligned16_ptr(A.x) && aligned16_ptr(A.w) && A.ldx % 16 == 0 && A.ldw % 16 == 0 && A.wg % 16 == 0 &&
-                  A.ldx < (1 << 23) && A.ldw < (1 << 23);  // offsets inside a tile are 32 bits
+  const bool al = aligned16_ptr(A.x) && aligned16_ptr(A.w) && A.ldx % 16 == 0 && A.ldw % 16 == 0 && A.wg % 16 == 0;
   if (in == IN_E4M3 && dt == TRK_F32)
     return wrow ? launch_tiles<IN_E4M3X, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3X, false>(what, A, dt, al, st);
   if (in == IN_E4M3) return wrow ? launch_tiles<IN_E4M3, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3, false>(what, A, dt, al, st);
@@ -1303,6 +1143,10 @@ int trk_matmul_grouped_bwd(const void* dy, int64_t ldy, const void* x, int64_t l
   TRK_REQUIRE(M == 0 || N == 0 || ((!dx || w) && (!dw || x)), "%s: null pointer", what);
   TRK_REQUIRE(ldy >= N && (!dx || (ldw >= K && lddx >= K)) && (!dw || (ldx >= K && lddw >= K)),
               "%s: row stride below the row's length", what);
+  if (ldy >= (1 << 23) || (dx && ldw >= (1 << 23)) || (dw && ldx >= (1 << 23))) {
+    set_error("%s: row strides of 16 MiB and more are not supported", what);
+    return TRK_EUNSUPPORTED;
+  }
   const GradArgs A{(const uint16_t*)dy, (const uint16_t*)x, (const uint16_t*)w, dx, dw, counts, ldy, ldx, ldw, wg, lddx,
                    lddw, dwg, M, N, K, G};
   hipStream_t st = (hipStream_t)stream;

@@ -388,6 +388,29 @@ def test_matmul_fp8(trk, gpu, M, N, K, block):
             assert float((y.double() - want).norm() / want.norm()) <= 0.75 * HALF[y.dtype] + (0 if y.dtype != F32 else 2.0 ** -20)
 
 
+# sizes that run as 128-tiles and (the last three) as 256-tiles: whole tiles, ragged edges, part steps, odd rows
+TILES = [(700, 1100, 16), (640, 1280, 128), (769, 1025, 300), (1000, 900, 272), (900, 1000, 131), (4096, 4096, 256),
+         (4100, 4200, 96), (4099, 4097, 277)]
+
+
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_matmul_fp8_tiles(trk, gpu, M, N, K, block):
+    g = gen_of(gpu, M, N, K, 7)
+    x, sx = codes_of(g, M, K, 1, gpu)
+    w, sw = codes_of(g, N, K, block, gpu)
+    xv, wv = widen(x, sx, 1), widen(w, sw, block)
+    bias = torch.randn(N, device=gpu, generator=g)
+    want = xv @ wv.t() + bias.double()
+    for dtype in (BF, F32):
+        y = trk.matmul_fp8(x, sx, w, sw, bias=bias, out_dtype=dtype)
+        near(y, want, dtype, product_slack(xv, wv, sx.shape[1], dtype) + want.abs() * 2 * U)
+        if K % 16:  # the same rows, padded to 16 bytes
+            px, pw = (torch.nn.functional.pad(t.view(torch.uint8), (0, -K % 16)).view(FP8)[:, :K] for t in (x, w))
+            assert torch.equal(trk.matmul_fp8(px, sx, pw, sw, bias=bias, out_dtype=dtype), y)
+
+
 @gpu_test
 def test_matmul_fp8_layouts(trk, gpu):
     """rows inside wider buffers (aligned and not), scales of other strides, an output inside a wider one"""
@@ -487,6 +510,51 @@ def test_matmul_grouped_and_gradients(trk, gpu, counts, dtype):
             trk.matmul_grouped(x, w, c, out=out[:, 1:-2])
             assert torch.equal(out[:end, 1:-2], y[:end]) and (out[end:] == 9).all()
             assert (out[:, 0] == 9).all() and (out[:, -2:] == 9).all()
+
+
+BIG = [([700, 0, 513, 1200, 1], 300, 200), ([0, 2500], 333, 129), ([300] * 9, 640, 64), ([1, 7000, 0, 300, 500], 2100, 136),
+       ([2000, 2048, 3500], 2304, 100)]
+
+
+@gpu_test
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8 1", "fp8 128"])
+@pytest.mark.parametrize("counts,N,K", BIG, ids=lambda c: str(len(c)) + "g" if isinstance(c, list) else str(c))
+def test_matmul_grouped_tiles(trk, gpu, counts, N, K, kind):
+    g = gen_of(gpu, sum(counts), N, K)
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    rows = sum(counts) + 77
+    end = sum(counts)
+    if kind in ("bf16", "f16"):
+        dtype = BF if kind == "bf16" else F16
+        for k in (K, K + 1):  # aligned rows (if K is), rows that start anywhere
+            x = torch.randn(rows, k, device=gpu, generator=g).to(dtype).requires_grad_()
+            w = torch.randn(len(counts), N, k, device=gpu, generator=g).to(dtype).requires_grad_()
+            dy = torch.randn(rows, N, device=gpu, generator=g).to(dtype)
+            y = trk.matmul_grouped(x, w, c)
+            dx, dw = torch.autograd.grad(y, (x, w), dy)
+            with torch.no_grad():
+                want, slack, _ = grouped64(x, w, counts)
+                near(y, want, dtype, slack * (k + 4) * U)
+                wx, sx, _ = grouped64(dy, w.transpose(1, 2), counts)
+                near(dx, wx, dtype, sx * (N + 4) * U)
+                for i, (a, b) in enumerate(bounds_of(counts, rows)[0]):
+                    d, v = dy[a:b].double(), x[a:b].double()
+                    near(dw[i], d.t() @ v, dtype, (d.abs().t() @ v.abs()) * (b - a + 4) * U)
+                assert (y[end:] == 0).all() and (dx[end:] == 0).all()
+        return
+    block = int(kind.split()[1])
+    x, sx = codes_of(g, rows, K, 1, gpu)
+    w, sw = codes_of(g, N, K, block, gpu, (len(counts),))
+    xv, wv = widen(x, sx, 1), widen(w, sw, block)
+    want, _, _ = grouped64(xv, wv, counts)
+    for dtype in (BF, F32):
+        slack = torch.zeros_like(want)
+        for i, (a, b) in enumerate(bounds_of(counts, rows)[0]):
+            slack[a:b] = product_slack(xv[a:b], wv[i], sx.shape[1], dtype)
+        out = torch.full((rows, N), 9.0, device=gpu, dtype=dtype)
+        trk.matmul_grouped(x, w, c, x_scale=sx, w_scale=sw, out=out)
+        near(out[:end], want[:end], dtype, slack[:end] + want[:end].abs() * 2 * U)
+        assert (out[end:] == 9).all()
 
 
 @gpu_test
