@@ -278,7 +278,9 @@ def _plain(s):
 
 # -------------------------------------------------------------------------------- the package's calls
 def _kernels(s):
-    trk = importlib.import_module(PACKAGE)
+    trk = getattr(_kernels, "package", None)  # a program imports it once, not at every call
+    if trk is None:
+        trk = _kernels.package = importlib.import_module(PACKAGE)
     case = s["case"]
     op = case["op"]
     if op == "quant":
