@@ -12,6 +12,7 @@
 // two 16x16x32 16-bit matrix instructions a tile).  Which k a lane's bytes hold does not matter
 // as long as both operands agree: a lane of group g = lane / 16 takes the 16-byte chunks g and
 // g + 4 of its row.
+#include <atomic>
 #include <type_traits>
 
 #include "trk_common.h"
@@ -989,10 +990,28 @@ bool grad_aligned(const GradArgs& A) {
          (!A.dx || (rows_aligned(A.w, A.ldw) && A.wg % 8 == 0));
 }
 
-// shared memory of a kernel above 64 KB has to be asked for, once for each device and kernel
+// Facts of the current device, asked for once each: its CUs, and that a kernel F may have more than 64 KB of
+// shared memory.
+struct Device {
+  int id = 0, cus = 256;
+};
+Device current_device() {
+  static std::atomic<int> known[64];
+  Device d;
+  if (hipGetDevice(&d.id) != hipSuccess) d.id = 0;
+  int n = d.id < 64 ? known[d.id].load(std::memory_order_relaxed) : 0;
+  if (n == 0 && hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, d.id) == hipSuccess && d.id < 64)
+    known[d.id].store(n, std::memory_order_relaxed);
+  if (n > 0) d.cus = n;
+  return d;
+}
 template <typename F>
-bool allow_lds(F* f, int bytes) {
-  return hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+bool allow_lds(F* f, int bytes, const Device& d, std::atomic<uint64_t>& allowed) {
+  const uint64_t bit = d.id < 64 ? 1ull << d.id : 0;
+  if (bit & allowed.load(std::memory_order_relaxed)) return true;
+  if (hipFuncSetAttribute((const void*)f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+  allowed.fetch_or(bit, std::memory_order_relaxed);
+  return true;
 }
 
 int row_tiles(const MmArgs& A, int tm) { return (int)(A.counts ? A.M / tm + A.G + 1 : (A.M + tm - 1) / tm); }
@@ -1000,8 +1019,10 @@ int row_tiles(const MmArgs& A, int tm) { return (int)(A.counts ? A.M / tm + A.G 
 template <int IN>
 int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
   constexpr int T = 256, lds = 4 * T * kStep;
-  auto* f = grad_aligned(A) ? grad_kernel<IN, true> : grad_kernel<IN, false>;
-  TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
+  static std::atomic<uint64_t> allowed[2];
+  const bool al = grad_aligned(A);
+  auto* f = al ? grad_kernel<IN, true> : grad_kernel<IN, false>;
+  TRK_REQUIRE(allow_lds(f, lds, current_device(), allowed[al]), "%s: %d bytes of shared memory are not available", what, lds);
   const int64_t ct = (A.K + T - 1) / T, rt = (A.N + T - 1) / T;
   // (whole rounds over the XCDs, so that both lists of tiles start at the first one)
   const int64_t dw = A.dw ? (ct * rt * A.G + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + A.G + 1) : 0;
@@ -1031,29 +1052,23 @@ int launch_few(const char* what, const MmArgs& A, int dt, hipStream_t st) {
   return trk::check_launch(what);
 }
 
-int cu_count() {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
-    cus = 256;
-  return cus;
-}
-
 template <int IN, bool WROW, bool DMA, int T, int WN, int WM>
-int launch_tile(const char* what, const MmArgs& A, int dt, int cus, hipStream_t st) {
+int launch_tile(const char* what, const MmArgs& A, int dt, const Device& dev, hipStream_t st) {
+  static std::atomic<uint64_t> allowed{0};
   constexpr int BT = WN * WM * 64;
   constexpr int lds = 2 * (2 * T * kStep + (is8(IN) ? (2 * T + BT - 1) / BT * BT * 4 : 0));
   auto* f = mm_tile_kernel<IN, WROW, DMA, T, T, WN, WM>;
-  TRK_REQUIRE(allow_lds(f, lds), "%s: %d bytes of shared memory are not available", what, lds);
+  TRK_REQUIRE(allow_lds(f, lds, dev, allowed), "%s: %d bytes of shared memory are not available", what, lds);
   const int64_t nt = (A.N + T - 1) / T, mt = row_tiles(A, T);
   TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
-  const int64_t grid = std::min<int64_t>(nt * mt, (int64_t)cus * (BT == 256 ? 2 : 1) / 8 * 8);
+  const int64_t grid = std::min<int64_t>(nt * mt, (int64_t)dev.cus * (BT == 256 ? 2 : 1) / 8 * 8);
   f<<<(unsigned)grid, BT, lds, st>>>(A, dt, (int)nt, (int)mt);
   return trk::check_launch(what);
 }
 
 template <int IN, bool WROW>
 int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStream_t st) {
-  const int cus = cu_count();
+  const Device dev = current_device();
   // CHOICE
   // Few strips of 16 JT rows x 16 columns: straight from memory to registers, 16 rows a strip while there
   // are at most 256, else the fewest strips by the work of one (1, 1.4 and 2.2 for 16, 32 and 64 rows).
@@ -1072,13 +1087,13 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
   // have wider fragments, and unaligned 8-bit rows are held in registers on their way: both leave room
   // for 128-tiles only.
   if constexpr (IN != IN_E4M3X) {
-    if ((A.N + 255) / 256 * (A.M / 256) >= cus) {
-      if (aligned) return launch_tile<IN, WROW, true, 256, 2, 4>(what, A, dt, cus, st);
-      if constexpr (!is8(IN)) return launch_tile<IN, WROW, false, 256, 2, 4>(what, A, dt, cus, st);
+    if ((A.N + 255) / 256 * (A.M / 256) >= dev.cus) {
+      if (aligned) return launch_tile<IN, WROW, true, 256, 2, 4>(what, A, dt, dev, st);
+      if constexpr (!is8(IN)) return launch_tile<IN, WROW, false, 256, 2, 4>(what, A, dt, dev, st);
     }
   }
-  return aligned ? launch_tile<IN, WROW, true, 128, 2, 2>(what, A, dt, cus, st)
-                 : launch_tile<IN, WROW, false, 128, 2, 2>(what, A, dt, cus, st);
+  return aligned ? launch_tile<IN, WROW, true, 128, 2, 2>(what, A, dt, dev, st)
+                 : launch_tile<IN, WROW, false, 128, 2, 2>(what, A, dt, dev, st);
 }
 
 int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t, void* stream) {

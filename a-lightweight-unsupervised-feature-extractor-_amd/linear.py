@@ -70,30 +70,37 @@ def _type(t: torch.Tensor, of: dict, what: str, name: str) -> int:
     return dt
 
 
-def _same(x: torch.Tensor, t: torch.Tensor, what: str, name: str):
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == x.get_device()):
-        _need_gpu(t, what)
-        raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
+def _on(x: torch.Tensor, what: str) -> int:
+    """index of the device x is on"""
+    if not isinstance(x, torch.Tensor) or x.get_device() < 0:
+        _need_gpu(x, what)
+    return x.get_device()
+
+
+def _elsewhere(x: torch.Tensor, t: torch.Tensor, what: str, name: str):
+    """error of a tensor that is not on x's device"""
+    _need_gpu(t, what)
+    raise ValueError(f"{what}: {name} is on {t.device}, x on {x.device}")
 
 
 def _no_grad(what: str, *ts):
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                raise NotImplementedError(f"{what}: the 8-bit form has no gradient; call it under torch.no_grad()")
+    for t in ts:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError(f"{what}: the 8-bit form has no gradient; call it under torch.no_grad()")
 
 
 def _rows(t: torch.Tensor):
     """(t [.., D] as [R, D] with unit column stride and a row stride >= D, that stride); a view where t allows it"""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t, t.shape[1] or 1
     R, D = t.shape
-    if not t.is_contiguous():
-        if (D > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < D):
-            t = t.contiguous()
-        elif R > 1:
-            return t, t.stride(0)
-    return t, D if D else 1
+    if (D > 1 and t.stride(1) != 1) or (R > 1 and t.stride(0) < D):
+        t = t.contiguous()
+    elif R > 1:
+        return t, t.stride(0)
+    return t, D or 1
 
 
 def _at(t: Optional[torch.Tensor]):
@@ -109,18 +116,22 @@ def _codes(shape, x):
 
 # ------------------------------------------------------------------------------------------- norm
 def _norm_inputs(what, x, weight, residual, eps):
-    _need_gpu(x, what)
-    dt = _type(x, _FLOAT, what, "x")
+    dev = _on(x, what)
+    dt = _FLOAT.get(x.dtype)
+    if dt is None:
+        _type(x, _FLOAT, what, "x")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must be [.., D] with D >= 1")
     if weight is not None:
-        _same(x, weight, what, "weight")
+        if weight.get_device() != dev:
+            _elsewhere(x, weight, what, "weight")
         if weight.dtype != x.dtype:
             raise TypeError(f"{what}: weight is {weight.dtype}, x {x.dtype}")
         if weight.dim() != 1 or weight.shape[0] != x.shape[-1]:
             raise ValueError(f"{what}: weight must be [{x.shape[-1]}], got {list(weight.shape)}")
     if residual is not None:
-        _same(x, residual, what, "residual")
+        if residual.get_device() != dev:
+            _elsewhere(x, residual, what, "residual")
         if residual.dtype != x.dtype:
             raise TypeError(f"{what}: residual is {residual.dtype}, x {x.dtype}")
         if residual.shape != x.shape:
@@ -188,8 +199,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
     residual (y, h): h is what the next layer adds to.  Sums are f32, the norm is of the unrounded f32
     sum; y and h are rounded once.  Differentiable in all three inputs, and through both outputs."""
     dt = _norm_inputs("rms_norm", x, weight, residual, eps)
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
+    if (x.requires_grad or (weight is not None and weight.requires_grad) or
+            (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
         return _RmsNorm.apply(x, weight, residual, dt, eps)
     y, h, _ = _norm_forward(dt, x, weight, residual, eps, False)
     return y if h is None else (y, h)
@@ -227,8 +238,10 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
     even).  NaN values keep a NaN code and are left out of the maximum; a block that holds an infinity has an
     infinite scale, so that all of it reads back as NaN."""
     what = "quantize_fp8"
-    _need_gpu(x, what)
-    dt = _type(x, _FLOAT, what, "x")
+    _on(x, what)
+    dt = _FLOAT.get(x.dtype)
+    if dt is None:
+        _type(x, _FLOAT, what, "x")
     if block_rows not in (1, 128):
         raise ValueError(f"{what}: block_rows must be 1 or 128")
     if x.dim() not in (2, 3) or x.shape[-1] < 1:
@@ -250,19 +263,19 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
 
 
 # ---------------------------------------------------------------------------------------- products
-def _scales(what, t, name, x, rows, kb, lead=()):
-    """(block_rows, strides) of the scales of a [.., rows, K] operand"""
+def _scales(what, t, name, x, dev, shape, few):
+    """rows of a block (1 or 128) of the scales of an operand: shape has one for each row, `few` one for 128"""
     if t is None:
         raise TypeError(f"{what}: {name} is required with 8-bit operands")
-    _same(x, t, what, name)
+    if t.get_device() != dev:
+        _elsewhere(x, t, what, name)
     if t.dtype != torch.float32:
         raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
-    few = (rows + 127) // 128
-    if t.shape == (*lead, rows, kb):
+    if t.shape == shape:
         return 1
-    if t.shape == (*lead, few, kb):
+    if few is not None and t.shape == few:
         return 128
-    raise ValueError(f"{what}: {name} must be {[*lead, rows, kb]} or {[*lead, few, kb]}, got {list(t.shape)}")
+    raise ValueError(f"{what}: {name} must be {list(shape)}{f' or {list(few)}' if few else ''}, got {list(t.shape)}")
 
 
 def _out(what, out, out_dtype, x, M, N, default):
@@ -271,7 +284,8 @@ def _out(what, out, out_dtype, x, M, N, default):
         if dt not in _FLOAT:
             raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {dt}")
         return x.new_empty((M, N), dtype=dt)
-    _same(x, out, what, "out")
+    if out.get_device() != x.get_device():
+        _elsewhere(x, out, what, "out")
     _type(out, _FLOAT, what, "out")
     if out_dtype is not None and out.dtype != out_dtype:
         raise TypeError(f"{what}: out is {out.dtype}, out_dtype {out_dtype}")
@@ -292,8 +306,9 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     (bfloat16 by default; float16, float32).  out: written in place of a new tensor (it must not overlap an
     input)."""
     what = "matmul_fp8"
-    _need_gpu(x, what)
-    _same(x, w, what, "w")
+    dev = _on(x, what)
+    if w.get_device() != dev:
+        _elsewhere(x, w, what, "w")
     if x.dtype != FP8 or w.dtype != FP8:
         raise TypeError(f"{what}: x and w must be float8_e4m3fn, got {x.dtype} and {w.dtype}")
     if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1]:
@@ -301,12 +316,12 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     M, K = x.shape
     N = w.shape[0]
     kb = (K + 127) // 128
+    _scales(what, x_scale, "x_scale", x, dev, (M, kb), None)
+    wb = _scales(what, w_scale, "w_scale", x, dev, (N, kb), ((N + 127) // 128, kb))
     _no_grad(what, x_scale, w_scale, bias)
-    if _scales(what, x_scale, "x_scale", x, M, kb) != 1:
-        raise ValueError(f"{what}: x_scale must be [{M}, {kb}]")
-    wb = _scales(what, w_scale, "w_scale", x, N, kb)
     if bias is not None:
-        _same(x, bias, what, "bias")
+        if bias.get_device() != dev:
+            _elsewhere(x, bias, what, "bias")
         if bias.dtype != torch.float32 or bias.dim() != 1 or bias.shape[0] != N:
             raise ValueError(f"{what}: bias must be float32 [{N}]")
         bias = bias.contiguous()
@@ -377,9 +392,11 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
     (x's type, or bfloat16 for 8 bits; float16, float32).  Rows behind the last group are zeros in a new y;
     with `out` they are left as they were."""
     what = "matmul_grouped"
-    _need_gpu(x, what)
-    _same(x, w, what, "w")
-    _same(x, counts, what, "counts")
+    dev = _on(x, what)
+    if w.get_device() != dev:
+        _elsewhere(x, w, what, "w")
+    if counts.get_device() != dev:
+        _elsewhere(x, counts, what, "counts")
     if x.dtype != w.dtype:
         raise TypeError(f"{what}: x is {x.dtype}, w {w.dtype}")
     if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2] or w.shape[0] < 1:
@@ -390,19 +407,20 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
         raise ValueError(f"{what}: counts must be int32 [{G}]")
     counts = counts.contiguous()
     if x.dtype == FP8:
-        _no_grad(what, x_scale, w_scale)
         kb = (K + 127) // 128
-        if _scales(what, x_scale, "x_scale", x, M, kb) != 1:
-            raise ValueError(f"{what}: x_scale must be [{M}, {kb}]")
-        wb = _scales(what, w_scale, "w_scale", x, N, kb, (G,))
+        _scales(what, x_scale, "x_scale", x, dev, (M, kb), None)
+        wb = _scales(what, w_scale, "w_scale", x, dev, (G, N, kb), (G, (N + 127) // 128, kb))
+        _no_grad(what, x_scale, w_scale)
         y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
         return _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, _lib.TRK_E4M3, y, int(out is None))
     dt = _type(x, _HALF, what, "x")
     if x_scale is not None or w_scale is not None:
         raise TypeError(f"{what}: scales go with float8_e4m3fn operands only")
-    y = _out(what, out, out_dtype, x, M, N, x.dtype)
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         if out is not None:
             raise ValueError(f"{what}: `out` has no gradient; call without it, or under torch.no_grad()")
-        return _Grouped.apply(x, w, counts, dt, y.dtype)
+        if out_dtype is not None and out_dtype not in _FLOAT:
+            raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {out_dtype}")
+        return _Grouped.apply(x, w, counts, dt, out_dtype or x.dtype)
+    y = _out(what, out, out_dtype, x, M, N, x.dtype)
     return _grouped_forward(what, x, None, w, None, 128, counts, dt, y, int(out is None))
