@@ -208,6 +208,8 @@ __device__ __forceinline__ void pair_lines(uint4& a, uint4& b, bool low) {
   turn(a.w, b.w);
 }
 
+constexpr int kRowsLds = 16 * 68 * 4;  // shared memory of a wave's 16 rows x 64 columns on their way out
+
 // A wave's IT x JT tiles of 16 x 16: columns wn + 16 i + 4 lg .. + 3 of rows wm + 16 j + lr, of a tile with
 // `rows` rows and `cols` columns at y (row stride ld).  bias: of the tile's columns, or null.
 // 16-bit rows: lanes of odd and even lg swap halves of two neighbouring column tiles, so that a lane
@@ -215,7 +217,7 @@ __device__ __forceinline__ void pair_lines(uint4& a, uint4& b, bool low) {
 // runs are then paired to lines.
 template <int IT, int JT>
 __device__ __forceinline__ void store_tiles(const f4v (&acc)[IT][JT], void* y, int dt, int64_t at, int64_t ld, int rows,
-                                            int cols, int wn, int wm, int lr, int lg, const float* bias) {
+                                            int cols, int wn, int wm, int lr, int lg, const float* bias, uint8_t* lds) {
   asm volatile("" : "+v"(lr), "+v"(lg));  // addresses are made here, not kept through the loops before
   by_type(dt, [&](auto t) {
     constexpr int DT = decltype(t)::value;
@@ -229,7 +231,42 @@ __device__ __forceinline__ void store_tiles(const f4v (&acc)[IT][JT], void* y, i
         for (int e = 0; e < 4; ++e) b[e] = n + e < cols ? bias[n + e] : 0.0f;
       return b;
     };
-    if (wn + IT * 16 <= cols) {  // the wave's columns are all there
+    // Rows that start anywhere: 64 columns of 16 rows at a time through the wave's own LDS, so that each
+    // store is of one row's neighbouring columns.  2048 x 50000 x 128 to f32 (rows 64 bytes off the lines): 102 us
+    // against 125 with the pieces below (92 for the whole lines of 50048 columns); 50001 columns: 107
+    // against 181, in 16 bits 77 against 104.
+    const bool lines = DT == TRK_F32 ? ((uintptr_t)tile | (uintptr_t)(ld * 4)) % 128 == 0
+                                     : ((uintptr_t)tile | (uintptr_t)(ld * 2)) % 16 == 0;
+    if (!lines) {
+      constexpr int P = DT == TRK_F32 ? 68 : 72;  // elements of a row there (padded against bank conflicts)
+      E* own = (E*)lds;
+      const int lane = lg * 16 + lr;
+#pragma unroll
+      for (int h = 0; h < IT; h += 4) {
+        f4v b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = column_bias(h + i);
+        const int n = wn + h * 16 + lane;
+#pragma unroll
+        for (int j = 0; j < JT; ++j) {
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const f4v v = acc[h + i][j] + b[i];
+            if constexpr (DT == TRK_F32) *(f4v*)(own + lr * P + i * 16 + lg * 4) = v;
+            else *(uint2*)(own + lr * P + i * 16 + lg * 4) = pack4<DT>(v);
+          }
+          __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations keep their order)
+          const int left = rows - wm - j * 16;
+          if (n < cols) {
+            E* to = tile + (int64_t)(wm + j * 16) * ld + n;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (r < left) to[r * ld] = own[r * P + lane];
+          }
+        }
+      }
+    } else if (wn + IT * 16 <= cols) {  // the wave's columns are all there
       constexpr int RUN = DT == TRK_F32 ? 1 : 2;  // column tiles of a 64-byte run
       const bool low = lr < 8;
       auto run = [&](int i, int j, const f4v* b) {
@@ -388,10 +425,11 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   constexpr int LX = TM * 8 / BT, LW = TN * 8 / BT, LOADS = LX + LW + LS, PER = (LOADS + IT - 1) / IT;
   static_assert(TM * 8 % BT == 0 && TN * 8 % BT == 0 && TM % 64 == 0, "whole loads");
   static_assert(WROW || 128 % (TN / WN) == 0, "a wave's columns lie in one block of 128");
+  static_assert(WN * WM * kRowsLds <= STAGE && IT % 4 == 0, "stores go through one stage");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   __shared__ int sums[BT / 64];
   __shared__ Runs runs[BT];
-  __shared__ Tile found;
+  __shared__ Tile found[2];  // of this tile and the next, in turn: a wave may be a barrier ahead
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wn = (wave % WN) * (TN / WN), wm = (wave / WN) * (TM / WM), lr = lane & 15, lg = lane >> 4;
   Finder<TM, BT> F;
@@ -416,7 +454,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
     nt = band * 8 + in % width;
     mt = in / width;
   };
-  auto setup = [&](int nt, int mt) {
+  auto setup = [&](int nt, int mt, const Tile& found) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // (as in store_tiles)
     if (A.counts) {
@@ -541,13 +579,13 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
     add(IT - 1);
     if constexpr (decltype(more)::value) keep(nx, hold);
   };
-  auto first_copies = [&](int at) {
+  auto first_copies = [&](uint8_t* __restrict st) __attribute__((always_inline)) {
     if (steps == 0) return;
     const Rsrc xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
     uint4 hold[LX + LW];
 #pragma unroll
-    for (int q = 0; q < LOADS; ++q) copy(q, 0, smem + at * STAGE, xr, wr, hold);
-    keep(smem + at * STAGE, hold);
+    for (int q = 0; q < LOADS; ++q) copy(q, 0, st, xr, wr, hold);
+    keep(st, hold);
   };
 
   int64_t idx = blockIdx.x;
@@ -555,12 +593,12 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   int nt, mt, at = 0;  // at: the stage of the step, 0 or 1
   tile_at(idx, nt, mt);
   if (A.counts) {
-    F.find(A.counts, (int)A.G, A.M, mt, runs, &found);
+    F.find(A.counts, (int)A.G, A.M, mt, runs, found);
     __syncthreads();
   }
-  setup(nt, mt);
-  first_copies(at);
-  while (true) {
+  setup(nt, mt, found[0]);
+  first_copies(smem);
+  for (int turn = 1;; turn ^= 1) {
     {
       const Rsrc xr = rows_at(xb, (rows - 1) * A.ldx + kbytes), wr = rows_at(wb, (cols - 1) * A.ldw + kbytes);
 #pragma unroll
@@ -605,6 +643,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
         at ^= 1;
       }
     }
+    // the tile's end: its stores, through the stage `free` where rows do not suit, behind the next one's copies
     const int64_t y0 = row0 * A.ldy + n0;
     const float* bias = A.bias && grp >= 0 ? A.bias + n0 : nullptr;
     const int yrows = rows, ycols = cols;
@@ -612,15 +651,20 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
     const bool more = idx < total;
     if (more) {
       tile_at(idx, nt, mt);
-      if (A.counts) F.find(A.counts, (int)A.G, A.M, mt, runs, &found);
-      // every wave is done with the last step's stage (and `found` is written)
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      setup(nt, mt);
-      first_copies(at);
+      if (A.counts) F.find(A.counts, (int)A.G, A.M, mt, runs, found + turn);
     }
-    store_tiles(acc, A.y, dt, y0, A.ldy, yrows, ycols, wn, wm, lr, lg, bias);
+    // every wave is done with the last step's stage (and `found` is written)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    auto finish = [&](uint8_t* __restrict st, uint8_t* __restrict free) __attribute__((always_inline)) {
+      if (more) {
+        setup(nt, mt, found[turn]);
+        first_copies(st);
+      }
+      store_tiles(acc, A.y, dt, y0, A.ldy, yrows, ycols, wn, wm, lr, lg, bias, free + wave * kRowsLds);
+    };
+    finish(smem + at * STAGE, smem + (at ^ 1) * STAGE);
     if (!more) break;
   }
 }
@@ -948,7 +992,8 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
     xp += xstep;
     wp += wstep;
   }
-  store_tiles(acc, out, dt, row0 * ldo + c0, ldo, rows, cols, wn, wm, lr, lg, nullptr);
+  __syncthreads();  // every wave is done with the last stage
+  store_tiles(acc, out, dt, row0 * ldo + c0, ldo, rows, cols, wn, wm, lr, lg, nullptr, smem + wave * kRowsLds);
 }
 
 // Both gradients in one grid (dw's tiles first): the workgroups that find no more tiles of the one
