@@ -349,20 +349,28 @@ struct QuantArgs {
   int64_t ldx, ldq, sld, R, D, xb, qb, sb;  // xb, qb, sb: strides of the batch
 };
 
-// 1 x 128 blocks: 16 lanes each
+// 1 x 128 blocks: 16 lanes each, kUnits blocks one after the other (their loads in flight together)
+constexpr int kUnits = 4;
 template <int DT>
 __global__ __launch_bounds__(256) void quant_rows_kernel(QuantArgs A) {
   typedef typename El<DT>::T E;
   const int64_t b = blockIdx.z;
-  const int64_t kb = (A.D + 127) >> 7;
-  const int64_t unit = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const bool on = unit < A.R * kb;
-  const int64_t row = on ? unit / kb : 0, blk = on ? unit % kb : 0;
-  const int64_t c = blk * 128 + (threadIdx.x & 15) * kV, D = on ? A.D : 0;
-  float v[kV];
-  load8<DT>((const E*)A.x + b * A.xb + row * A.ldx + c, D - c, v);
-  if (!on) return;
-  quant8(v, A.q + b * A.qb + row * A.ldq, c, A.D, A.ldq, A.scale + b * A.sb + blk * A.sld + row);
+  const uint32_t kb = (uint32_t)((A.D + 127) >> 7);
+  const int64_t first = (int64_t)blockIdx.x * (16 * kUnits) + (threadIdx.x >> 4), row0 = first / kb;
+  const uint32_t blk0 = (uint32_t)(first - row0 * kb);
+  float v[kUnits][kV];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const uint32_t at = blk0 + 16 * u;
+    const int64_t row = row0 + at / kb, c = (at % kb) * 128 + (threadIdx.x & 15) * kV;
+    load8<DT>((const E*)A.x + b * A.xb + (row < A.R ? row : 0) * A.ldx + c, row < A.R ? A.D - c : 0, v[u]);
+  }
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    const uint32_t at = blk0 + 16 * u, blk = at % kb;
+    const int64_t row = row0 + at / kb, c = blk * 128 + (threadIdx.x & 15) * kV;
+    if (row < A.R) quant8(v[u], A.q + b * A.qb + row * A.ldq, c, A.D, A.ldq, A.scale + b * A.sb + blk * A.sld + row);
+  }
 }
 
 // 128 x 128 blocks: one workgroup each, the block in registers (16 lanes a row, 16 rows a pass)
@@ -526,12 +534,12 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
   TRK_REQUIRE(x && q && scale, "trk_quantize_fp8: null pointer");
   const int64_t kb = (D + 127) / 128, rb = block_rows == 1 ? R : (R + 127) / 128;
   TRK_REQUIRE(ldx >= D && ldq >= D && scale_ld >= rb, "trk_quantize_fp8: row stride below D, or scale_ld too small");
-  TRK_REQUIRE((block_rows == 1 ? (R * kb + 15) / 16 : kb) < ((int64_t)1 << 31) && (block_rows == 1 || rb <= 65535),
+  TRK_REQUIRE((block_rows == 1 ? (R * kb + 63) / 64 : kb) < ((int64_t)1 << 31) && (block_rows == 1 || rb <= 65535),
               "trk_quantize_fp8: too many blocks");
   const QuantArgs A{x, (uint8_t*)q, scale, ldx, ldq, scale_ld, R, D, xb, qb, sb};
   hipStream_t st = (hipStream_t)stream;
   if (block_rows == 1) {
-    const dim3 grid((unsigned)((R * kb + 15) / 16), 1, (unsigned)B);
+    const dim3 grid((unsigned)((R * kb + 16 * kUnits - 1) / (16 * kUnits)), 1, (unsigned)B);
 #define CALL(DT) quant_rows_kernel<DT><<<grid, 256, 0, st>>>(A)
     TRK_BY_TYPE(dtype, CALL);
 #undef CALL
