@@ -356,9 +356,26 @@ def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_ta
     return y
 
 
+def _lay(t: torch.Tensor) -> torch.Tensor:
+    """t [.., K] of 16-bit values with every row at a multiple of 16 bytes: t, or a copy with padded rows"""
+    ld = (t.shape[-1] + 7) // 8 * 8
+    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.new_empty((*t.shape[:-1], ld))[..., :t.shape[-1]].copy_(t)
+
+
+def _pays_to_lay(M: int, N: int, K: int, G: int) -> bool:
+    """Whether rows off the multiples of 16 bytes are copied first.  The product reads them through registers, at
+    a third of the rate (8 groups of 16384 x 1501 x 1203 in all: 239 us against 81 us aligned); the copies cost their
+    bytes and two launches."""
+    return M * N * K > 4_000_000_000 and M * N > 400 * (M + G * N)
+
+
 class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, counts, dt, out_dtype):
+        if _pays_to_lay(x.shape[0], w.shape[1], w.shape[2], w.shape[0]):
+            x, w = _lay(x), _lay(w)
         ctx.save_for_backward(x, w, counts)
         ctx.dt = dt
         y = x.new_empty((x.shape[0], w.shape[1]), dtype=out_dtype)
@@ -372,7 +389,11 @@ class _Grouped(torch.autograd.Function):
         w, ldw = _weights(w)
         M, K = x.shape
         G, N = w.shape[:2]
-        dy, ldy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+        if dy.dtype != x.dtype:
+            dy = dy.to(x.dtype)
+        if _pays_to_lay(M, N, K, G):
+            dy = _lay(dy)
+        dy, ldy = _rows(dy)
         dx = x.new_empty((M, K)) if ctx.needs_input_grad[0] else None
         dw = x.new_empty((G, N, K)) if ctx.needs_input_grad[1] else None
         _launch("matmul_grouped backward", "trk_matmul_grouped_bwd", x, dy.data_ptr(), ldy, x.data_ptr(), ldx, w.data_ptr(), ldw,
@@ -423,4 +444,6 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
             raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {out_dtype}")
         return _Grouped.apply(x, w, counts, dt, out_dtype or x.dtype)
     y = _out(what, out, out_dtype, x, M, N, x.dtype)
+    if _pays_to_lay(M, N, K, G):
+        x, w = _lay(x), _lay(w)
     return _grouped_forward(what, x, None, w, None, 128, counts, dt, y, int(out is None))
