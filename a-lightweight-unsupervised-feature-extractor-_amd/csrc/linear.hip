@@ -1059,7 +1059,11 @@ bool allow_lds(F* f, int bytes, const Device& d, std::atomic<uint64_t>& allowed)
   return true;
 }
 
-int row_tiles(const MmArgs& A, int tm) { return (int)(A.counts ? A.M / tm + A.G + 1 : (A.M + tm - 1) / tm); }
+// row tiles there can be: at most M groups have rows, each with at most one part tile, and the rows behind them
+// have one
+int64_t row_tiles(const MmArgs& A, int tm) {
+  return A.counts ? A.M / tm + std::min(A.G, A.M) + 1 : (A.M + tm - 1) / tm;
+}
 
 template <int IN>
 int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
@@ -1070,8 +1074,8 @@ int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
   TRK_REQUIRE(allow_lds(f, lds, current_device(), allowed[al]), "%s: %d bytes of shared memory are not available", what, lds);
   const int64_t ct = (A.K + T - 1) / T, rt = (A.N + T - 1) / T;
   // (whole rounds over the XCDs, so that both lists of tiles start at the first one)
-  const int64_t dw = A.dw ? (ct * rt * A.G + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + A.G + 1) : 0;
-  TRK_REQUIRE(dw + dx < ((int64_t)1 << 31), "%s: too many tiles", what);
+  const int64_t dw = A.dw ? (ct * rt * A.G + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + std::min(A.G, A.M) + 1) : 0;
+  TRK_REQUIRE(dw + dx < (1 << 23), "%s: too many tiles", what);  // (2^32 threads)
   f<<<(unsigned)(dw + dx), 512, lds, st>>>(A, dt, ct, rt, dw);
   return trk::check_launch(what);
 }

@@ -8,6 +8,8 @@
 //
 // All of them are bound by memory (4-14 operations a value).  A row lives in the registers of
 // the T lanes that own it between its one read and its one write; every statistic is f32.
+#include <type_traits>
+
 #include "trk_common.h"
 
 using namespace trk;
@@ -430,18 +432,32 @@ __global__ __launch_bounds__(256) void quant_tiles_kernel(QuantArgs A) {
 }
 
 template <int DT, bool FP8>
-void launch_norm(const NormArgs& A, hipStream_t st) {
-  const int64_t D = A.D;
+void launch_norm(NormArgs A, hipStream_t st) {
+  const int64_t D = A.D, R = A.R, e = DT == TRK_F32 ? 4 : 2;
+  // at most 2^23 workgroups of 256 a launch (a launch has fewer than 2^32 threads)
+  const int64_t most = ((int64_t)1 << 23) * (D <= 128 ? 16 : D <= 1024 ? 4 : 1);
+  for (int64_t r = 0; r < R; r += most) {
+    A.R = std::min(most, R - r);
 #define TRK_NORM(T, NV, BT, LOOP) \
   rms_norm_kernel<DT, T, NV, BT, FP8, LOOP><<<(unsigned)((A.R + (BT / T) - 1) / (BT / T)), BT, 0, st>>>(A)
-  if (D <= 128) TRK_NORM(16, 1, 256, false);
-  else if (D <= 512) TRK_NORM(64, 1, 256, false);
-  else if (D <= 1024) TRK_NORM(64, 2, 256, false);
-  else if (D <= 2048) TRK_NORM(256, 1, 256, false);
-  else if (D <= 4096) TRK_NORM(256, 2, 256, false);
-  else if (D <= 8192) TRK_NORM(256, 4, 256, false);
-  else TRK_NORM(256, 4, 256, true);
+    if (D <= 128) TRK_NORM(16, 1, 256, false);
+    else if (D <= 512) TRK_NORM(64, 1, 256, false);
+    else if (D <= 1024) TRK_NORM(64, 2, 256, false);
+    else if (D <= 2048) TRK_NORM(256, 1, 256, false);
+    else if (D <= 4096) TRK_NORM(256, 2, 256, false);
+    else if (D <= 8192) TRK_NORM(256, 4, 256, false);
+    else TRK_NORM(256, 4, 256, true);
 #undef TRK_NORM
+    auto next = [&](auto& p, int64_t bytes) {
+      if (p) p = (std::remove_reference_t<decltype(p)>)((uintptr_t)p + bytes);
+    };
+    next(A.x, most * A.ldx * e);
+    next(A.res, most * A.ldr * e);
+    next(A.y, most * A.ldy * (FP8 ? 1 : e));
+    next(A.h, most * A.ldh * e);
+    next(A.rstd, most * 4);
+    next(A.scale, most * 4);
+  }
 }
 
 // workgroups of the backward kernel, each with one partial row of dw
@@ -455,7 +471,7 @@ void launch_bwd(const BwdArgs& A, hipStream_t st) {
   const int64_t D = A.D;
   const unsigned grid = (unsigned)A.parts;
   // rows over more threads before more values a thread: with up to 32 values in each of 256 threads, 12800 rows
-  // of 8000 took 239 us, with 8 in each of 1024 x
+  // of 8000 took 239 us, with 8 in each of 1024 147
 #define TRK_BWD(T, NV, BT, LOOP) rms_norm_bwd_kernel<DT, T, NV, BT, LOOP><<<grid, BT, 0, st>>>(A)
   if (D <= 128) TRK_BWD(16, 1, 256, false);
   else if (D <= 512) TRK_BWD(64, 1, 256, false);
@@ -559,12 +575,12 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
   TRK_REQUIRE(x && q && scale, "trk_quantize_fp8: null pointer");
   const int64_t kb = (D + 127) / 128, rb = block_rows == 1 ? R : (R + 127) / 128;
   TRK_REQUIRE(ldx >= D && ldq >= D && scale_ld >= rb, "trk_quantize_fp8: row stride below D, or scale_ld too small");
-  TRK_REQUIRE((block_rows == 1 ? (R * kb + 63) / 64 : kb) < ((int64_t)1 << 31) && (block_rows == 1 || rb <= 65535),
-              "trk_quantize_fp8: too many blocks");
+  const int64_t groups = block_rows == 1 ? (R * kb + 16 * kUnits - 1) / (16 * kUnits) : kb * rb;
+  TRK_REQUIRE(groups * B < (1 << 24) && (block_rows == 1 || rb <= 65535), "trk_quantize_fp8: too many blocks for a launch");
   const QuantArgs A{x, (uint8_t*)q, scale, ldx, ldq, scale_ld, R, D, xb, qb, sb};
   hipStream_t st = (hipStream_t)stream;
   if (block_rows == 1) {
-    const dim3 grid((unsigned)((R * kb + 16 * kUnits - 1) / (16 * kUnits)), 1, (unsigned)B);
+    const dim3 grid((unsigned)groups, 1, (unsigned)B);
 #define CALL(DT) quant_rows_kernel<DT><<<grid, 256, 0, st>>>(A)
     TRK_BY_TYPE(dtype, CALL);
 #undef CALL

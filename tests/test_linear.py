@@ -171,7 +171,7 @@ def test_refusals(trk, gpu):
 
 
 # ----------------------------------------------------------------------------------------------- norm
-NORM = [(1, 1), (3, 7), (5, 16), (17, 127), (16, 128), (33, 129), (7, 500), (9, 512), (3, 513), (5, 1000), (2, 1024),
+NORM = [(1, 1), (3, 7), (3, 9), (4, 15), (5, 16), (17, 127), (16, 128), (33, 129), (7, 500), (9, 512), (3, 513), (5, 1000), (2, 1024),
         (3, 2047), (2, 2048), (1, 4096), (2, 5001), (2, 8192), (3, 8193), (1, 20001)]
 
 
@@ -582,6 +582,78 @@ def test_matmul_grouped_fp8(trk, gpu, counts, block):
         trk.matmul_grouped(x, w, c, x_scale=sx, w_scale=sw, out=out)
         assert (out[end:] == 9).all()
         near(out[:end], want[:end], BF, slack[BF][:end] + want[:end].abs() * 2 * U)
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, FP8])
+def test_matmul_grouped_empty_groups(trk, gpu, dtype):
+    """many groups and few rows; all groups empty and many rows behind them (they are zeros, or stay as they were)"""
+    g = gen_of(gpu, 33)
+    for G, rows, N, K, used in ((30000, 3, 40, 32, {7: 1, 29999: 2}), (2, 6000, 1100, 128, {}), (3, 70000, 300, 64, {1: 5}),
+                                (5000, 700, 520, 144, {i: 1 for i in range(0, 5000, 10)})):
+        counts = torch.zeros(G, dtype=torch.int32)
+        for i, n in used.items():
+            counts[i] = n
+        end = int(counts.sum())
+        c = counts.to(gpu)
+        x, sx = codes_of(g, rows, K, 1, gpu)
+        w, sw = codes_of(g, N, K, 128, gpu, (G,))
+        more = dict(x_scale=sx, w_scale=sw)
+        if dtype == BF:
+            x, w, more = x.to(BF), w.to(BF), {}
+        y = trk.matmul_grouped(x, w, c, out_dtype=F32, **more)
+        assert y.shape == (rows, N) and (y[end:] == 0).all()
+        at = 0
+        for i, n in used.items():
+            xv, wv = (x[at:at + n].double(), w[i].double()) if dtype == BF else \
+                (widen(x[at:at + n], sx[at:at + n], 1), widen(w[i], sw[i], 128))
+            near(y[at:at + n], xv @ wv.t(), F32, (xv.abs() @ wv.abs().t()) * (K + 8) * U)
+            at += n
+        out = torch.full((rows, N), 3.0, device=gpu)
+        trk.matmul_grouped(x, w, c, out=out, **more)
+        assert torch.equal(out[:end], y[:end]) and (out[end:] == 3).all()
+
+
+@gpu_test
+def test_products_of_turned_operands(trk, gpu):
+    """operands whose columns are not next to each other in memory are laid out first"""
+    g = gen_of(gpu, 34)
+    x, sx = codes_of(g, 40, 256, 1, gpu)
+    w, sw = codes_of(g, 50, 256, 1, gpu)
+    y = trk.matmul_fp8(x, sx, w, sw, out_dtype=F32)
+    assert torch.equal(trk.matmul_fp8(x.t().contiguous().t(), sx, w.t().contiguous().t(), sw, out_dtype=F32), y)
+    assert torch.equal(trk.matmul_fp8(x[:1].expand(40, -1), sx[:1].expand(40, -1), w, sw, out_dtype=F32), y[:1].expand(40, -1))
+    c = torch.tensor([11, 20], device=gpu, dtype=torch.int32)
+    a, b = torch.randn(33, 48, device=gpu, generator=g).to(BF), torch.randn(2, 24, 48, device=gpu, generator=g).to(BF)
+    y = trk.matmul_grouped(a, b, c)
+    assert torch.equal(trk.matmul_grouped(a.t().contiguous().t(), b.transpose(1, 2).contiguous().transpose(1, 2), c), y)
+    assert torch.equal(trk.matmul_grouped(a, b, c.repeat_interleave(2)[::2]), y)
+
+
+@gpu_test
+def test_matmul_grouped_odd_rows_copied(trk, gpu):
+    """sizes whose odd rows are copied to padded ones first: the same bits as rows padded by the caller"""
+    g = gen_of(gpu, 35)
+    counts = [1500, 0, 1600]
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    R, N, K = 3105, 1301, 1111
+    big_x, big_w = (torch.randn(*s, K + 1, device=gpu, generator=g).to(BF) for s in ((R,), (3, N)))
+    dy = torch.randn(R, N, device=gpu, generator=g).to(BF)
+    got = []
+    for x, w in ((big_x[:, :K].contiguous(), big_w[..., :K].contiguous()), (big_x[:, :K], big_w[..., :K])):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = trk.matmul_grouped(x, w, c)
+        got.append((y,) + torch.autograd.grad(y, (x, w), dy))
+        with torch.no_grad():
+            assert torch.equal(trk.matmul_grouped(x, w, c), y)
+    assert all(torch.equal(p, q) for p, q in zip(*got))
+    want, slack, end = grouped64(big_x[:, :K], big_w[..., :K], counts)
+    near(got[0][0].detach(), want, BF, slack * (K + 4) * U)
+    wx, sx, _ = grouped64(dy, big_w[..., :K].transpose(1, 2), counts)
+    near(got[0][1], wx, BF, sx * (N + 4) * U)
+    for i, (a, b) in enumerate(bounds_of(counts, R)[0]):
+        d, v = dy[a:b].double(), big_x[a:b, :K].double()
+        near(got[0][2][i], d.t() @ v, BF, (d.abs().t() @ v.abs()) * (b - a + 4) * U)
 
 
 @gpu_test
