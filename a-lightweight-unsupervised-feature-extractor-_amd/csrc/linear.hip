@@ -380,11 +380,24 @@ __device__ __forceinline__ Frag<IN> frag(const uint8_t* tile, int row, int lg) {
   return f;
 }
 
-// 16 bytes of a row from byte k on, of which `left` exist (the rest 0)
-__device__ __forceinline__ uint4 load16(const uint8_t* p, int64_t left) {
+// 16 bytes at p, of which `left` exist (the rest 0), in a row of `row` bytes that ends with them: a part
+// piece is the row's last 16 bytes, shifted down
+__device__ __forceinline__ uint4 load16(const uint8_t* p, int64_t left, int64_t row) {
   uint4 v = make_uint4(0, 0, 0, 0);
   if (left >= 16) {
     __builtin_memcpy(&v, p, 16);
+  } else if (left > 0 && row >= 16) {
+    const int s = 16 - (int)left;
+    uint64_t t[2];
+    __builtin_memcpy(t, p - s, 16);
+    if (s >= 8) {
+      t[0] = t[1] >> (8 * (s - 8));
+      t[1] = 0;
+    } else {
+      t[0] = t[0] >> (8 * s) | t[1] << (64 - 8 * s);
+      t[1] >>= 8 * s;
+    }
+    __builtin_memcpy(&v, t, 16);
   } else if (left > 0) {
     uint8_t t[16];
 #pragma unroll
@@ -625,12 +638,12 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
 #pragma unroll
           for (int q = 0; q < LX; ++q) {
             const int p = q * BT + t, c = (p & 7) ^ ((p >> 3) & 7);
-            *(uint4*)(d + p * 16) = load16(xb + xoff(q) + k, kbytes - k - c * 16);
+            *(uint4*)(d + p * 16) = load16(xb + xoff(q) + k, kbytes - k - c * 16, kbytes);
           }
 #pragma unroll
           for (int q = 0; q < LW; ++q) {
             const int p = q * BT + t, c = (p & 7) ^ ((p >> 3) & 7);
-            *(uint4*)(d + XB + p * 16) = load16(wb + woff(q) + k, kbytes - k - c * 16);
+            *(uint4*)(d + XB + p * 16) = load16(wb + woff(q) + k, kbytes - k - c * 16, kbytes);
           }
 #pragma unroll
           for (int q = 0; q < LS; ++q) {
@@ -728,11 +741,11 @@ __global__ __launch_bounds__(512) void mm_few_kernel(MmArgs A, int dt) {
         if (kt >= steps) break;
         const int64_t k = (int64_t)kt * kStep, left = kbytes - k - lg * 16;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) a[u][h] = load16(wp + k + h * 64, left - h * 64);
+        for (int h = 0; h < 2; ++h) a[u][h] = load16(wp + k + h * 64, left - h * 64, kbytes);
 #pragma unroll
         for (int j = 0; j < JT; ++j) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) b[u][j][h] = load16(xp[j] + k + h * 64, left - h * 64);
+          for (int h = 0; h < 2; ++h) b[u][j][h] = load16(xp[j] + k + h * 64, left - h * 64, kbytes);
           if constexpr (is8(IN)) s[u][j] = sx[j][kt * A.sx_kb];
         }
         if constexpr (is8(IN)) {
@@ -793,6 +806,8 @@ struct GradArgs {
   const int32_t* counts;
   int64_t ldy, ldx, ldw, wg, lddx, ldo, og;        // elements; ldo, og: rows and groups of dw
   int64_t M, N, K, G;
+  float* part;                                     // [parts][G][N][K]: dw in parts of each group's rows
+  int64_t parts;
 };
 
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -837,7 +852,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
     F.init(A.counts, (int)A.G, A.M, true, sums, runs);
     rtiles = F.all;
   }
-  const int64_t total = ctiles * rtiles * (DW ? A.G : 1);
+  const int64_t total = ctiles * rtiles * (DW ? A.G * A.parts : 1);
   if (block >= total) return;
   // dx: a contiguous run of tiles for each XCD.  dw: a run of every group's tiles for each XCD, because
   // groups differ in length (runs over the groups: 267 us against 215 for 16 groups of 16384 rows)
@@ -855,23 +870,32 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
   int rows;
   const uint16_t *wsrc0, *xsrc0;
   int64_t wld, xld;
-  uint16_t* out = (uint16_t*)(DW ? A.dw : A.dx);
-  const int64_t ldo = DW ? A.ldo : A.lddx;
+  void* out = DW ? A.dw : A.dx;
+  int64_t ldo = DW ? A.ldo : A.lddx, out0 = 0;
   if constexpr (DW) {
-    const int64_t g = rt / rtiles;
+    const int64_t gs = rt / rtiles, g = gs / A.parts, part = gs % A.parts;
     int64_t before = 0;
     for (int64_t i = tid; i < g; i += BT) before = min(before + max(0, A.counts[i]), A.M);
     int end;
     Finder<T, BT>::scan_rows((int)before, sums, (int)A.M, end);
-    const int64_t first = end;
+    int64_t first = end;
     steps_of = min((int64_t)max(0, A.counts[g]), A.M - first);
+    if (A.parts > 1) {  // this part's share of the rows, in whole steps
+      const int64_t share = ((steps_of + 63) / 64 + A.parts - 1) / A.parts * 64, skip = min(part * share, steps_of);
+      first += skip;
+      steps_of = min(share, steps_of - skip);
+      out = A.part + (part * A.G + g) * A.N * A.K;
+      ldo = A.K;
+      dt = TRK_F32;
+    } else {
+      out0 = g * A.og;
+    }
     row0 = (rt % rtiles) * T;
     rows = (int)min((int64_t)T, A.N - row0);
     wsrc0 = A.x + first * A.ldx + c0;
     wld = A.ldx;
     xsrc0 = A.dy + first * A.ldy + row0;
     xld = A.ldy;
-    out += g * A.og;
   } else {
     F.find(A.counts, (int)A.G, A.M, (int)rt, runs, found);
     __syncthreads();
@@ -902,7 +926,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
   // piece q of a turned operand, whose row has `n` columns (without DMA: any alignment, nothing read behind them)
   auto turned_piece = [&](const uint8_t* p, uint32_t off, int q, int n) {
     const int slot = q * BT + tid, c = ((((slot >> 1) & 15) ^ turn_of(slot >> 5)) << 4) + (slot & 1) * 8;
-    return load16(p + off, 2 * (n - c));
+    return load16(p + off, 2 * (n - c), 2 * n);
   };
   auto copy = [&](int q, __amdgpu_buffer_rsrc_t xr, __amdgpu_buffer_rsrc_t wr, uint8_t* d, uint4* hold)
       __attribute__((always_inline)) {
@@ -983,7 +1007,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
           *(uint4*)(d + p * 16) = (p >> 5) >= left ? zero : DMA ? *(const uint4*)(xp + xoff[q]) : turned_piece(xp, xoff[q], q, rows);
         } else {
           const int c = (p & 7) ^ ((p >> 3) & 7);
-          *(uint4*)(d + p * 16) = load16(xp + xoff[q], 2 * (left - c * 8));
+          *(uint4*)(d + p * 16) = load16(xp + xoff[q], 2 * (left - c * 8), 2 * steps_of);
         }
       }
       __syncthreads();
@@ -993,7 +1017,21 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
     wp += wstep;
   }
   __syncthreads();  // every wave is done with the last stage
-  store_tiles(acc, out, dt, row0 * ldo + c0, ldo, rows, cols, wn, wm, lr, lg, nullptr, smem + wave * kRowsLds);
+  store_tiles(acc, out, dt, out0 + row0 * ldo + c0, ldo, rows, cols, wn, wm, lr, lg, nullptr, smem + wave * kRowsLds);
+}
+
+// dw[g][n][k] = sum over the parts, in order
+template <int DT>
+__global__ __launch_bounds__(256) void dw_join_kernel(const float* part, int64_t parts, int64_t G, int64_t N, int64_t K,
+                                                      void* dw, int64_t ldo, int64_t og) {
+  const int64_t each = G * N * K;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < each; i += (int64_t)gridDim.x * 256) {
+    float a = 0.0f;
+#pragma unroll 4
+    for (int64_t p = 0; p < parts; ++p) a += part[p * each + i];
+    const int64_t r = i / K, g = r / N;
+    put<DT>(dw, g * og + (r - g * N) * ldo + (i - r * K), a);
+  }
 }
 
 // Both gradients in one grid (dw's tiles first): the workgroups that find no more tiles of the one
@@ -1074,9 +1112,13 @@ int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
   TRK_REQUIRE(allow_lds(f, lds, current_device(), allowed[al]), "%s: %d bytes of shared memory are not available", what, lds);
   const int64_t ct = (A.K + T - 1) / T, rt = (A.N + T - 1) / T;
   // (whole rounds over the XCDs, so that both lists of tiles start at the first one)
-  const int64_t dw = A.dw ? (ct * rt * A.G + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + std::min(A.G, A.M) + 1) : 0;
+  const int64_t dw = A.dw ? (ct * rt * A.G * A.parts + 7) / 8 * 8 : 0, dx = A.dx ? ct * (A.M / T + std::min(A.G, A.M) + 1) : 0;
   TRK_REQUIRE(dw + dx < (1 << 23), "%s: too many tiles", what);  // (2^32 threads)
   f<<<(unsigned)(dw + dx), 512, lds, st>>>(A, dt, ct, rt, dw);
+  if (A.dw && A.parts > 1) {
+    const unsigned blocks = (unsigned)std::min<int64_t>((A.G * A.N * A.K + 255) / 256, 4096);
+    dw_join_kernel<IN == IN_BF16 ? TRK_BF16 : TRK_F16><<<blocks, 256, 0, st>>>(A.part, A.parts, A.G, A.N, A.K, A.dw, A.ldo, A.og);
+  }
   return trk::check_launch(what);
 }
 
@@ -1192,9 +1234,17 @@ int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_r
                    M / 128 + G + 1, stream);
 }
 
+// Few tiles and many rows: a group's rows are split into parts, so that the tiles fill the CUs, of at least 4 steps
+// of 64 rows on average (3 groups of 9082 rows in all, 121 x 102: 619 us in one part, x in 28).
+int64_t trk_matmul_grouped_bwd_parts(int64_t G, int64_t M, int64_t N, int64_t K) {
+  if (G < 1 || M < 1 || N < 1 || K < 1) return 1;
+  const int64_t tiles = (N + 255) / 256 * ((K + 255) / 256) * G;
+  return std::max<int64_t>(1, std::min(256 / tiles, M / (G * 256)));
+}
+
 int trk_matmul_grouped_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t wg,
                            const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int dtype, void* dx,
-                           int64_t lddx, void* dw, int64_t lddw, int64_t dwg, void* stream) {
+                           int64_t lddx, void* dw, int64_t lddw, int64_t dwg, float* part, int64_t parts, void* stream) {
   const char* what = "trk_matmul_grouped_bwd";
   TRK_REQUIRE(dtype == TRK_BF16 || dtype == TRK_F16, "%s: dtype must be TRK_BF16 or TRK_F16", what);
   TRK_REQUIRE(G >= 1 && G <= 65535 && counts, "%s: 1 to 65535 groups and their counts are required", what);
@@ -1211,8 +1261,9 @@ int trk_matmul_grouped_bwd(const void* dy, int64_t ldy, const void* x, int64_t l
     set_error("%s: row strides of 16 MiB and more are not supported", what);
     return TRK_EUNSUPPORTED;
   }
+  TRK_REQUIRE(parts >= 1 && parts <= 4096 && (parts == 1 || !dw || part), "%s: parts > 1 need the workspace part", what);
   const GradArgs A{(const uint16_t*)dy, (const uint16_t*)x, (const uint16_t*)w, dx, dw, counts, ldy, ldx, ldw, wg, lddx,
-                   lddw, dwg, M, N, K, G};
+                   lddw, dwg, M, N, K, G, part, parts};
   hipStream_t st = (hipStream_t)stream;
   return dtype == TRK_BF16 ? launch_grad<IN_BF16>(what, A, dtype, st) : launch_grad<IN_F16>(what, A, dtype, st);
 }

@@ -39,7 +39,8 @@ _lib.register({
     "trk_matmul_grouped": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I64,
                             _I64, _I, _P, _I64, _I, _I, _P], _I),
     "trk_matmul_grouped_bwd": ([_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _I64,
-                                _I64, _P], _I),
+                                _I64, _P, _I64, _P], _I),
+    "trk_matmul_grouped_bwd_parts": ([_I64, _I64, _I64, _I64], _I64),
 })
 
 FP8 = torch.float8_e4m3fn
@@ -395,9 +396,16 @@ class _Grouped(torch.autograd.Function):
             dy = _lay(dy)
         dy, ldy = _rows(dy)
         dx = x.new_empty((M, K)) if ctx.needs_input_grad[0] else None
-        dw = x.new_empty((G, N, K)) if ctx.needs_input_grad[1] else None
+        dw = part = None
+        parts = 1
+        if ctx.needs_input_grad[1]:
+            dw = x.new_empty((G, N, K))
+            parts = lib().trk_matmul_grouped_bwd_parts(G, M, N, K)
+            if parts > 1:
+                part = x.new_empty((parts, G, N, K), dtype=torch.float32)
         _launch("matmul_grouped backward", "trk_matmul_grouped_bwd", x, dy.data_ptr(), ldy, x.data_ptr(), ldx, w.data_ptr(), ldw,
-                w.stride(0), counts.data_ptr(), G, M, N, K, ctx.dt, _at(dx), max(K, 1), _at(dw), max(K, 1), N * K)
+                w.stride(0), counts.data_ptr(), G, M, N, K, ctx.dt, _at(dx), max(K, 1), _at(dw), max(K, 1), N * K, _at(part),
+                parts)
         return dx, dw, None, None, None
 
 

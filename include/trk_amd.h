@@ -347,7 +347,9 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
  *   left as they were.
  * trk_matmul_grouped_bwd: the 16-bit product's gradients, dx [M][lddx] = dy . w[g] (rows behind
  *   the last group: zeros; NULL: not wanted, w is not read) and dw [G][dwg] = dy_g^T . x_g
- *   (a group without rows: zeros; NULL: not wanted, x is not read). */
+ *   (a group without rows: zeros; NULL: not wanted, x is not read).  parts >= 1: dw is
+ *   summed from so many parts of each group's rows, joined in order, in the workspace part
+ *   [parts][G][N][K] (not read with 1); trk_matmul_grouped_bwd_parts suggests a number. */
 int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
                    int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_kb, int w_block_rows, const float* bias,
                    int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, void* stream);
@@ -357,7 +359,8 @@ int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_r
                        void* y, int64_t ldy, int out_dtype, int zero_tail, void* stream);
 int trk_matmul_grouped_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t wg,
                            const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int dtype, void* dx,
-                           int64_t lddx, void* dw, int64_t lddw, int64_t dwg, void* stream);
+                           int64_t lddx, void* dw, int64_t lddw, int64_t dwg, float* part, int64_t parts, void* stream);
+int64_t trk_matmul_grouped_bwd_parts(int64_t G, int64_t M, int64_t N, int64_t K);
 
 /* ------------------------------------------------------------------------
  * Device-resident track state.  Track slots of all

@@ -117,11 +117,12 @@ def test_host_argument_errors(trk):
     refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, v, 0, 4, 4, 8, 1, v, 4, 1, 0, z), b"groups")
     refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, v, 2, 4, 4, 8, 0, v, 4, 1, 0, z), b"input")
     refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, z, 2, 4, 4, 8, 1, v, 4, 1, 0, z), b"groups")
-    refused(L.trk_matmul_grouped_bwd(v, 4, v, 8, v, 8, 32, v, 2, 4, 4, 8, 0, v, 8, v, 8, 32, z), b"dtype")
-    refused(L.trk_matmul_grouped_bwd(v, 3, v, 8, v, 8, 32, v, 2, 4, 4, 8, 1, v, 8, v, 8, 32, z), b"row stride")
-    refused(L.trk_matmul_grouped_bwd(v, 4, z, 8, v, 8, 32, v, 2, 4, 4, 8, 1, v, 8, v, 8, 32, z), b"null")
-    refused(L.trk_matmul_grouped_bwd(v, 4, v, 8, z, 8, 32, v, 2, 4, 4, 8, 1, v, 8, z, 8, 32, z), b"null")
-    assert L.trk_matmul_grouped_bwd(v, 4, v, 8, v, 8, 32, v, 2, 4, 4, 8, 1, z, 8, z, 8, 32, z) == 0
+    refused(L.trk_matmul_grouped_bwd(v, 4, v, 8, v, 8, 32, v, 2, 4, 4, 8, 0, v, 8, v, 8, 32, z, 1, z), b"dtype")
+    refused(L.trk_matmul_grouped_bwd(v, 3, v, 8, v, 8, 32, v, 2, 4, 4, 8, 1, v, 8, v, 8, 32, z, 1, z), b"row stride")
+    refused(L.trk_matmul_grouped_bwd(v, 4, z, 8, v, 8, 32, v, 2, 4, 4, 8, 1, v, 8, v, 8, 32, z, 1, z), b"null")
+    refused(L.trk_matmul_grouped_bwd(v, 4, v, 8, z, 8, 32, v, 2, 4, 4, 8, 1, v, 8, z, 8, 32, z, 1, z), b"null")
+    refused(L.trk_matmul_grouped_bwd(v, 4, v, 8, v, 8, 32, v, 2, 4, 4, 8, 1, v, 8, v, 8, 32, z, 2, z), b"parts")
+    assert L.trk_matmul_grouped_bwd(v, 4, v, 8, v, 8, 32, v, 2, 4, 4, 8, 1, z, 8, z, 8, 32, z, 1, z) == 0
     # nothing to do
     assert L.trk_rms_norm(z, 8, z, 0, z, 1e-6, 0, 8, 0, z, 8, z, 0, z, z) == 0
     assert L.trk_quantize_fp8(z, 8, 0, 0, 4, 8, 1, 0, z, 8, 0, z, 4, 0, z) == 0
@@ -513,7 +514,7 @@ def test_matmul_grouped_and_gradients(trk, gpu, counts, dtype):
 
 
 BIG = [([700, 0, 513, 1200, 1], 300, 200), ([0, 2500], 333, 129), ([300] * 9, 640, 64), ([1, 7000, 0, 300, 500], 2100, 136),
-       ([2000, 2048, 3500], 2304, 100)]
+       ([2000, 2048, 3500], 2304, 100), ([4000, 0, 5082], 121, 102), ([9000], 64, 64), ([130, 2500, 1], 40, 300)]
 
 
 @gpu_test
