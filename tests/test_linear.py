@@ -285,6 +285,19 @@ def test_norm_gradient_against_differences(trk, gpu):
 
 
 @gpu_test
+def test_no_second_derivative(trk, gpu):
+    """asked for, it is an error and not zero"""
+    x = torch.randn(4, 16, device=gpu, generator=gen_of(gpu, 13)).requires_grad_()
+    a = torch.randn(4, 16, device=gpu, generator=gen_of(gpu, 14)).to(BF).requires_grad_()
+    w = torch.randn(1, 8, 16, device=gpu, generator=gen_of(gpu, 15)).to(BF).requires_grad_()
+    c = torch.tensor([4], device=gpu, dtype=torch.int32)
+    for y, leaf in ((trk.rms_norm(x), x), (trk.matmul_grouped(a, w, c), a)):
+        d, = torch.autograd.grad(y.square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            d.sum().backward()  # (autograd.grad would say that the leaf is not in the graph)
+
+
+@gpu_test
 def test_norm_gradient_uses(trk, gpu):
     """only one output used, gradients of some inputs only, a gradient that is a broadcast"""
     x = torch.randn(9, 130, device=gpu, dtype=F32, generator=gen_of(gpu, 9)).requires_grad_()
