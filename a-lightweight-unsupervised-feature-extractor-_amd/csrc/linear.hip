@@ -740,13 +740,24 @@ __global__ __launch_bounds__(512) void mm_few_kernel(MmArgs A, int dt) {
         const int kt = k0 + u * KW;
         if (kt >= steps) break;
         const int64_t k = (int64_t)kt * kStep, left = kbytes - k - lg * 16;
+        if (k + kStep <= kbytes) {  // the same in every lane
 #pragma unroll
-        for (int h = 0; h < 2; ++h) a[u][h] = load16(wp + k + h * 64, left - h * 64, kbytes);
+          for (int h = 0; h < 2; ++h) {
+            __builtin_memcpy(&a[u][h], wp + k + h * 64, 16);
 #pragma unroll
-        for (int j = 0; j < JT; ++j) {
+            for (int j = 0; j < JT; ++j) __builtin_memcpy(&b[u][j][h], xp[j] + k + h * 64, 16);
+          }
+        } else {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) b[u][j][h] = load16(xp[j] + k + h * 64, left - h * 64, kbytes);
-          if constexpr (is8(IN)) s[u][j] = sx[j][kt * A.sx_kb];
+          for (int h = 0; h < 2; ++h) {
+            a[u][h] = load16(wp + k + h * 64, left - h * 64, kbytes);
+#pragma unroll
+            for (int j = 0; j < JT; ++j) b[u][j][h] = load16(xp[j] + k + h * 64, left - h * 64, kbytes);
+          }
+        }
+        if constexpr (is8(IN)) {
+#pragma unroll
+          for (int j = 0; j < JT; ++j) s[u][j] = sx[j][kt * A.sx_kb];
         }
         if constexpr (is8(IN)) {
 #pragma unroll
