@@ -428,6 +428,16 @@ __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
   return x * per + min(x, more) + id / 8;
 }
 
+// The product.  Bound by the matrix cores at the clock the chip holds under them: 8192 x 8192 x 8192 in 8 bits
+// 457 us (2.4 PFLOP/s; the library's product with one scale for all runs at 2.7, 408 us), matrix instructions busy
+// 59 % of the cycles at 1.8 GHz; in 16 bits 850 us (1.3 PFLOP/s, the library 813).  What brought the 8-bit
+// one there, us: 128-tiles through registers 2064, 256-tiles with straight copies a step ahead 547, copies
+// spread over the step 484, several tiles a workgroup 478, rows of tiles kept in order 424-457.  Tried and
+// dropped: 128 x 256 and 256 x 128 tiles with two or three stages (562-650 us; more bytes to LDS for each
+// operation), four waves of 128 x 128 (949: one wave a SIMD hides nothing), workgroups that start apart and
+// stores that stay in flight into the next tile's first step (no change: a wave is held while its
+// stores are taken in, so a tile of few steps pays for them, about 6 us of 22 at 256 x 256 x 1024).
+//
 // TN x TM tiles, WN x WM waves, operands copied to LDS one step ahead.  DMA: straight, 16 bytes a lane;
 // every row starts at a multiple of 16 bytes.  Else through registers, at any alignment.  A
 // workgroup runs several tiles: the next tile's first copies are sent before a tile's stores.
@@ -684,7 +694,8 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
 
 // ------------------------------------------------------------------ few rows
 // 16 JT rows by 16 columns a wave, the operands straight from memory to registers: with few rows the
-// weights are read once and that is what counts.  KW waves of the 8 share 16 columns, each with
+// weights are read once and that is what counts (16 x 4096 x 4096 in 8 bits 7.1 us, 2.4 TB/s: one round of latencies;
+// 16 x 8192 x 8192 20 us, 3.4 TB/s; 80 rows of 64 groups x 1024 x 1024 in 16 bits 22 us, 6 TB/s).  KW waves of the 8 share 16 columns, each with
 // every KW-th step, and are joined in order through LDS; the others take the next columns.
 // U steps are loaded before they are multiplied.  Any alignment.
 template <int IN, bool WROW, int JT, int KW>
@@ -849,6 +860,10 @@ __device__ __forceinline__ Frag<IN> frag_turned(const uint8_t* tile, uint32_t at
   return f;
 }
 
+// The gradients: 16 groups of 16384 rows in all, 2048 x 2048: both in 328 us (840 TFLOP/s; 2000 us through
+// registers with scalar turns, 390 in two launches).  The last round of tiles and each tile's first copies and
+// stores cost what is missing to the product's rate.
+//
 // T x T tile `block` of dx (DW false: rows m of one group, columns k, contracted over n) or of dw[g] (rows n,
 // columns k, contracted over the group's rows), 8 waves, copies one step of 64 ahead.
 template <int IN, bool DW, bool DMA>
@@ -866,7 +881,7 @@ __device__ __forceinline__ void grad_tile(const GradArgs& A, int dt, int64_t blo
   const int64_t total = ctiles * rtiles * (DW ? A.G * A.parts : 1);
   if (block >= total) return;
   // dx: a contiguous run of tiles for each XCD.  dw: a run of every group's tiles for each XCD, because
-  // groups differ in length (runs over the groups: 267 us against 215 for 16 groups of 16384 rows)
+  // groups differ in length (runs over the groups: dw alone 267 us against 211 for 16 groups of 16384 rows)
   int64_t id = block;
   if constexpr (DW) {
     const int64_t each = ctiles * rtiles;
@@ -1246,7 +1261,8 @@ int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_r
 }
 
 // Few tiles and many rows: a group's rows are split into parts, so that the tiles fill the CUs, of at least 4 steps
-// of 64 rows on average (3 groups of 9082 rows in all, 121 x 102: 619 us in one part, x in 28).
+// of 64 rows on average (3 groups of 9082 rows in all, 121 x 102, with forward and autograd: 619 us in one
+// part, under 110 in 11).
 int64_t trk_matmul_grouped_bwd_parts(int64_t G, int64_t M, int64_t N, int64_t K) {
   if (G < 1 || M < 1 || N < 1 || K < 1) return 1;
   const int64_t tiles = (N + 255) / 256 * ((K + 255) / 256) * G;
