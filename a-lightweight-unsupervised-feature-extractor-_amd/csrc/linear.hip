@@ -29,7 +29,6 @@ typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 
 constexpr int kStep = 128;  // bytes of K a step
-constexpr int kBK = 128;    // columns that share a scale
 
 struct MmArgs {
   const uint8_t *x, *w;      // rows; strides below in bytes
@@ -695,9 +694,10 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
 // ------------------------------------------------------------------ few rows
 // 16 JT rows by 16 columns a wave, the operands straight from memory to registers: with few rows the
 // weights are read once and that is what counts (16 x 4096 x 4096 in 8 bits 7.1 us, 2.4 TB/s: one round of latencies;
-// 16 x 8192 x 8192 20 us, 3.4 TB/s; 80 rows of 64 groups x 1024 x 1024 in 16 bits 22 us, 6 TB/s).  KW waves of the 8 share 16 columns, each with
-// every KW-th step, and are joined in order through LDS; the others take the next columns.
-// U steps are loaded before they are multiplied.  Any alignment.
+// 16 x 8192 x 8192 20 us, 3.4 TB/s; 80 rows of 64 groups x 1024 x 1024 in 16 bits 22 us, 6 TB/s).
+// KW waves of the 8 share 16 columns, each with every KW-th step, and are joined in order through
+// LDS; the others take the next columns.  U steps are loaded before they are multiplied.  Any
+// alignment.
 template <int IN, bool WROW, int JT, int KW>
 __global__ __launch_bounds__(512) void mm_few_kernel(MmArgs A, int dt) {
   constexpr int TM = 16 * JT, NW = 8 / KW, U = JT >= 4 || IN == IN_E4M3X ? 2 : 4;

@@ -431,7 +431,7 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
     theirs), or float8_e4m3fn with x_scale
     [R, ceil(K / 128)] and w_scale [G, N or ceil(N / 128), ceil(K / 128)].  y is rounded once to out_dtype
     (x's type, or bfloat16 for 8 bits; float16, float32).  Rows behind the last group are zeros in a new y;
-    with `out` they are left as they were."""
+    with `out` (which must not overlap an input) they are left as they were."""
     what = "matmul_grouped"
     dev = _on(x, what)
     if w.get_device() != dev:

@@ -549,6 +549,7 @@ def test_matmul_grouped_tiles(trk, gpu, counts, N, K, kind):
             with torch.no_grad():
                 want, slack, _ = grouped64(x, w, counts)
                 near(y, want, dtype, slack * (k + 4) * U)
+                near(trk.matmul_grouped(x, w, c, out_dtype=F32), want, F32, slack * (k + 4) * U)
                 wx, sx, _ = grouped64(dy, w.transpose(1, 2), counts)
                 near(dx, wx, dtype, sx * (N + 4) * U)
                 for i, (a, b) in enumerate(bounds_of(counts, rows)[0]):
