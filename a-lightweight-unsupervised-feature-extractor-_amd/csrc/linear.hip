@@ -40,6 +40,7 @@ struct MmArgs {
   int64_t ldy;               // elements
   int64_t M, N, K, G;        // K in elements
   int zero_tail;             // rows behind the last group are written as zeros
+  int parts, share;          // tiles only: K in so many parts of `share` steps, each with its own y [M][N] (f32)
 };
 
 // ------------------------------------------------------------------ which rows a tile has
@@ -459,19 +460,23 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
     F.init(A.counts, (int)A.G, A.M, A.zero_tail, sums, runs);
     mtiles = __builtin_amdgcn_readfirstlane(F.all);
   }
-  const int64_t total = (int64_t)ntiles * mtiles;
+  const int64_t total = (int64_t)ntiles * mtiles * A.parts;
 
   // the tile that is worked on: its rows, columns and sources
   int64_t row0, n0;
-  int rows, cols, grp, steps, rest;
+  int rows, cols, grp, steps, rest, part;
   int64_t kbytes;
   const uint8_t *xb, *wb;
   uint32_t x0, w0, xend, wend;  // a lane's first piece of its operand's rows, and its piece of the last row
   const float* ssrc[LS > 0 ? LS : 1];
+  int next_part = 0;
   auto tile_at = [&](int64_t idx, int& nt, int& mt) {
     // bands of 8 column tiles, row tiles inside a band one after the other: an XCD's share of the
     // grid at any time is near square, so its L2 serves most operand reads
-    const int id = (int)xcd_run(idx, total), bsize = 8 * mtiles, band = id / bsize, in = id - band * bsize;
+    int id = (int)xcd_run(idx, total);
+    next_part = id % A.parts;
+    id /= A.parts;
+    const int bsize = 8 * mtiles, band = id / bsize, in = id - band * bsize;
     const int width = min(8, ntiles - band * 8);
     nt = band * 8 + in % width;
     mt = in / width;
@@ -490,12 +495,15 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
     }
     n0 = (int64_t)nt * TN;
     cols = (int)min((int64_t)TN, A.N - n0);
-    kbytes = grp < 0 ? 0 : A.K * (is8(IN) ? 1 : 2);
+    part = next_part;
+    const int64_t k0 = (int64_t)part * A.share * kStep;  // (0 where K is whole)
+    kbytes = grp < 0 ? 0 : A.K * (is8(IN) ? 1 : 2) - k0;  // (no part is empty)
+    if (A.parts > 1) kbytes = min(kbytes, (int64_t)A.share * kStep);
     steps = (int)(kbytes / kStep);
     rest = steps * kStep < kbytes;  // a last, partial step: masked loads through registers
     const int64_t g = max(0, grp);
-    xb = A.x + row0 * A.ldx;
-    wb = A.w + g * A.wg + n0 * A.ldw;
+    xb = A.x + row0 * A.ldx + k0;
+    wb = A.w + g * A.wg + n0 * A.ldw + k0;
     // LDS slot p of an operand holds row p / 8, chunk (p % 8) ^ (row % 8): a lane's q-th copy is of row
     // tid / 8 + q BT / 8; rows past the end repeat the last one
     const uint32_t c = ((tid & 7) ^ ((tid >> 3) & 7)) << 4;
@@ -508,6 +516,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
       const int p = q * BT + tid, r = p - TM;
       ssrc[q] = p < TM ? A.sx + (row0 + min(p, rows - 1)) * A.sx_row
                        : A.sw + g * A.sw_g + (WROW ? n0 + min(r, cols - 1) : (n0 + min(r, cols - 1)) / 128) * A.sw_row;
+      ssrc[q] += (p < TM ? A.sx_kb : A.sw_kb) * (int64_t)part * A.share;
     }
   };
   auto xoff = [&](int q) { return min(x0 + (uint32_t)(q * (BT / 8)) * (uint32_t)A.ldx, xend); };
@@ -666,7 +675,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
       }
     }
     // the tile's end: its stores, through the stage `free` where rows do not suit, behind the next one's copies
-    const int64_t y0 = row0 * A.ldy + n0;
+    const int64_t y0 = (part * A.M + row0) * A.ldy + n0;
     const float* bias = A.bias && grp >= 0 ? A.bias + n0 : nullptr;
     const int yrows = rows, ycols = cols;
     idx += gridDim.x;
@@ -688,6 +697,28 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
     };
     finish(smem + at * STAGE, smem + (at ^ 1) * STAGE);
     if (!more) break;
+  }
+}
+
+// y = sum over the parts, in order, + bias; four columns a thread
+__global__ __launch_bounds__(256) void mm_join_kernel(const float* part, int64_t parts, const float* bias, int64_t M, int64_t N,
+                                                      void* y, int64_t ldy, int dt) {
+  const int64_t n4 = (N + 3) / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * n4; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / n4, n = (i - m * n4) * 4;
+    const int left = (int)min((int64_t)4, N - n);
+    f4v a = {0, 0, 0, 0};
+    for (int64_t p = 0; p < parts; ++p) {
+      const float* q = part + (p * M + m) * N + n;
+      f4v v = {0, 0, 0, 0};
+      if (left == 4) __builtin_memcpy(&v, q, 16);
+      else
+        for (int e = 0; e < left; ++e) v[e] = q[e];
+      a += v;
+    }
+    if (bias)
+      for (int e = 0; e < left; ++e) a[e] += bias[n + e];
+    by_type(dt, [&](auto t) { put4<decltype(t)::value>(y, m * ldy + n, left, a); });
   }
 }
 
@@ -1177,14 +1208,14 @@ int launch_tile(const char* what, const MmArgs& A, int dt, const Device& dev, hi
   auto* f = mm_tile_kernel<IN, WROW, DMA, T, T, WN, WM>;
   TRK_REQUIRE(allow_lds(f, lds, dev, allowed), "%s: %d bytes of shared memory are not available", what, lds);
   const int64_t nt = (A.N + T - 1) / T, mt = row_tiles(A, T);
-  TRK_REQUIRE(nt * mt < ((int64_t)1 << 31), "%s: too many tiles", what);
-  const int64_t grid = std::min<int64_t>(nt * mt, (int64_t)dev.cus * (BT == 256 ? 2 : 1) / 8 * 8);
+  TRK_REQUIRE(nt * mt * A.parts < ((int64_t)1 << 31), "%s: too many tiles", what);
+  const int64_t grid = std::min<int64_t>(nt * mt * A.parts, (int64_t)dev.cus * (BT == 256 ? 2 : 1) / 8 * 8);
   f<<<(unsigned)grid, BT, lds, st>>>(A, dt, (int)nt, (int)mt);
   return trk::check_launch(what);
 }
 
 template <int IN, bool WROW>
-int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStream_t st) {
+int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, float* part, hipStream_t st) {
   const Device dev = current_device();
   // CHOICE
   // Few strips of 16 JT rows x 16 columns: straight from memory to registers, 16 rows a strip while there
@@ -1194,6 +1225,18 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
   // 16 x 50000 x 1024 18.0 / 12.7, 512 x 8192 x 1024 40.7 / 10.5.
   const int64_t strips = (A.N + 15) / 16, s16 = strips * live_tiles(A, 16), s32 = strips * live_tiles(A, 32),
                 s64 = strips * live_tiles(A, 64);
+  if (A.parts > 1) {
+    MmArgs P = A;
+    P.y = part;
+    P.ldy = A.N;
+    P.bias = nullptr;
+    if (int rc = aligned ? launch_tile<IN, WROW, true, 128, 2, 2>(what, P, TRK_F32, dev, st)
+                         : launch_tile<IN, WROW, false, 128, 2, 2>(what, P, TRK_F32, dev, st))
+      return rc;
+    const unsigned blocks = (unsigned)std::min<int64_t>((A.M * ((A.N + 3) / 4) + 255) / 256, 8 * dev.cus);
+    mm_join_kernel<<<blocks, 256, 0, st>>>(part, A.parts, A.bias, A.M, A.N, A.y, A.ldy, dt);
+    return trk::check_launch(what);
+  }
   if (row_tiles(A, 16) <= 65535) {
     if (s16 <= 256 || (s16 <= 1024 && 5 * s16 <= 7 * s32 && 5 * s16 <= 11 * s64)) return launch_few<IN, WROW, 1>(what, A, dt, st);
     if (s32 <= 1024 && 7 * s32 <= 11 * s64) return launch_few<IN, WROW, 2>(what, A, dt, st);
@@ -1213,31 +1256,47 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, hipStr
                  : launch_tile<IN, WROW, false, 128, 2, 2>(what, A, dt, dev, st);
 }
 
-int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, int64_t, void* stream) {
+int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, float* part, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   const bool al = aligned16_ptr(A.x) && aligned16_ptr(A.w) && A.ldx % 16 == 0 && A.ldw % 16 == 0 && A.wg % 16 == 0;
   if (in == IN_E4M3 && dt == TRK_F32)
-    return wrow ? launch_tiles<IN_E4M3X, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3X, false>(what, A, dt, al, st);
-  if (in == IN_E4M3) return wrow ? launch_tiles<IN_E4M3, true>(what, A, dt, al, st) : launch_tiles<IN_E4M3, false>(what, A, dt, al, st);
-  if (in == IN_BF16) return launch_tiles<IN_BF16, false>(what, A, dt, al, st);
-  return launch_tiles<IN_F16, false>(what, A, dt, al, st);
+    return wrow ? launch_tiles<IN_E4M3X, true>(what, A, dt, al, part, st) : launch_tiles<IN_E4M3X, false>(what, A, dt, al, part, st);
+  if (in == IN_E4M3)
+    return wrow ? launch_tiles<IN_E4M3, true>(what, A, dt, al, part, st) : launch_tiles<IN_E4M3, false>(what, A, dt, al, part, st);
+  if (in == IN_BF16) return launch_tiles<IN_BF16, false>(what, A, dt, al, part, st);
+  return launch_tiles<IN_F16, false>(what, A, dt, al, part, st);
 }
 
 }  // namespace
 
 extern "C" {
 
+// Few tiles and more than 24 steps: K in up to 6 parts, as many as leave a tile for each of 256 CUs.  In 16 / 32
+// bits, us, 1 / 4 / 8 parts: 256 x 4096 x 4096 29 / 20 / 21 and 42 / 23 / 24, 600 x 928 x 6288 56 / 25 / 24 and
+// 71 / 28 / 28; but 1000 x 1000 x 2048 15 / 21 / 21 and 24 / 22 / 23: the join costs about 8 us.
+int64_t trk_matmul_fp8_parts(int64_t M, int64_t N, int64_t K) {
+  const int64_t steps = (K + kStep - 1) / kStep, tiles = (M + 127) / 128 * ((N + 127) / 128), strips = (N + 15) / 16;
+  if (M <= 64 || N < 1 || steps <= 24 || strips * ((M + 63) / 64) <= 512) return 1;
+  return std::max<int64_t>(1, std::min<int64_t>(256 / tiles, 6));
+}
+
 int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
                    int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_kb, int w_block_rows, const float* bias,
-                   int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, void* stream) {
+                   int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, float* part, int64_t parts,
+                   void* stream) {
   const char* what = "trk_matmul_fp8";
   if (int rc = check_out(what, out_dtype)) return rc;
   TRK_REQUIRE(w_block_rows == 1 || w_block_rows == 128, "%s: w_block_rows must be 1 or 128", what);
+  const int64_t steps = (K + kStep - 1) / kStep;
+  TRK_REQUIRE(parts == 1 || (parts > 1 && part && parts <= steps && parts <= 4096),
+              "%s: parts must be 1, or at most the blocks of K with the workspace part", what);
+  const int64_t share = parts > 1 ? (steps + parts - 1) / parts : 0;
+  if (parts > 1) parts = (steps + share - 1) / share;  // none of them empty
   const MmArgs A{(const uint8_t*)x, (const uint8_t*)w, sx, sw, bias, y, nullptr, ldx, ldw, 0, sx_row, sx_kb,
-                 sw_row, sw_kb, 0, ldy, M, N, K, 1, 0};
+                 sw_row, sw_kb, 0, ldy, M, N, K, 1, 0, (int)parts, (int)share};
   if (int rc = check_mm(what, A, 1, true)) return rc;
   if (M == 0 || N == 0) return TRK_OK;
-  return launch_mm(what, A, IN_E4M3, w_block_rows == 1, out_dtype, (M + 127) / 128, stream);
+  return launch_mm(what, A, IN_E4M3, w_block_rows == 1, out_dtype, part, stream);
 }
 
 int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
@@ -1253,11 +1312,11 @@ int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_r
   TRK_REQUIRE(G >= 1 && G <= 65535 && counts, "%s: 1 to 65535 groups and their counts are required", what);
   const int64_t item = f8 ? 1 : 2;
   const MmArgs A{(const uint8_t*)x, (const uint8_t*)w, sx, sw, nullptr, y, counts, ldx * item, ldw * item, wg * item,
-                 sx_row, sx_kb, sw_row, sw_kb, sw_g, ldy, M, N, K, G, zero_tail};
+                 sx_row, sx_kb, sw_row, sw_kb, sw_g, ldy, M, N, K, G, zero_tail, 1, 0};
   if (int rc = check_mm(what, A, item, f8)) return rc;
   if (M == 0 || N == 0) return TRK_OK;
   return launch_mm(what, A, f8 ? IN_E4M3 : in_dtype == TRK_BF16 ? IN_BF16 : IN_F16, f8 && w_block_rows == 1, out_dtype,
-                   M / 128 + G + 1, stream);
+                   nullptr, stream);
 }
 
 // Few tiles and many rows: a group's rows are split into parts, so that the tiles fill the CUs, of at least 4 steps

@@ -34,8 +34,9 @@ _lib.register({
     "trk_rms_norm_bwd_parts": ([_I64, _I64], _I64),
     "trk_rms_norm_bwd": ([_P, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _P, _I64, _P, _P], _I),
     "trk_quantize_fp8": ([_P, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _I64, _I64, _P, _I64, _I64, _P], _I),
-    "trk_matmul_fp8": ([_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _I64, _P, _I64, _I, _P],
-                       _I),
+    "trk_matmul_fp8": ([_P, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I, _P, _I64, _I64, _I64, _P, _I64, _I,
+                        _P, _I64, _P], _I),
+    "trk_matmul_fp8_parts": ([_I64, _I64, _I64], _I64),
     "trk_matmul_grouped": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I64,
                             _I64, _I, _P, _I64, _I, _I, _P], _I),
     "trk_matmul_grouped_bwd": ([_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _I64,
@@ -340,9 +341,14 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
     x, ldx = _rows(x)
     w, ldw = _rows(w)
+    part, parts = None, 1
+    if M > 64 and K > 24 * 128:  # (one part always, else)
+        parts = lib().trk_matmul_fp8_parts(M, N, K)
+        if parts > 1:
+            part = x.new_empty((parts, M, N), dtype=torch.float32)
     _launch(what, "trk_matmul_fp8", x, x.data_ptr(), ldx, x_scale.data_ptr(), *x_scale.stride(), w.data_ptr(), ldw,
             w_scale.data_ptr(), *w_scale.stride(), wb, _at(bias), M, N, K, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1),
-            _FLOAT[y.dtype])
+            _FLOAT[y.dtype], _at(part), parts)
     return y
 
 

@@ -339,7 +339,9 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
 /* trk_matmul_fp8: y [M][N] = x [M][K] . w [N][K]^T + bias (f32 [N], NULL: 0) of e4m3 codes:
  *   sum over the blocks kb of 128 columns of sx[m * sx_row + kb * sx_kb] *
  *   sw[(n / w_block_rows) * sw_row + kb * sw_kb] * (the block's products); w_block_rows 1 or
- *   128; out_dtype TRK_F32 / BF16 / F16.
+ *   128; out_dtype TRK_F32 / BF16 / F16.  parts >= 1 (at most ceil(K / 128)): K is summed in so
+ *   many parts, joined in order, in the f32 workspace part [parts][M][N] (not read with 1);
+ *   trk_matmul_fp8_parts suggests a number.
  * trk_matmul_grouped: the rows of x sorted by group, counts[g] (device, int32) of them for
  *   w [g] (wg: stride of the groups): y = x . w[g]^T.  in_dtype TRK_E4M3 (with scales; sw_g:
  *   stride of the groups) or TRK_BF16 / F16 (scales not read).  Counts below 0 are 0 and
@@ -352,7 +354,9 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
  *   [parts][G][N][K] (not read with 1); trk_matmul_grouped_bwd_parts suggests a number. */
 int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
                    int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_kb, int w_block_rows, const float* bias,
-                   int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, void* stream);
+                   int64_t M, int64_t N, int64_t K, void* y, int64_t ldy, int out_dtype, float* part, int64_t parts,
+                   void* stream);
+int64_t trk_matmul_fp8_parts(int64_t M, int64_t N, int64_t K);
 int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
                        int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
                        int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype,

@@ -109,11 +109,13 @@ def test_host_argument_errors(trk):
     refused(L.trk_rms_norm_bwd(v, 8, z, v, v, 8, z, 0, 4, 8, 0, v, 8, v, 77, v, z), b"parts")
     refused(L.trk_quantize_fp8(v, 8, 0, 1, 4, 8, 64, 0, v, 8, 0, v, 4, 0, z), b"block_rows")
     refused(L.trk_quantize_fp8(v, 8, 0, 1, 4, 8, 1, 0, v, 8, 0, v, 3, 0, z), b"scale_ld")
-    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 7, z, 4, 4, 8, v, 4, 0, z), b"w_block_rows")
-    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 2, z), b"output")
-    refused(L.trk_matmul_fp8(v, 7, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, z), b"row stride")
-    refused(L.trk_matmul_fp8(v, 8, z, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, z), b"null")
-    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, -8, v, 4, 0, z), b"bad shape")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 7, z, 4, 4, 8, v, 4, 0, z, 1, z), b"w_block_rows")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 2, z, 1, z), b"output")
+    refused(L.trk_matmul_fp8(v, 7, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, z, 1, z), b"row stride")
+    refused(L.trk_matmul_fp8(v, 8, z, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, z, 1, z), b"null")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, -8, v, 4, 0, z, 1, z), b"bad shape")
+    refused(L.trk_matmul_fp8(v, 8, v, 1, 1, v, 8, v, 1, 1, 1, z, 4, 4, 8, v, 4, 0, v, 2, z), b"parts")
+    refused(L.trk_matmul_fp8(v, 512, v, 1, 1, v, 512, v, 1, 1, 1, z, 4, 4, 512, v, 4, 0, z, 2, z), b"parts")
     refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, v, 0, 4, 4, 8, 1, v, 4, 1, 0, z), b"groups")
     refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, v, 2, 4, 4, 8, 0, v, 4, 1, 0, z), b"input")
     refused(L.trk_matmul_grouped(v, 8, z, 0, 0, v, 8, 32, z, 0, 0, 0, 128, z, 2, 4, 4, 8, 1, v, 4, 1, 0, z), b"groups")
@@ -126,7 +128,7 @@ def test_host_argument_errors(trk):
     # nothing to do
     assert L.trk_rms_norm(z, 8, z, 0, z, 1e-6, 0, 8, 0, z, 8, z, 0, z, z) == 0
     assert L.trk_quantize_fp8(z, 8, 0, 0, 4, 8, 1, 0, z, 8, 0, z, 4, 0, z) == 0
-    assert L.trk_matmul_fp8(z, 8, z, 0, 0, z, 8, z, 0, 0, 1, z, 0, 4, 8, z, 4, 0, z) == 0
+    assert L.trk_matmul_fp8(z, 8, z, 0, 0, z, 8, z, 0, 0, 1, z, 0, 4, 8, z, 4, 0, z, 1, z) == 0
 
 
 def test_host_tensors_are_refused(trk):
@@ -402,8 +404,8 @@ def test_matmul_fp8(trk, gpu, M, N, K, block):
             assert float((y.double() - want).norm() / want.norm()) <= 0.75 * HALF[y.dtype] + (0 if y.dtype != F32 else 2.0 ** -20)
 
 
-# sizes that run as 128-tiles and (the last three) as 256-tiles: whole tiles, ragged edges, part steps, odd rows
-TILES = [(700, 1100, 16), (640, 1280, 128), (769, 1025, 300), (1000, 900, 272), (900, 1000, 131), (4096, 4096, 256),
+# sizes that run as 128-tiles (the first three with K in parts) and (the last three) as 256-tiles: whole tiles, ragged edges, part steps, odd rows
+TILES = [(600, 928, 6288), (130, 4096, 4000), (300, 2051, 3299), (700, 1100, 16), (640, 1280, 128), (769, 1025, 300), (1000, 900, 272), (900, 1000, 131), (4096, 4096, 256),
          (4100, 4200, 96), (4099, 4097, 277)]
 
 
