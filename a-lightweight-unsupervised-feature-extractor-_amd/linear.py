@@ -382,17 +382,30 @@ def _lay(t: torch.Tensor) -> torch.Tensor:
     return t.new_empty((*t.shape[:-1], ld))[..., :t.shape[-1]].copy_(t)
 
 
-def _pays_to_lay(M: int, N: int, K: int, G: int) -> bool:
-    """Whether rows off the multiples of 16 bytes are copied first.  The product reads them through registers, at
-    a third of the rate (8 groups of 16384 x 1501 x 1203 in all: 239 us against 81 us aligned); the copies cost their
-    bytes and two launches."""
-    return M * N * K > 4_000_000_000 and M * N > 400 * (M + G * N)
+def _lay_pays(M: int, N: int, K: int, G: int) -> bool:
+    """Whether x and w with rows off the multiples of 16 bytes are copied first (_lay).  The tiles take such rows
+    through registers, about 1.5 us a step of 64 columns slower (8 groups of 16384 x 1501 x 1203 in all: 239 us,
+    117 with the copies, 81 for aligned rows); the copies cost two launches and their bytes.  Few strips of rows
+    are read at any alignment at no loss."""
+    if -(-N // 16) * max(-(-M // 64), min(G, M)) <= 512:
+        return False
+    rounds = -(-(M // 128 + min(G, M)) * -(-N // 128) // 512)
+    return 1.5 * (K // 64) * rounds > 10 + (M + G * N) * K / 750_000
+
+
+def _lay_pays_backward(M: int, N: int, K: int, G: int) -> bool:
+    """The same for the gradients, of x, w and dy: about 3.5 us a step of 64 columns of dy, or of 64 rows of a
+    group where its rows are not split into parts."""
+    tiles = -(-N // 256) * -(-K // 256) * G
+    steps = N // 64 + M // (64 * G * max(1, min(256 // tiles, M // (256 * G))))
+    rounds = max(1, (tiles + (M // 256 + min(G, M)) * -(-K // 256)) // 512)
+    return 3.5 * steps * rounds > 20 + (M * (N + K) + G * N * K) / 750_000
 
 
 class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, counts, dt, out_dtype):
-        if _pays_to_lay(x.shape[0], w.shape[1], w.shape[2], w.shape[0]):
+        if _lay_pays(x.shape[0], w.shape[1], w.shape[2], w.shape[0]):
             x, w = _lay(x), _lay(w)
         ctx.save_for_backward(x, w, counts)
         ctx.dt = dt
@@ -403,14 +416,14 @@ class _Grouped(torch.autograd.Function):
     @_backward_once
     def backward(ctx, dy):
         x, w, counts = ctx.saved_tensors
-        x, ldx = _rows(x)
-        w, ldw = _weights(w)
         M, K = x.shape
         G, N = w.shape[:2]
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
-        if _pays_to_lay(M, N, K, G):
-            dy = _lay(dy)
+        if _lay_pays_backward(M, N, K, G):
+            x, w, dy = _lay(x), _lay(w), _lay(dy)
+        x, ldx = _rows(x)
+        w, ldw = _weights(w)
         dy, ldy = _rows(dy)
         dx = x.new_empty((M, K)) if ctx.needs_input_grad[0] else None
         dw = part = None
@@ -470,6 +483,6 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
             raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {out_dtype}")
         return _Grouped.apply(x, w, counts, dt, out_dtype or x.dtype)
     y = _out(what, out, out_dtype, x, M, N, x.dtype)
-    if _pays_to_lay(M, N, K, G):
+    if _lay_pays(M, N, K, G):
         x, w = _lay(x), _lay(w)
     return _grouped_forward(what, x, None, w, None, 128, counts, dt, y, int(out is None))
