@@ -428,6 +428,33 @@ def test_matmul_fp8_tiles(trk, gpu, M, N, K, block):
 
 
 @gpu_test
+@pytest.mark.parametrize("K", [300, 2100, 2176])
+def test_matmul_fp8_parts(trk, gpu, K):
+    """any number of parts of K, also ones that would leave the last parts empty"""
+    g = gen_of(gpu, 36, K)
+    M, N = 150, 203
+    x, sx = codes_of(g, M, K, 1, gpu)
+    w, sw = codes_of(g, N, K, 128, gpu)
+    px, pw = (torch.nn.functional.pad(t.view(torch.uint8), (0, -K % 16)).view(FP8)[:, :K] for t in (x, w))
+    xv, wv = widen(x, sx, 1), widen(w, sw, 128)
+    bias = torch.randn(N, device=gpu, generator=g)
+    want = xv @ wv.t() + bias.double()
+    kb = sx.shape[1]
+    for a, b in ((x, w), (px, pw)):
+        for parts in (2, 3, 5, 16, 17):
+            if parts > kb:
+                continue
+            part = torch.empty(parts, M, N, device=gpu)
+            y = torch.full((M + 1, N), 7.0, device=gpu)
+            rc = trk.lib().trk_matmul_fp8(a.data_ptr(), a.stride(0), sx.data_ptr(), *sx.stride(), b.data_ptr(), b.stride(0),
+                                          sw.data_ptr(), *sw.stride(), 128, bias.data_ptr(), M, N, K, y.data_ptr(), N, 0,
+                                          part.data_ptr(), parts, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0
+            near(y[:M], want, F32, product_slack(xv, wv, kb + parts) + want.abs() * 2 * U)
+            assert (y[M] == 7).all()
+
+
+@gpu_test
 def test_matmul_fp8_layouts(trk, gpu):
     """rows inside wider buffers (aligned and not), scales of other strides, an output inside a wider one"""
     g = gen_of(gpu, 20)
