@@ -396,6 +396,8 @@ def _lay_pays(M: int, N: int, K: int, G: int) -> bool:
 def _lay_pays_backward(M: int, N: int, K: int, G: int) -> bool:
     """The same for the gradients, of x, w and dy: about 3.5 us a step of 64 columns of dy, or of 64 rows of a
     group where its rows are not split into parts."""
+    if not (N and K):
+        return False
     tiles = -(-N // 256) * -(-K // 256) * G
     steps = N // 64 + M // (64 * G * max(1, min(256 // tiles, M // (256 * G))))
     rounds = max(1, (tiles + (M // 256 + min(G, M)) * -(-K // 256)) // 512)

@@ -659,6 +659,18 @@ def test_matmul_grouped_empty_groups(trk, gpu, dtype):
 
 
 @gpu_test
+@pytest.mark.parametrize("rows,N,K", [(0, 40, 24), (7, 0, 24), (7, 40, 0), (0, 0, 0)])
+def test_gradients_of_empty_sides(trk, gpu, rows, N, K):
+    x = torch.randn(rows, K, device=gpu).to(BF).requires_grad_()
+    w = torch.randn(3, N, K, device=gpu).to(BF).requires_grad_()
+    c = torch.tensor([2, 0, 5], device=gpu, dtype=torch.int32)
+    y = trk.matmul_grouped(x, w, c)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert y.shape == (rows, N) and dx.shape == x.shape and dw.shape == w.shape
+    assert (y == 0).all() and (dx == 0).all() and (dw == 0).all()
+
+
+@gpu_test
 def test_products_of_turned_operands(trk, gpu):
     """operands whose columns are not next to each other in memory are laid out first"""
     g = gen_of(gpu, 34)
