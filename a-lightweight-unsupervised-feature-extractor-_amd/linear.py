@@ -331,7 +331,7 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     kb = (K + 127) // 128
     _scales(what, x_scale, "x_scale", x, dev, (M, kb), None)
     wb = _scales(what, w_scale, "w_scale", x, dev, (N, kb), ((N + 127) // 128, kb))
-    _no_grad(what, x_scale, w_scale, bias)
+    _no_grad(what, x, x_scale, w, w_scale, bias)
     if bias is not None:
         if bias.get_device() != dev:
             _elsewhere(x, bias, what, "bias")
@@ -472,7 +472,7 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
         kb = (K + 127) // 128
         _scales(what, x_scale, "x_scale", x, dev, (M, kb), None)
         wb = _scales(what, w_scale, "w_scale", x, dev, (G, N, kb), (G, (N + 127) // 128, kb))
-        _no_grad(what, x_scale, w_scale)
+        _no_grad(what, x, x_scale, w, w_scale)
         y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
         return _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, _lib.TRK_E4M3, y, int(out is None))
     dt = _type(x, _HALF, what, "x")

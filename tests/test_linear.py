@@ -173,6 +173,21 @@ def test_refusals(trk, gpu):
             call()
 
 
+@gpu_test
+def test_codes_with_a_gradient_are_refused(trk, gpu):
+    """codes cast from a tensor that requires a gradient carry it on; none comes back from the 8-bit products"""
+    a = torch.zeros(4, 32, device=gpu, requires_grad=True)
+    p, q, s = a.to(FP8), torch.zeros(4, 32, device=gpu).to(FP8), torch.ones(4, 1, device=gpu)
+    c = torch.tensor([4], device=gpu, dtype=torch.int32)
+    for x, w in ((p, q), (q, p)):
+        with pytest.raises(NotImplementedError):
+            trk.matmul_fp8(x, s, w, s)
+        with pytest.raises(NotImplementedError):
+            trk.matmul_grouped(x, w[None], c, x_scale=s, w_scale=s[None])
+        with torch.no_grad():
+            assert (trk.matmul_fp8(x, s, w, s) == 0).all()
+
+
 # ----------------------------------------------------------------------------------------------- norm
 NORM = [(1, 1), (3, 7), (3, 9), (4, 15), (5, 16), (17, 127), (16, 128), (33, 129), (7, 500), (9, 512), (3, 513), (5, 1000), (2, 1024),
         (3, 2047), (2, 2048), (1, 4096), (2, 5001), (2, 8192), (3, 8193), (1, 20001)]
