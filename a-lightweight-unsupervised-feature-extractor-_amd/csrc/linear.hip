@@ -700,15 +700,28 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(MmArgs A, int 
   }
 }
 
-// y = sum over the parts, in order, + bias; four columns a thread
-__global__ __launch_bounds__(256) void mm_join_kernel(const float* part, int64_t parts, const float* bias, int64_t M, int64_t N,
-                                                      void* y, int64_t ldy, int dt) {
-  const int64_t n4 = (N + 3) / 4;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < M * n4; i += (int64_t)gridDim.x * 256) {
+// y = sum over the parts, in order, + bias; four columns a thread.  Grouped: the rows behind the last group, which
+// have no parts, are zeros (zero_tail) or stay as they are.
+__global__ __launch_bounds__(256) void mm_join_kernel(MmArgs A, const float* part, int dt) {
+  __shared__ int64_t sums[4];
+  const float* bias = A.bias;
+  const int64_t M = A.M, N = A.N, n4 = (N + 3) / 4;
+  int64_t end = M;
+  if (A.counts) {  // fewer than 2^16 counts below 2^31
+    int64_t rows = 0;
+    for (int64_t g = threadIdx.x; g < A.G; g += 256) rows += max(0, A.counts[g]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) rows += __shfl_xor(rows, d, 64);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = rows;
+    __syncthreads();
+    end = min(M, sums[0] + sums[1] + sums[2] + sums[3]);
+  }
+  const int64_t rows = A.zero_tail ? M : end;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * n4; i += (int64_t)gridDim.x * 256) {
     const int64_t m = i / n4, n = (i - m * n4) * 4;
     const int left = (int)min((int64_t)4, N - n);
     f4v a = {0, 0, 0, 0};
-    for (int64_t p = 0; p < parts; ++p) {
+    for (int64_t p = 0; p < (m < end ? A.parts : 0); ++p) {
       const float* q = part + (p * M + m) * N + n;
       f4v v = {0, 0, 0, 0};
       if (left == 4) __builtin_memcpy(&v, q, 16);
@@ -718,7 +731,7 @@ __global__ __launch_bounds__(256) void mm_join_kernel(const float* part, int64_t
     }
     if (bias)
       for (int e = 0; e < left; ++e) a[e] += bias[n + e];
-    by_type(dt, [&](auto t) { put4<decltype(t)::value>(y, m * ldy + n, left, a); });
+    by_type(dt, [&](auto t) { put4<decltype(t)::value>(A.y, m * A.ldy + n, left, a); });
   }
 }
 
@@ -1123,6 +1136,16 @@ int check_mm(const char* what, const MmArgs& A, int64_t item, bool scaled) {
   return TRK_OK;
 }
 
+// the steps of a part of rows of `kbytes`, and as many parts as have any
+int check_parts(const char* what, int64_t kbytes, const float* part, int64_t& parts, int& share) {
+  const int64_t steps = (kbytes + kStep - 1) / kStep;
+  TRK_REQUIRE(parts == 1 || (parts > 1 && part && parts <= steps && parts <= 4096),
+              "%s: parts must be 1, or at most the blocks of K with the workspace part", what);
+  share = parts > 1 ? (int)((steps + parts - 1) / parts) : 0;
+  if (parts > 1) parts = (steps + share - 1) / share;
+  return TRK_OK;
+}
+
 // whole 16-byte pieces of every row at multiples of 16 bytes (offsets inside a tile are 32 bits)
 bool rows_aligned(const void* p, int64_t ld) { return aligned16_ptr(p) && ld % 8 == 0; }
 bool grad_aligned(const GradArgs& A) {
@@ -1180,14 +1203,38 @@ int launch_grad(const char* what, const GradArgs& A, int dt, hipStream_t st) {
 }
 
 // row tiles that have rows, as far as the host knows: groups have at least a tile each
-int64_t live_tiles(const MmArgs& A, int tm) {
-  const int64_t full = (A.M + tm - 1) / tm;
-  return A.counts ? std::max(full, std::min(A.G, A.M)) : full;
+int64_t live_tiles(int64_t G, int64_t M, int tm) { return std::max((M + tm - 1) / tm, std::min(G, M)); }
+
+// Few strips of 16 JT rows x 16 columns: straight from memory to registers, 16 rows a strip while there
+// are at most 256, else the fewest strips by the work of one (1, 1.4 and 2.2 for 16, 32 and 64 rows).
+// In 8 bits, us, strips / 128-tiles: 16 x 4096 x 4096 7.0 / 20.9, 64 x 4096 x 4096 13.9 / 21.0, 256 x
+// 1024 x 1024 6.2 / 8.6, 32 x 16384 x 4096 26.5 / 28.5; past the limits 128 x 4096 x 4096 22.8 / 21.2,
+// 16 x 50000 x 1024 18.0 / 12.7, 512 x 8192 x 1024 40.7 / 10.5.  JT, or 0: tiles.
+int few_strips(int64_t G, int64_t M, int64_t N) {
+  const int64_t strips = (N + 15) / 16, s16 = strips * live_tiles(G, M, 16), s32 = strips * live_tiles(G, M, 32),
+                s64 = strips * live_tiles(G, M, 64);
+  if (s16 <= 256 || (s16 <= 1024 && 5 * s16 <= 7 * s32 && 5 * s16 <= 11 * s64)) return 1;
+  if (s32 <= 1024 && 7 * s32 <= 11 * s64) return 2;
+  return s64 <= 512 ? 4 : 0;
+}
+
+// Few 128-tiles (of even groups) and long rows: K in parts, as many as give 384 tiles of at least 8 steps, up to 8.
+// In 16 / 8 bits, us, 1 part / the rule's: 8 groups, 512 x 2048 x 8192 115 / 66 and 55 / 36; 1000 x 1024 x 8192 in 4
+// 83 / 38 and 54 / 29; 600 x 1024 x 16384 in 2 162 / 50 and 100 / 36; 600 x 928 x 6288 90 / 32 and 57 / 25; 1000 x
+// 1000 x 2048 28 / 22 in 16 bits, in 8 (16 steps) 18 against 22 in 4 parts.  Rows that strips of 16 take stay whole
+// (8 groups, 64 x 2048 x 8192 52 against 56 in 3 parts), and up to 64 steps 256 strips of 64 (64 x 4096 x 4096 24 /
+// 19 in 16 bits, 17 / 18 in 8).  The join costs about 8 us.
+int64_t parts_of(int64_t G, int64_t M, int64_t N, int64_t steps) {
+  if (G < 1 || M < 1 || N < 1 || steps <= 24) return 1;
+  const int64_t groups = std::min(G, M), tiles = groups * (((M + groups - 1) / groups + 127) / 128) * ((N + 127) / 128);
+  if (tiles > 192 || few_strips(G, M, N) == 1) return 1;
+  if (steps <= 64 && (N + 15) / 16 * live_tiles(G, M, 64) <= 256) return 1;
+  return std::min({384 / tiles, steps / 8, (int64_t)8});
 }
 
 template <int IN, bool WROW, int JT>
 int launch_few(const char* what, const MmArgs& A, int dt, hipStream_t st) {
-  const int64_t strips = (A.N + 15) / 16, live = live_tiles(A, 16 * JT), steps = (A.K * (is8(IN) ? 1 : 2) + kStep - 1) / kStep;
+  const int64_t strips = (A.N + 15) / 16, live = live_tiles(A.G, A.M, 16 * JT), steps = (A.K * (is8(IN) ? 1 : 2) + kStep - 1) / kStep;
   // waves that share 16 columns: enough for 2048 waves in all, no more than there are steps (16 x 4096 x
   // 4096 in 8 bits: 7.0 us with 8, 10.5 with 4; 64 groups of 1 row x 1024 x 1024: 15.2 with 1, 23.5 with 4)
   int kw = 8;
@@ -1217,30 +1264,23 @@ int launch_tile(const char* what, const MmArgs& A, int dt, const Device& dev, hi
 template <int IN, bool WROW>
 int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, float* part, hipStream_t st) {
   const Device dev = current_device();
-  // CHOICE
-  // Few strips of 16 JT rows x 16 columns: straight from memory to registers, 16 rows a strip while there
-  // are at most 256, else the fewest strips by the work of one (1, 1.4 and 2.2 for 16, 32 and 64 rows).
-  // In 8 bits, us, strips / 128-tiles: 16 x 4096 x 4096 7.0 / 20.9, 64 x 4096 x 4096 13.9 / 21.0, 256 x
-  // 1024 x 1024 6.2 / 8.6, 32 x 16384 x 4096 26.5 / 28.5; past the limits 128 x 4096 x 4096 22.8 / 21.2,
-  // 16 x 50000 x 1024 18.0 / 12.7, 512 x 8192 x 1024 40.7 / 10.5.
-  const int64_t strips = (A.N + 15) / 16, s16 = strips * live_tiles(A, 16), s32 = strips * live_tiles(A, 32),
-                s64 = strips * live_tiles(A, 64);
   if (A.parts > 1) {
     MmArgs P = A;
     P.y = part;
     P.ldy = A.N;
     P.bias = nullptr;
+    P.zero_tail = 0;
     if (int rc = aligned ? launch_tile<IN, WROW, true, 128, 2, 2>(what, P, TRK_F32, dev, st)
                          : launch_tile<IN, WROW, false, 128, 2, 2>(what, P, TRK_F32, dev, st))
       return rc;
     const unsigned blocks = (unsigned)std::min<int64_t>((A.M * ((A.N + 3) / 4) + 255) / 256, 8 * dev.cus);
-    mm_join_kernel<<<blocks, 256, 0, st>>>(part, A.parts, A.bias, A.M, A.N, A.y, A.ldy, dt);
+    mm_join_kernel<<<blocks, 256, 0, st>>>(A, part, dt);
     return trk::check_launch(what);
   }
-  if (row_tiles(A, 16) <= 65535) {
-    if (s16 <= 256 || (s16 <= 1024 && 5 * s16 <= 7 * s32 && 5 * s16 <= 11 * s64)) return launch_few<IN, WROW, 1>(what, A, dt, st);
-    if (s32 <= 1024 && 7 * s32 <= 11 * s64) return launch_few<IN, WROW, 2>(what, A, dt, st);
-    if (s64 <= 512) return launch_few<IN, WROW, 4>(what, A, dt, st);
+  switch (few_strips(A.G, A.M, A.N)) {  // (the grid's second length is below 4096)
+    case 1: return launch_few<IN, WROW, 1>(what, A, dt, st);
+    case 2: return launch_few<IN, WROW, 2>(what, A, dt, st);
+    case 4: return launch_few<IN, WROW, 4>(what, A, dt, st);
   }
   // 256-tiles where whole ones alone fill the CUs (2048 x 8192 x 1024 in 8 bits 23.2 us against 25.8 with 128-tiles;
   // 1024 x 8192 x 1024 20.2 against 15.2; 64 groups of 8 rows x 2048 x 2048 70 against 48).  f32 outputs
@@ -1271,14 +1311,7 @@ int launch_mm(const char* what, const MmArgs& A, int in, int wrow, int dt, float
 
 extern "C" {
 
-// Few tiles and more than 24 steps: K in up to 6 parts, as many as leave a tile for each of 256 CUs.  In 16 / 32
-// bits, us, 1 / 4 / 8 parts: 256 x 4096 x 4096 29 / 20 / 21 and 42 / 23 / 24, 600 x 928 x 6288 56 / 25 / 24 and
-// 71 / 28 / 28; but 1000 x 1000 x 2048 15 / 21 / 21 and 24 / 22 / 23: the join costs about 8 us.
-int64_t trk_matmul_fp8_parts(int64_t M, int64_t N, int64_t K) {
-  const int64_t steps = (K + kStep - 1) / kStep, tiles = (M + 127) / 128 * ((N + 127) / 128), strips = (N + 15) / 16;
-  if (M <= 64 || N < 1 || steps <= 24 || strips * ((M + 63) / 64) <= 512) return 1;
-  return std::max<int64_t>(1, std::min<int64_t>(256 / tiles, 6));
-}
+int64_t trk_matmul_fp8_parts(int64_t M, int64_t N, int64_t K) { return parts_of(1, M, N, (K + kStep - 1) / kStep); }
 
 int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
                    int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_kb, int w_block_rows, const float* bias,
@@ -1287,22 +1320,24 @@ int trk_matmul_fp8(const void* x, int64_t ldx, const float* sx, int64_t sx_row, 
   const char* what = "trk_matmul_fp8";
   if (int rc = check_out(what, out_dtype)) return rc;
   TRK_REQUIRE(w_block_rows == 1 || w_block_rows == 128, "%s: w_block_rows must be 1 or 128", what);
-  const int64_t steps = (K + kStep - 1) / kStep;
-  TRK_REQUIRE(parts == 1 || (parts > 1 && part && parts <= steps && parts <= 4096),
-              "%s: parts must be 1, or at most the blocks of K with the workspace part", what);
-  const int64_t share = parts > 1 ? (steps + parts - 1) / parts : 0;
-  if (parts > 1) parts = (steps + share - 1) / share;  // none of them empty
+  int share;
+  if (int rc = check_parts(what, K, part, parts, share)) return rc;
   const MmArgs A{(const uint8_t*)x, (const uint8_t*)w, sx, sw, bias, y, nullptr, ldx, ldw, 0, sx_row, sx_kb,
-                 sw_row, sw_kb, 0, ldy, M, N, K, 1, 0, (int)parts, (int)share};
+                 sw_row, sw_kb, 0, ldy, M, N, K, 1, 0, (int)parts, share};
   if (int rc = check_mm(what, A, 1, true)) return rc;
   if (M == 0 || N == 0) return TRK_OK;
   return launch_mm(what, A, IN_E4M3, w_block_rows == 1, out_dtype, part, stream);
 }
 
-int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
-                       int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
-                       int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype,
-                       void* y, int64_t ldy, int out_dtype, int zero_tail, void* stream) {
+int64_t trk_matmul_grouped_parts(int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype) {
+  return parts_of(G, M, N, (K * (in_dtype == TRK_E4M3 ? 1 : 2) + kStep - 1) / kStep);
+}
+
+int trk_matmul_grouped_split(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                             int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
+                             int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K,
+                             int in_dtype, void* y, int64_t ldy, int out_dtype, int zero_tail, float* part, int64_t parts,
+                             void* stream) {
   const char* what = "trk_matmul_grouped";
   if (int rc = check_out(what, out_dtype)) return rc;
   TRK_REQUIRE(in_dtype == TRK_E4M3 || in_dtype == TRK_BF16 || in_dtype == TRK_F16,
@@ -1311,12 +1346,22 @@ int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_r
   TRK_REQUIRE(!f8 || w_block_rows == 1 || w_block_rows == 128, "%s: w_block_rows must be 1 or 128", what);
   TRK_REQUIRE(G >= 1 && G <= 65535 && counts, "%s: 1 to 65535 groups and their counts are required", what);
   const int64_t item = f8 ? 1 : 2;
+  int share;
+  if (int rc = check_parts(what, K * item, part, parts, share)) return rc;
   const MmArgs A{(const uint8_t*)x, (const uint8_t*)w, sx, sw, nullptr, y, counts, ldx * item, ldw * item, wg * item,
-                 sx_row, sx_kb, sw_row, sw_kb, sw_g, ldy, M, N, K, G, zero_tail, 1, 0};
+                 sx_row, sx_kb, sw_row, sw_kb, sw_g, ldy, M, N, K, G, zero_tail, (int)parts, share};
   if (int rc = check_mm(what, A, item, f8)) return rc;
   if (M == 0 || N == 0) return TRK_OK;
   return launch_mm(what, A, f8 ? IN_E4M3 : in_dtype == TRK_BF16 ? IN_BF16 : IN_F16, f8 && w_block_rows == 1, out_dtype,
-                   nullptr, stream);
+                   part, stream);
+}
+
+int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                       int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
+                       int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype,
+                       void* y, int64_t ldy, int out_dtype, int zero_tail, void* stream) {
+  return trk_matmul_grouped_split(x, ldx, sx, sx_row, sx_kb, w, ldw, wg, sw, sw_row, sw_kb, sw_g, w_block_rows, counts, G, M,
+                                  N, K, in_dtype, y, ldy, out_dtype, zero_tail, nullptr, 1, stream);
 }
 
 // Few tiles and many rows: a group's rows are split into parts, so that the tiles fill the CUs, of at least 4 steps

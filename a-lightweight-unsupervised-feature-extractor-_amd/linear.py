@@ -39,6 +39,9 @@ _lib.register({
     "trk_matmul_fp8_parts": ([_I64, _I64, _I64], _I64),
     "trk_matmul_grouped": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I64,
                             _I64, _I, _P, _I64, _I, _I, _P], _I),
+    "trk_matmul_grouped_split": ([_P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I64,
+                                  _I64, _I, _P, _I64, _I, _I, _P, _I64, _P], _I),
+    "trk_matmul_grouped_parts": ([_I64, _I64, _I64, _I64, _I], _I64),
     "trk_matmul_grouped_bwd": ([_P, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _P, _I64, _P, _I64,
                                 _I64, _P, _I64, _P], _I),
     "trk_matmul_grouped_bwd_parts": ([_I64, _I64, _I64, _I64], _I64),
@@ -342,7 +345,7 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     x, ldx = _rows(x)
     w, ldw = _rows(w)
     part, parts = None, 1
-    if M > 64 and K > 24 * 128:  # (one part always, else)
+    if M > 16 and K > 24 * 128:  # (one part always, else)
         parts = lib().trk_matmul_fp8_parts(M, N, K)
         if parts > 1:
             part = x.new_empty((parts, M, N), dtype=torch.float32)
@@ -369,8 +372,18 @@ def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_ta
     else:
         sx = (x_scale.data_ptr(), *x_scale.stride())
         sw = (w_scale.data_ptr(), w_scale.stride(1), w_scale.stride(2), w_scale.stride(0))
-    _launch(what, "trk_matmul_grouped", x, x.data_ptr(), ldx, *sx, w.data_ptr(), ldw, w.stride(0), *sw, wb, counts.data_ptr(),
-            G, M, N, K, in_dt, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype], zero_tail)
+    args = (x.data_ptr(), ldx, *sx, w.data_ptr(), ldw, w.stride(0), *sw, wb, counts.data_ptr(), G, M, N, K, in_dt,
+            y.data_ptr(), y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype], zero_tail)
+    item = x.element_size()
+    if M > 16 and K * item > 24 * 128:  # (one part always, else)
+        parts = lib().trk_matmul_grouped_parts(G, M, N, K, in_dt)
+        # rows off the multiples of 16 bytes that were not copied are bound by their way through the registers (64 x
+        # 6000 x 3500: strips 32 us, 47 in 6 parts)
+        if parts > 1 and (x.data_ptr() | w.data_ptr() | ldx * item | ldw * item | w.stride(0) * item) % 16 == 0:
+            part = x.new_empty((parts, M, N), dtype=torch.float32)
+            _launch(what, "trk_matmul_grouped_split", x, *args, part.data_ptr(), parts)
+            return y
+    _launch(what, "trk_matmul_grouped", x, *args)
     return y
 
 

@@ -347,6 +347,9 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
  *   stride of the groups) or TRK_BF16 / F16 (scales not read).  Counts below 0 are 0 and
  *   their sum is cut at M.  Rows behind the last group are written as zeros (zero_tail) or
  *   left as they were.
+ * trk_matmul_grouped_split: the same with K summed in parts >= 1 (at most the steps of 128 bytes of
+ *   a row), joined in order, in the f32 workspace part [parts][M][N]; trk_matmul_grouped_parts suggests
+ *   a number.
  * trk_matmul_grouped_bwd: the 16-bit product's gradients, dx [M][lddx] = dy . w[g] (rows behind
  *   the last group: zeros; NULL: not wanted, w is not read) and dw [G][dwg] = dy_g^T . x_g
  *   (a group without rows: zeros; NULL: not wanted, x is not read).  parts >= 1: dw is
@@ -361,6 +364,12 @@ int trk_matmul_grouped(const void* x, int64_t ldx, const float* sx, int64_t sx_r
                        int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
                        int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype,
                        void* y, int64_t ldy, int out_dtype, int zero_tail, void* stream);
+int trk_matmul_grouped_split(const void* x, int64_t ldx, const float* sx, int64_t sx_row, int64_t sx_kb, const void* w,
+                             int64_t ldw, int64_t wg, const float* sw, int64_t sw_row, int64_t sw_kb, int64_t sw_g,
+                             int w_block_rows, const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K,
+                             int in_dtype, void* y, int64_t ldy, int out_dtype, int zero_tail, float* part, int64_t parts,
+                             void* stream);
+int64_t trk_matmul_grouped_parts(int64_t G, int64_t M, int64_t N, int64_t K, int in_dtype);
 int trk_matmul_grouped_bwd(const void* dy, int64_t ldy, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t wg,
                            const int32_t* counts, int64_t G, int64_t M, int64_t N, int64_t K, int dtype, void* dx,
                            int64_t lddx, void* dw, int64_t lddw, int64_t dwg, float* part, int64_t parts, void* stream);

@@ -686,6 +686,82 @@ def test_gradients_of_empty_sides(trk, gpu, rows, N, K):
 
 
 @gpu_test
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8 1", "fp8 128"])
+@pytest.mark.parametrize("counts,rows", [([5], 5), ([0, 0], 9), ([200, 0, 1, 130], 340), ([17, -3, 40], 60), ([150, 2 ** 30, 7], 290),
+                                         ([1] * 300, 310), ([2 ** 31 - 1] * 3, 130)], ids=lambda c: str(len(c)) if isinstance(c, list) else str(c))
+def test_matmul_grouped_parts(trk, gpu, counts, rows, kind):
+    """K in any number of parts: ragged groups, rows behind them left or zeroed, rows at any alignment"""
+    g = gen_of(gpu, 37, rows)
+    G, N = len(counts), 203
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    L, st = trk.lib(), torch.cuda.current_stream().cuda_stream
+    for K in (300, 1288):
+        if kind[:3] == "fp8":
+            bl = int(kind[4:])
+            x, sx = codes_of(g, rows, K, 1, gpu)
+            w, sw = codes_of(g, N, K, bl, gpu, (G,))
+            xv, wv, dt = widen(x, sx, 1), torch.stack([widen(a, b, bl) for a, b in zip(w, sw)]), 4
+            sc = (sx.data_ptr(), *sx.stride()), (sw.data_ptr(), sw.stride(1), sw.stride(2), sw.stride(0), bl)
+        else:
+            dt = 1 if kind == "bf16" else 3
+            x = torch.randn(rows, K, device=gpu, generator=g).to(BF if dt == 1 else F16)
+            w = torch.randn(G, N, K, device=gpu, generator=g).to(x.dtype)
+            xv, wv, sc = x.double(), w.double(), ((None, 0, 0), (None, 0, 0, 0, 128))
+        want, slack, end = grouped64(xv, wv, counts)
+        steps = -(-K * x.element_size() // 128)
+        for parts in (1, 2, 3, 7, steps):
+            if parts > steps:
+                continue
+            part = torch.full((parts, rows, N), float("nan"), device=gpu)
+            for tail in (0, 1):
+                y = torch.full((rows + 1, N + 1), 7.0, device=gpu)
+                assert L.trk_matmul_grouped_split(x.data_ptr(), x.stride(0), *sc[0], w.data_ptr(), w.stride(1), w.stride(0), *sc[1],
+                                                  c.data_ptr(), G, rows, N, K, dt, y.data_ptr(), N + 1, 0, tail,
+                                                  part.data_ptr(), parts, st) == 0
+                near(y[:end, :N], want[:end], F32, slack[:end] * (K + 8 + parts) * U)
+                assert (y[end:rows, :N] == (0 if tail else 7)).all() and (y[rows] == 7).all() and (y[:, N] == 7).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, FP8])
+def test_matmul_grouped_long_rows(trk, gpu, dtype):
+    """few tiles and long rows through the public call, with gradients, also captured and at odd rows"""
+    g = gen_of(gpu, 38)
+    counts, rows, N = [140, 0, 300, 61], 520, 700
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    for K in (8192, 5003):
+        assert trk.lib().trk_matmul_grouped_parts(4, rows, N, K, 4 if dtype == FP8 else 1) > 1
+        x, sx = codes_of(g, rows, K, 1, gpu)
+        w, sw = codes_of(g, N, K, 128, gpu, (4,))
+        if dtype == FP8:
+            more = dict(x_scale=sx, w_scale=sw)
+            xv, wv = widen(x, sx, 1), torch.stack([widen(a, b, 128) for a, b in zip(w, sw)])
+        else:
+            x, w, more = x.to(BF), w.to(BF), {}
+            xv, wv = x.double(), w.double()
+        want, slack, end = grouped64(xv, wv, counts)
+        y = trk.matmul_grouped(x, w, c, out_dtype=F32, **more)
+        near(y, want, F32, slack * (K + 8) * U)
+        out = torch.full((rows, N), 3.0, device=gpu)
+        trk.matmul_grouped(x, w, c, out=out, **more)
+        assert torch.equal(out[:end], y[:end]) and (out[end:] == 3).all()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            z = trk.matmul_grouped(x, w, c, out_dtype=F32, **more)
+        for _ in range(3):
+            z.zero_()
+            trk.matmul_grouped(x, w, c, out=out, **more)
+            graph.replay()
+            assert torch.equal(z, y)
+        if dtype == BF:
+            yg = trk.matmul_grouped(x.requires_grad_(), w.requires_grad_(), c, out_dtype=F32)
+            assert torch.equal(yg, y)
+            dx, = torch.autograd.grad(yg, x, torch.ones_like(yg))
+            wx, ws, _ = grouped64(torch.ones(rows, N, device=gpu, dtype=torch.float64), wv.transpose(1, 2), counts)
+            near(dx, wx, BF, ws * (N + 4) * U)
+
+
+@gpu_test
 def test_products_of_turned_operands(trk, gpu):
     """operands whose columns are not next to each other in memory are laid out first"""
     g = gen_of(gpu, 34)
