@@ -318,9 +318,14 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     """y [M, N] = x [M, K] @ w [N, K]^T (+ bias [N] f32) of float8_e4m3fn codes with their scales: x_scale
     [M, ceil(K / 128)]; w_scale [N, ceil(K / 128)] (block_rows 1) or [ceil(N / 128), ceil(K / 128)] (128).
 
-    Each block's products are summed in f32, scaled and added in f32, and y is rounded once to out_dtype
-    (bfloat16 by default; float16, float32).  out: written in place of a new tensor (it must not overlap an
-    input)."""
+    Each block's sum is scaled by the product of its two scales (which has to stay in f32's normal range) and
+    added in f32, and y is rounded once to out_dtype (bfloat16 by default; float16, float32).  For float32 the
+    products of a block are summed in f32.  For the 16-bit types the 8-bit matrix instruction sums them: in each 8
+    columns (8 i .. 8 i + 7) it cuts every product, towards zero, to a multiple of 2^-13 of the largest one's power of
+    two.  That is 1.5e-5 of an ordinary sum, far below a rounding of y; but where large products cancel, small
+    ones beside them are lost, and float32 is the type to ask for.
+
+    out: written in place of a new tensor (it must not overlap an input)."""
     what = "matmul_fp8"
     dev = _on(x, what)
     if w.get_device() != dev:
@@ -463,7 +468,8 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
 
     bfloat16 / float16 x and w (one type; differentiable in both, a gradient of another type is rounded to
     theirs), or float8_e4m3fn with x_scale
-    [R, ceil(K / 128)] and w_scale [G, N or ceil(N / 128), ceil(K / 128)].  y is rounded once to out_dtype
+    [R, ceil(K / 128)] and w_scale [G, N or ceil(N / 128), ceil(K / 128)], summed as matmul_fp8 does it.  16-bit
+    products are summed in f32.  y is rounded once to out_dtype
     (x's type, or bfloat16 for 8 bits; float16, float32).  Rows behind the last group are zeros in a new y;
     with `out` (which must not overlap an input) they are left as they were."""
     what = "matmul_grouped"

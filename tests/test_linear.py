@@ -969,3 +969,39 @@ def test_long_offsets(trk, gpu):
     _, _, y64 = norm64(z[-1:], None, None, 1e-6)
     near(y[-1:], y64, BF, y64.abs() * 2.0 ** -18)
     check_codes(q[-1:], s[-1:], z[-1:].double(), 1)
+
+
+# ------------------------------------------------------------------------- what the 8-bit sums hold
+@gpu_test
+@pytest.mark.parametrize("M,N,K", [(5, 40, 128), (16, 200, 1024), (200, 300, 640), (640, 1280, 256), (600, 928, 6288), (4096, 4096, 128)])
+def test_matmul_fp8_cancelling_products(trk, gpu, M, N, K):
+    """Where large products cancel, f32 outputs keep what is left.  16-bit ones are within what their contract says: each
+    product cut to a multiple of 2^-13 of the power of two of the largest of its 8 columns' products, so off by less
+    than 2^-13 of that; columns without a large product lose no more than a sum in f32 does."""
+    g = gen_of(gpu, 55, M, N, K)
+    kb = -(-K // 128)
+    sx, sw = torch.ones(M, kb, device=gpu), torch.full((N, kb), 2.0 ** -6, device=gpu)
+    for low, period in ((1.0, 16), (2.0 ** -5, 16), (1.0, 128), (2.0 ** -5, 128)):
+        if period == 128 and K % 128:
+            continue
+        x, w = (torch.randint(1, 9, (n, K), device=gpu, generator=g).float() * low for n in (M, N))
+        for v, second in ((x, 448.0), (w, -448.0)):
+            if period == 128:  # two large products a block, alone in their 8 columns
+                for c in range(8):
+                    v[:, c::128] = 0
+            v[:, 3::period] = 448.0
+            v[:, (6 if period == 128 else 10)::period] = second
+        x, w = x.to(FP8), w.to(FP8)
+        xv, wv = x.double(), w.double() / 64
+        want, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+        near(trk.matmul_fp8(x, sx, w, sw, out_dtype=F32), want, F32, size * (132 + kb) * U)
+        # Each of a group's 8 products is cut by less than 2^-13 of the group's largest, max |x| max |w| at most, and 8 such
+        # cuts add up.  Two large products alone in their group are not cut: such columns count as zeros here.  The groups
+        # are added in f32, with the large products among the partial sums: every one of the n - 1 additions rounds
+        # what may be as large as the sum of all |products|.
+        if period == 128:
+            xv, wv = (v.unflatten(1, (-1, 128))[..., 8:].flatten(1) for v in (xv, wv))
+        top = [v.abs().unflatten(1, (-1, 8)).amax(2) for v in (torch.nn.functional.pad(t, (0, -t.shape[1] % 8)) for t in (xv, wv))]
+        slack = size * (132 + kb) * U + 8 * 2.0 ** -13 * (top[0] @ top[1].t())
+        for dtype in (BF, F16):
+            near(trk.matmul_fp8(x, sx, w, sw, out_dtype=dtype), want, dtype, slack)
