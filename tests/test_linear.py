@@ -1005,3 +1005,38 @@ def test_matmul_fp8_cancelling_products(trk, gpu, M, N, K):
         slack = size * (132 + kb) * U + 8 * 2.0 ** -13 * (top[0] @ top[1].t())
         for dtype in (BF, F16):
             near(trk.matmul_fp8(x, sx, w, sw, out_dtype=dtype), want, dtype, slack)
+
+
+def _nearest_code(v, top):
+    """The e4m3 code (as a value) nearest to v * 448 / top, ties to even, exactly: v and top have at most 11 bits, a
+    midpoint between two codes 5, so both sides of 448 |v| <> midpoint * top are whole in 64 bits."""
+    codes = torch.arange(127, dtype=torch.uint8, device=v.device).view(FP8).double()  # 0 .. 448, in order
+    a = v.abs() * 448
+    at = torch.searchsorted(codes, (a / top).contiguous()).clamp(1, 126)  # codes[at - 1] and codes[at] are around it, or next to that
+    best = torch.zeros_like(at)
+    for k in range(-2, 2):  # the number of midpoints below it, an exact midpoint counted where the code above it is even
+        i = (at + k).clamp(0, 125)
+        mid = (codes[i] + codes[i + 1]) / 2 * top
+        best = torch.maximum(best, torch.where((a > mid) | ((a == mid) & (i % 2 == 1)), i + 1, 0))
+    return codes[best] * v.sign()
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("block", [1, 128])
+def test_quantize_is_the_nearest_code(trk, gpu, dtype, block):
+    """codes of 16-bit values are the nearest ones with ties to even, without exception: a value next to a tie is
+    2^-17 of itself away from it, a tie stays one"""
+    g = gen_of(gpu, 60)
+    x = (torch.randn(2048, 1024, device=gpu, generator=g) * torch.exp(torch.randn(2048, 1, device=gpu, generator=g))).to(dtype)
+    q, s = trk.quantize_fp8(x, block_rows=block)
+    top = block_top(x.double(), block).repeat_interleave(128, 1).repeat_interleave(block, 0)
+    want = _nearest_code(x.double(), top)
+    assert int((q.double() != want).sum()) == 0
+    # there are ties among them
+    c = torch.arange(127, dtype=torch.uint8, device=gpu).view(FP8).double()
+    mid = (c[:-1] + c[1:]) / 2
+    a, t = (x.double().abs() * 448).view(-1)[:1 << 18], top.reshape(-1)[:1 << 18]
+    i = torch.searchsorted(mid, a / t).clamp(0, 125)
+    ties = sum(int((a == mid[(i + k).clamp(0, 125)] * t).sum()) for k in (-1, 0, 1))
+    assert ties > 50
