@@ -12,7 +12,7 @@ with the rows next to each other in memory.  A call takes scales of any strides.
 
 Every call runs on the current stream of its inputs' device and never waits for it; each may be
 captured into a graph.  The 16- and 32-bit norm and the 16-bit grouped product have gradients; the
-8-bit forms are for serving and refuse inputs that require one.
+8-bit forms are for serving and refuse inputs that require one.  Forward-mode derivatives are refused by all.
 """
 from __future__ import annotations
 
@@ -20,6 +20,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, lib
@@ -94,6 +95,15 @@ def _no_grad(what: str, *ts):
             raise NotImplementedError(f"{what}: the 8-bit form has no gradient; call it under torch.no_grad()")
 
 
+def _no_tangent(what: str, *ts):
+    """error of a dual tensor: the kernels know no forward-mode derivative, and a result without one reads as zero"""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # (no level is open, so no tensor has a tangent)
+        return
+    for t in ts:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what}: no forward-mode derivative")
+
+
 def _rows(t: torch.Tensor):
     """(t [.., D] as [R, D] with unit column stride and a row stride >= D, that stride); a view where t allows it"""
     if t.dim() != 2:
@@ -143,6 +153,7 @@ def _norm_inputs(what, x, weight, residual, eps):
             raise ValueError(f"{what}: residual is {list(residual.shape)}, x {list(x.shape)}")
     if not eps >= 0:
         raise ValueError(f"{what}: eps must not be negative")
+    _no_tangent(what, x, weight, residual)
     return dt
 
 
@@ -213,7 +224,8 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, residual
 
     x, residual [.., D] and weight [D] in bfloat16, float16 or float32 (one type).  Returns y, or with a
     residual (y, h): h is what the next layer adds to.  Sums are f32, the norm is of the unrounded f32
-    sum; y and h are rounded once.  Differentiable in all three inputs, and through both outputs."""
+    sum; y and h are rounded once.  Differentiable (backwards, once) in all three inputs, and through
+    both outputs."""
     dt = _norm_inputs("rms_norm", x, weight, residual, eps)
     if (x.requires_grad or (weight is not None and weight.requires_grad) or
             (residual is not None and residual.requires_grad)) and torch.is_grad_enabled():
@@ -263,6 +275,7 @@ def quantize_fp8(x: torch.Tensor, *, block_rows: int = 1):
     if x.dim() not in (2, 3) or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must be [rows, cols] or [B, rows, cols] with cols >= 1")
     _no_grad(what, x)
+    _no_tangent(what, x)
     R, D = x.shape[-2:]
     B = x.shape[0] if x.dim() == 3 else 1
     if not x.is_contiguous() and ((D > 1 and x.stride(-1) != 1) or (R > 1 and x.stride(-2) < D)):
@@ -347,6 +360,7 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
             raise ValueError(f"{what}: bias must be float32 [{N}]")
         bias = bias.contiguous()
     y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
+    _no_tangent(what, x, x_scale, w, w_scale, bias, out)
     x, ldx = _rows(x)
     w, ldw = _rows(w)
     part, parts = None, 1
@@ -487,6 +501,7 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
     if counts.dtype != torch.int32 or counts.dim() != 1 or counts.shape[0] != G:
         raise ValueError(f"{what}: counts must be int32 [{G}]")
     counts = counts.contiguous()
+    _no_tangent(what, x, x_scale, w, w_scale, out)
     if x.dtype == FP8:
         kb = (K + 127) // 128
         _scales(what, x_scale, "x_scale", x, dev, (M, kb), None)

@@ -1040,3 +1040,38 @@ def test_quantize_is_the_nearest_code(trk, gpu, dtype, block):
     i = torch.searchsorted(mid, a / t).clamp(0, 125)
     ties = sum(int((a == mid[(i + k).clamp(0, 125)] * t).sum()) for k in (-1, 0, 1))
     assert ties > 50
+
+
+# ------------------------------------------------------------------------- what autograd is told of a call
+@gpu_test
+def test_forward_mode_is_refused(trk, gpu):
+    """a dual tensor (forward-mode differentiation) is an error in each input of each operator: its tangent would be
+    lost, which reads as a derivative of zero"""
+    fw = torch.autograd.forward_ad
+    x = torch.randn(4, 32, device=gpu, generator=gen_of(gpu, 50))
+    b, w1 = x.to(BF), x[0].clone()
+    w3, c = b[None].repeat(2, 1, 1), torch.tensor([1, 3], device=gpu, dtype=torch.int32)
+    q, s = x.to(FP8), torch.ones(4, 1, device=gpu)
+    q3, s3, bias = q[None].repeat_interleave(2, 0), s[None].repeat(2, 1, 1), torch.zeros(4, device=gpu)
+    calls = [(trk.rms_norm, (x, w1), dict(residual=x)), (trk.rms_norm_fp8, (x, w1), dict(residual=x)),
+             (trk.quantize_fp8, (x,), {}), (trk.matmul_fp8, (q, s, q, s), dict(bias=bias, out=torch.empty(4, 4, device=gpu))),
+             (trk.matmul_grouped, (b, w3, c), dict(out=torch.empty(4, 4, device=gpu))),
+             (trk.matmul_grouped, (q, q3, c), dict(x_scale=s, w_scale=s3))]
+    for f, args, more in calls:
+        want = f(*args, **more)
+        with fw.dual_level():
+            got = f(*args, **more)  # (a level by itself is nothing)
+            for p, r in zip(*((t if isinstance(t, tuple) else (t,)) for t in (got, want))):
+                assert torch.equal(p.float(), r.float())
+            for at in [*range(len(args)), *more]:
+                t = args[at] if isinstance(at, int) else more[at]
+                if not t.is_floating_point():
+                    continue
+                d = fw.make_dual(t.detach(), torch.ones_like(t, dtype=F32).to(t.dtype))
+                a = [d if k == at else v for k, v in enumerate(args)]
+                m = {k: d if k == at else v for k, v in more.items()}
+                for mode in (torch.enable_grad, torch.no_grad):
+                    with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        f(*a, **m)
+    with fw.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        trk.rms_norm(x.clone().requires_grad_(), fw.make_dual(w1, w1))  # a gradient of the one, a tangent of the other
