@@ -325,6 +325,12 @@ def _out(what, out, out_dtype, x, M, N, default):
     return out
 
 
+def _wrote(out) -> None:
+    """tells autograd that the caller's `out` was written: a graph that saved it before refuses to go back over it"""
+    if out is not None:
+        torch.autograd.graph.increment_version(out)
+
+
 def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
                bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -371,6 +377,7 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     _launch(what, "trk_matmul_fp8", x, x.data_ptr(), ldx, x_scale.data_ptr(), *x_scale.stride(), w.data_ptr(), ldw,
             w_scale.data_ptr(), *w_scale.stride(), wb, _at(bias), M, N, K, y.data_ptr(), y.stride(0) if M > 1 else max(N, 1),
             _FLOAT[y.dtype], _at(part), parts)
+    _wrote(out)
     return y
 
 
@@ -401,9 +408,8 @@ def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_ta
         if parts > 1 and (x.data_ptr() | w.data_ptr() | ldx * item | ldw * item | w.stride(0) * item) % 16 == 0:
             part = x.new_empty((parts, M, N), dtype=torch.float32)
             _launch(what, "trk_matmul_grouped_split", x, *args, part.data_ptr(), parts)
-            return y
+            return
     _launch(what, "trk_matmul_grouped", x, *args)
-    return y
 
 
 def _lay(t: torch.Tensor) -> torch.Tensor:
@@ -444,7 +450,8 @@ class _Grouped(torch.autograd.Function):
         ctx.save_for_backward(x, w, counts)
         ctx.dt = dt
         y = x.new_empty((x.shape[0], w.shape[1]), dtype=out_dtype)
-        return _grouped_forward("matmul_grouped", x, None, w, None, 128, counts, dt, y, 1)
+        _grouped_forward("matmul_grouped", x, None, w, None, 128, counts, dt, y, 1)
+        return y
 
     @staticmethod
     @_backward_once
@@ -508,7 +515,9 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
         wb = _scales(what, w_scale, "w_scale", x, dev, (G, N, kb), (G, (N + 127) // 128, kb))
         _no_grad(what, x, x_scale, w, w_scale)
         y = _out(what, out, out_dtype, x, M, N, torch.bfloat16)
-        return _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, _lib.TRK_E4M3, y, int(out is None))
+        _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, _lib.TRK_E4M3, y, int(out is None))
+        _wrote(out)
+        return y
     dt = _type(x, _HALF, what, "x")
     if x_scale is not None or w_scale is not None:
         raise TypeError(f"{what}: scales go with float8_e4m3fn operands only")
@@ -521,4 +530,6 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
     y = _out(what, out, out_dtype, x, M, N, x.dtype)
     if _lay_pays(M, N, K, G):
         x, w = _lay(x), _lay(w)
-    return _grouped_forward(what, x, None, w, None, 128, counts, dt, y, int(out is None))
+    _grouped_forward(what, x, None, w, None, 128, counts, dt, y, int(out is None))
+    _wrote(out)
+    return y

@@ -1075,3 +1075,28 @@ def test_forward_mode_is_refused(trk, gpu):
                         f(*a, **m)
     with fw.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         trk.rms_norm(x.clone().requires_grad_(), fw.make_dual(w1, w1))  # a gradient of the one, a tangent of the other
+
+
+@gpu_test
+def test_out_counts_as_written(trk, gpu):
+    """a graph that saved `out` (or what it is a view of) before a call wrote it refuses its backward pass"""
+    g = gen_of(gpu, 51)
+    q, s = codes_of(g, 6, 64, 1, gpu)
+    b, c = torch.randn(6, 64, device=gpu, generator=g).to(BF), torch.tensor([6], device=gpu, dtype=torch.int32)
+    calls = (lambda o: trk.matmul_fp8(q, s, q, s, out=o), lambda o: trk.matmul_grouped(b, b[None], c, out=o),
+             lambda o: trk.matmul_grouped(q, q[None], c, x_scale=s, w_scale=s[None], out=o))
+    for call in calls:
+        for whole in (True, False):
+            big = torch.randn(8, 6, device=gpu, generator=g)
+            leaf = torch.randn(8, 6, device=gpu, generator=g).requires_grad_()
+            y, v = (leaf * big).sum(), big._version
+            call(big[:6] if not whole else big.view(-1)[:36].view(6, 6))
+            assert big._version == v + 1
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+        with torch.inference_mode():  # (no versions there)
+            o = torch.empty(6, 6, device=gpu)
+            assert call(o) is o
+        x, v = (t._version for t in (b, q))
+        call(torch.empty(6, 6, device=gpu))
+        assert (b._version, q._version) == (x, v)  # inputs are not written
