@@ -412,12 +412,16 @@ def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_ta
     _launch(what, "trk_matmul_grouped", x, *args)
 
 
+def _laid(t: torch.Tensor) -> bool:
+    """whether every row of t [.., K] of 16-bit values starts at a multiple of 16 bytes"""
+    return t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1])
+
+
 def _lay(t: torch.Tensor) -> torch.Tensor:
-    """t [.., K] of 16-bit values with every row at a multiple of 16 bytes: t, or a copy with padded rows"""
-    ld = (t.shape[-1] + 7) // 8 * 8
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]):
+    """t, or a copy of it with padded rows, so that _laid holds"""
+    if _laid(t):
         return t
-    return t.new_empty((*t.shape[:-1], ld))[..., :t.shape[-1]].copy_(t)
+    return t.new_empty((*t.shape[:-1], (t.shape[-1] + 7) // 8 * 8))[..., :t.shape[-1]].copy_(t)
 
 
 def _lay_pays(M: int, N: int, K: int, G: int) -> bool:
@@ -431,24 +435,40 @@ def _lay_pays(M: int, N: int, K: int, G: int) -> bool:
     return 1.5 * (K // 64) * rounds > 10 + (M + G * N) * K / 750_000
 
 
-def _lay_pays_backward(M: int, N: int, K: int, G: int) -> bool:
-    """The same for the gradients, of x, w and dy: about 3.5 us a step of 64 columns of dy, or of 64 rows of a
-    group where its rows are not split into parts."""
-    if not (N and K):
+def _lay_pays_backward(M: int, N: int, K: int, G: int, x, w, dy) -> bool:
+    """The same for the gradients, of the operands they read (x: dw is wanted, w: dx is).  dx goes over dy and w in steps of
+    64 columns of dy, about 3.5 us a step slower off the multiples of 16 bytes; dw over dy and x in steps of 64 rows of
+    a group's part, about 5.5 us a step; even groups.  Below 50 us the kernels run under the host's part of a call,
+    and the copies' host part is what counts.  us without / with copies of all operands, dx, dw, both: 8 groups of 16384 x
+    1501 x 1203 in all 243 / 122, 265 / 119, 399 / 222; 3 of 3105 x 1301 x 1111 120 / 68, 96 / 71, 193 / 98; 64 of 4096 x
+    511 x 513 55 / 67, 51 / 67, 81 / 84; 2 of 214 x 755 x 943 66 / 67, 51 / 67, 67 / 86."""
+    if not (M and N and K):
         return False
-    tiles = -(-N // 256) * -(-K // 256) * G
-    steps = N // 64 + M // (64 * G * max(1, min(256 // tiles, M // (256 * G))))
-    rounds = max(1, (tiles + (M // 256 + min(G, M)) * -(-K // 256)) // 512)
-    return 3.5 * steps * rounds > 20 + (M * (N + K) + G * N * K) / 750_000
+    used, wide = min(G, M), -(-K // 256)
+    slower = 0.0
+    if w is not None:
+        slower += 3.5 * (N // 64) * -(-used * -(-M // (used * 256)) * wide // 256)
+    if x is not None:
+        tiles = -(-N // 256) * wide * G
+        split = max(1, min(256 // tiles, M // (256 * G)))
+        slower += 5.5 * (M // (64 * G * split)) * -(-tiles * split // 256)
+    both = x is not None and w is not None
+    if slower + (1 + both) * M * N * K / 300_000_000 <= 50:
+        return False
+    copied = [t.numel() for t in (x, w, dy) if t is not None and not _laid(t)]
+    return slower > 7 * len(copied) + sum(copied) / 1_270_000
 
 
 class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, counts, dt, out_dtype):
+        want_x, want_w = ctx.needs_input_grad[:2]
+        ctx.dt, ctx.sizes = dt, (x.shape[0], *w.shape)
         if _lay_pays(x.shape[0], w.shape[1], w.shape[2], w.shape[0]):
             x, w = _lay(x), _lay(w)
-        ctx.save_for_backward(x, w, counts)
-        ctx.dt = dt
+        # What the wanted gradients read; where x and w were copied, the copies: made again in the backward pass they would
+        # cost 454 us a training step against 374 (16 groups of 8192 x 2047 x 2047), kept they cost their bytes till then
+        ctx.save_for_backward(x if want_w else None, w if want_x else None, counts)
         y = x.new_empty((x.shape[0], w.shape[1]), dtype=out_dtype)
         _grouped_forward("matmul_grouped", x, None, w, None, 128, counts, dt, y, 1)
         return y
@@ -457,26 +477,29 @@ class _Grouped(torch.autograd.Function):
     @_backward_once
     def backward(ctx, dy):
         x, w, counts = ctx.saved_tensors
-        M, K = x.shape
-        G, N = w.shape[:2]
-        if dy.dtype != x.dtype:
-            dy = dy.to(x.dtype)
-        if _lay_pays_backward(M, N, K, G):
-            x, w, dy = _lay(x), _lay(w), _lay(dy)
-        x, ldx = _rows(x)
-        w, ldw = _weights(w)
+        M, G, N, K = ctx.sizes
+        read = w if x is None else x
+        if dy.dtype != read.dtype:
+            dy = dy.to(read.dtype)
+        if _lay_pays_backward(M, N, K, G, x, w, dy):
+            x, w, dy = (None if t is None else _lay(t) for t in (x, w, dy))
         dy, ldy = _rows(dy)
-        dx = x.new_empty((M, K)) if ctx.needs_input_grad[0] else None
-        dw = part = None
+        px, pw = (None, 0), (None, 0, 0)
+        dx = dw = part = None
         parts = 1
-        if ctx.needs_input_grad[1]:
-            dw = x.new_empty((G, N, K))
+        if w is not None:
+            w, ldw = _weights(w)
+            pw = (w.data_ptr(), ldw, w.stride(0))
+            dx = dy.new_empty((M, K))
+        if x is not None:
+            x, ldx = _rows(x)
+            px = (x.data_ptr(), ldx)
+            dw = dy.new_empty((G, N, K))
             parts = lib().trk_matmul_grouped_bwd_parts(G, M, N, K)
             if parts > 1:
-                part = x.new_empty((parts, G, N, K), dtype=torch.float32)
-        _launch("matmul_grouped backward", "trk_matmul_grouped_bwd", x, dy.data_ptr(), ldy, x.data_ptr(), ldx, w.data_ptr(), ldw,
-                w.stride(0), counts.data_ptr(), G, M, N, K, ctx.dt, _at(dx), max(K, 1), _at(dw), max(K, 1), N * K, _at(part),
-                parts)
+                part = dy.new_empty((parts, G, N, K), dtype=torch.float32)
+        _launch("matmul_grouped backward", "trk_matmul_grouped_bwd", dy, dy.data_ptr(), ldy, *px, *pw, counts.data_ptr(), G, M, N, K,
+                ctx.dt, _at(dx), max(K, 1), _at(dw), max(K, 1), N * K, _at(part), parts)
         return dx, dw, None, None, None
 
 

@@ -1100,3 +1100,29 @@ def test_out_counts_as_written(trk, gpu):
         x, v = (t._version for t in (b, q))
         call(torch.empty(6, 6, device=gpu))
         assert (b._version, q._version) == (x, v)  # inputs are not written
+
+
+@gpu_test
+@pytest.mark.parametrize("K", [1112, 1111])
+def test_gradients_asked_for_alone(trk, gpu, K):
+    """each gradient alone has the bits of both together, and what only the other one reads is neither kept nor copied"""
+    g = gen_of(gpu, 53)
+    c = torch.tensor([1500, 0, 1600], device=gpu, dtype=torch.int32)
+    R, N = 3105, 1301
+    x0, w0 = (torch.randn(*s, K, device=gpu, generator=g).to(BF) for s in ((R,), (3, N)))
+    dy = torch.randn(R, N, device=gpu, generator=g).to(BF)
+
+    def grads(on_x, on_w):
+        x, w = x0.detach().requires_grad_(on_x), w0.detach().requires_grad_(on_w)
+        y = trk.matmul_grouped(x, w, c)
+        saved = [t for t in y.grad_fn.saved_tensors if t is not None and t.dtype == BF]
+        if K % 8 == 0:
+            assert {t.data_ptr() for t in saved} <= {x.data_ptr(), w.data_ptr()}  # no copies
+        return torch.autograd.grad(y, [t for t in (x, w) if t.requires_grad], dy), [t.dim() for t in saved]
+
+    (dx, dw), saved = grads(True, True)
+    assert saved == [2, 3]
+    (one,), saved = grads(True, False)
+    assert torch.equal(one, dx) and saved == [3]
+    (one,), saved = grads(False, True)
+    assert torch.equal(one, dw) and saved == [2]
