@@ -258,8 +258,8 @@ struct BwdArgs {
   int64_t ldh, ldy, lddh, ldx, R, D, parts;
 };
 
-// dx of the rows of workgroup blockIdx.x, blockIdx.x + gridDim.x, ..; part[blockIdx.x][D] its
-// sum of dy n over those rows.  (T, NV, LOOP as above.)
+// dx (null: not wanted) of the rows of workgroup blockIdx.x, blockIdx.x + gridDim.x, ..; part[blockIdx.x][D]
+// its sum of dy n over those rows.  (T, NV, LOOP as above.)
 template <int DT, int T, int NV, int BT, bool LOOP>
 __global__ __launch_bounds__(BT) void rms_norm_bwd_kernel(BwdArgs A) {
   typedef typename El<DT>::T E;
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(BT) void rms_norm_bwd_kernel(BwdArgs A) {
       const float r = on ? A.rstd[rr] : 0.0f;
       float n[NV][kV], g[NV][kV], dot = 0.0f;
       if constexpr (LOOP) {  // the whole row's mean(g n) first
-        for (int64_t b2 = 0; b2 < A.D; b2 += (int64_t)T * kV) {
+        for (int64_t b2 = 0; b2 < (A.dx ? A.D : 0); b2 += (int64_t)T * kV) {
           const int64_t c = b2 + (int64_t)t * kV;
           float a[kV], b[kV], ww[kV];
           load8<DT>(hp + c, D - c, D, a);
@@ -311,6 +311,7 @@ __global__ __launch_bounds__(BT) void rms_norm_bwd_kernel(BwdArgs A) {
           if constexpr (!LOOP) dot = fmaf(g[i][j], n[i][j], dot);
         }
       }
+      if (!A.dx) continue;  // the same in every thread
       const float m = sum_row<T>(dot, red) / (float)A.D;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -547,11 +548,12 @@ int64_t trk_rms_norm_bwd_parts(int64_t R, int64_t D) { return R <= 0 || D <= 0 ?
 int trk_rms_norm_bwd(const void* h, int64_t ldh, const void* weight, const float* rstd, const void* dy, int64_t ldy,
                      const void* dh, int64_t lddh, int64_t R, int64_t D, int dtype, void* dx, int64_t ldx,
                      float* part, int64_t parts, void* dw, void* stream) {
-  if (int rc = check_norm("trk_rms_norm_bwd", h, ldh, dh, lddh, R, D, dtype, dx, ldx, dy, ldy, 0.0f)) return rc;
+  if (int rc = check_norm("trk_rms_norm_bwd", h, ldh, dh, lddh, R, D, dtype, dy, ldy, dx, ldx, 0.0f)) return rc;
+  if (!dx && !dw) return TRK_OK;
   hipStream_t st = (hipStream_t)stream;
   TRK_REQUIRE(!dw || (part && parts >= 1), "trk_rms_norm_bwd: dw needs the workspace part [parts][D]");
   if (R > 0) {
-    TRK_REQUIRE(dy && rstd, "trk_rms_norm_bwd: null pointer");
+    TRK_REQUIRE(rstd, "trk_rms_norm_bwd: null pointer");
     TRK_REQUIRE(!dw || parts == bwd_parts(R, D), "trk_rms_norm_bwd: parts must be trk_rms_norm_bwd_parts(R, D)");
   }
   const BwdArgs A{h, weight, dy, dh, rstd, dx, dw, dw ? part : nullptr, ldh, ldy, lddh, ldx, R, D,

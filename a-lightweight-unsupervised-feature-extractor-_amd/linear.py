@@ -204,9 +204,10 @@ class _RmsNorm(torch.autograd.Function):
         h2, ldh = _rows(h)
         y2, ldy = _rows(dy)
         R, D = h2.shape
-        e2, lde = (None, 0) if dh is None else _rows(dh)
+        want = need_x or need_r
+        e2, lde = (None, 0) if dh is None or not want else _rows(dh)
         w = None if weight is None else weight.contiguous()
-        dx = _like(h)
+        dx = _like(h) if want else None
         part = dw = None
         parts = 1
         if need_w:
@@ -214,7 +215,7 @@ class _RmsNorm(torch.autograd.Function):
             part = h.new_empty((parts, D), dtype=torch.float32)
             dw = h.new_empty(D)
         _launch("rms_norm backward", "trk_rms_norm_bwd", h, h2.data_ptr(), ldh, _at(w), rstd.data_ptr(), y2.data_ptr(), ldy,
-                _at(e2), lde, R, D, ctx.dt, dx.data_ptr(), D, _at(part), parts, _at(dw))
+                _at(e2), lde, R, D, ctx.dt, _at(dx), D, _at(part), parts, _at(dw))
         return dx if need_x else None, dw, dx if need_r else None, None, None
 
 

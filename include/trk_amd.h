@@ -316,8 +316,8 @@ int trk_enc_head(const long long* tsums, int64_t R, int64_t P, int64_t C, const 
  *   multiple of 16 bytes (q must own those bytes).  scale = max(|y|, 2^-117) / 448 over
  *   the block; NaN values give NaN codes and are left out of the maximum; a block that
  *   holds an infinity has an infinite scale (all of it comes back as NaN).
- * trk_rms_norm_bwd: dx = r (g - n mean(g n)) + dh with g = dy weight, n = h r (dh NULL: 0),
- *   and dw (NULL: not wanted) [D] = sum over rows of dy n, joined in a fixed order from the
+ * trk_rms_norm_bwd: dx = r (g - n mean(g n)) + dh with g = dy weight, n = h r (dh NULL: 0; dx NULL:
+ *   not wanted, dh is not read), and dw (NULL: not wanted) [D] = sum over rows of dy n, joined in a fixed order from the
  *   workspace part [parts][D] f32, parts = trk_rms_norm_bwd_parts(R, D).
  * trk_quantize_fp8: B matrices x [R][D] (xb, qb, sb: strides of the batch) in blocks of
  *   block_rows (1 or 128) x 128: scale[b * sb + kb * scale_ld + row or row block]; padding

@@ -1126,3 +1126,29 @@ def test_gradients_asked_for_alone(trk, gpu, K):
     assert torch.equal(one, dx) and saved == [3]
     (one,), saved = grads(False, True)
     assert torch.equal(one, dw) and saved == [2]
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,cols", [(7, 100), (2500, 512), (300, 1500), (40, 5000), (3, 20001)])
+def test_norm_weight_gradient_alone(trk, gpu, rows, cols, dtype):
+    """dw without dx has the same bits, and no rows are made for dx"""
+    g = gen_of(gpu, 54, rows)
+    x, dy = (torch.randn(rows, cols, device=gpu, generator=g).to(dtype) for _ in range(2))
+    w = torch.randn(cols, device=gpu, generator=g).to(dtype).requires_grad_()
+    a = x.detach().requires_grad_()
+    _, want = torch.autograd.grad(trk.rms_norm(a, w, eps=1e-5), (a, w), dy)
+    y = trk.rms_norm(x, w, eps=1e-5)
+    torch.cuda.synchronize()
+    made = torch.cuda.memory_stats()["allocation.all.allocated"]
+    got, = torch.autograd.grad(y, w, dy)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] - made == 2  # the partial rows and dw
+    assert torch.equal(got, want)
+
+
+def test_norm_backward_of_nothing(trk):
+    """neither gradient wanted: nothing is launched; dx alone and dw alone are what a call may ask for"""
+    L, v, z = trk.lib(), ctypes.c_void_p(256), None
+    assert L.trk_rms_norm_bwd(v, 8, z, v, v, 8, z, 0, 4, 8, 0, z, 8, z, 1, z, z) == 0
+    assert L.trk_rms_norm_bwd(v, 8, z, v, z, 8, z, 0, 4, 8, 0, v, 8, z, 1, z, z) == -1 and b"null" in L.trk_last_error()
+    assert L.trk_rms_norm_bwd(v, 8, z, z, v, 8, z, 0, 4, 8, 0, v, 8, z, 1, z, z) == -1 and b"null" in L.trk_last_error()
