@@ -174,15 +174,38 @@ def _norm_forward(dt, x, weight, residual, eps, want_rstd):
     return y, h, rstd
 
 
-def _backward_once(backward):
-    """backward, which torch.autograd.function.once_differentiable marks (so that a second derivative is an error and not
-    zero) where a graph of it is asked for; it costs 4 us of every call"""
-    marked = torch.autograd.function.once_differentiable(backward)
+class _Tied(torch.autograd.Function):
+    """The n first tensors, hung on all of them: whoever differentiates them gets an error."""
+    @staticmethod
+    def forward(ctx, what, n, *ts):
+        ctx.what = what
+        return ts[:n]
 
-    def call(ctx, *grads):
-        return (marked if torch.is_grad_enabled() else backward)(ctx, *grads)
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what}: no second derivative (its backward pass is once_differentiable)")
 
-    return call
+
+def _backward_once(what):
+    """For a backward pass without a derivative.  Where a graph of it is asked for, its gradients are hung on what came in and
+    on every saved input: a second derivative is then an error for each of them.  (torch's own mark looks at
+    what came in only: after a sum, whose gradient is a constant, the second derivative would silently be zero.)"""
+    def mark(backward):
+        def call(ctx, *grads):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *grads)
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            of = [t for t in (*grads, *ctx.saved_tensors, *ctx.links) if t is not None and t.requires_grad]
+            given = [t for t in out if t is not None]
+            if not of or not given:
+                return out
+            tied = iter(_Tied.apply(what, len(given), *given, *of))
+            return tuple(None if t is None else next(tied) for t in out)
+
+        return call
+
+    return mark
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -190,12 +213,12 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, dt, eps):
         y, h, rstd = _norm_forward(dt, x, weight, residual, eps, True)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
-        ctx.dt, ctx.pair = dt, h is not None
+        ctx.dt, ctx.links = dt, ()
         ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
 
     @staticmethod
-    @_backward_once
+    @_backward_once("rms_norm")
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
@@ -462,10 +485,10 @@ def _lay_pays_backward(M: int, N: int, K: int, G: int, x, w, dy) -> bool:
 
 class _Grouped(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, counts, dt, out_dtype):
+    def forward(ctx, x, w, counts, dt, out_dtype, lay, links):
         want_x, want_w = ctx.needs_input_grad[:2]
-        ctx.dt, ctx.sizes = dt, (x.shape[0], *w.shape)
-        if _lay_pays(x.shape[0], w.shape[1], w.shape[2], w.shape[0]):
+        ctx.dt, ctx.sizes, ctx.links = dt, (x.shape[0], *w.shape), links
+        if lay:
             x, w = _lay(x), _lay(w)
         # What the wanted gradients read; where x and w were copied, the copies: made again in the backward pass they would
         # cost 454 us a training step against 374 (16 groups of 8192 x 2047 x 2047), kept they cost their bytes till then
@@ -475,7 +498,7 @@ class _Grouped(torch.autograd.Function):
         return y
 
     @staticmethod
-    @_backward_once
+    @_backward_once("matmul_grouped")
     def backward(ctx, dy):
         x, w, counts = ctx.saved_tensors
         M, G, N, K = ctx.sizes
@@ -501,7 +524,7 @@ class _Grouped(torch.autograd.Function):
                 part = dy.new_empty((parts, G, N, K), dtype=torch.float32)
         _launch("matmul_grouped backward", "trk_matmul_grouped_bwd", dy, dy.data_ptr(), ldy, *px, *pw, counts.data_ptr(), G, M, N, K,
                 ctx.dt, _at(dx), max(K, 1), _at(dw), max(K, 1), N * K, _at(part), parts)
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_scale: Optional[torch.Tensor] = None,
@@ -550,7 +573,10 @@ def matmul_grouped(x: torch.Tensor, w: torch.Tensor, counts: torch.Tensor, *, x_
             raise ValueError(f"{what}: `out` has no gradient; call without it, or under torch.no_grad()")
         if out_dtype is not None and out_dtype not in _FLOAT:
             raise TypeError(f"{what}: out_dtype must be one of {', '.join(str(k)[6:] for k in _FLOAT)}, got {out_dtype}")
-        return _Grouped.apply(x, w, counts, dt, out_dtype or x.dtype)
+        lay = _lay_pays(M, N, K, G)
+        # (empty tensors with the history of x and w, which their padded copies lack)
+        links = tuple(t[:0].clone() for t in (x, w) if t.requires_grad) if lay else ()
+        return _Grouped.apply(x, w, counts, dt, out_dtype or x.dtype, lay, links)
     y = _out(what, out, out_dtype, x, M, N, x.dtype)
     if _lay_pays(M, N, K, G):
         x, w = _lay(x), _lay(w)

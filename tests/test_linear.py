@@ -1152,3 +1152,33 @@ def test_norm_backward_of_nothing(trk):
     assert L.trk_rms_norm_bwd(v, 8, z, v, v, 8, z, 0, 4, 8, 0, z, 8, z, 1, z, z) == 0
     assert L.trk_rms_norm_bwd(v, 8, z, v, z, 8, z, 0, 4, 8, 0, v, 8, z, 1, z, z) == -1 and b"null" in L.trk_last_error()
     assert L.trk_rms_norm_bwd(v, 8, z, z, v, 8, z, 0, 4, 8, 0, v, 8, z, 1, z, z) == -1 and b"null" in L.trk_last_error()
+
+
+@gpu_test
+def test_no_second_derivative_of_a_constant_gradient(trk, gpu):
+    """the first derivative also depends on the inputs where the gradient that came in does not: its derivative is an
+    error then too, for every leaf it depends on and beside other terms of a loss, and not left out of the sum"""
+    g = gen_of(gpu, 52)
+    x, r = (torch.randn(9, 37, device=gpu, generator=g).requires_grad_() for _ in range(2))
+    v = torch.randn(37, device=gpu, generator=g).requires_grad_()
+    c = torch.tensor([40, 0, 500], device=gpu, dtype=torch.int32)
+    cases = [(lambda: trk.rms_norm(x), (x,), x), (lambda: trk.rms_norm(x, v), (x, v), v), (lambda: trk.rms_norm(x, v), (x, v), x),
+             (lambda: trk.rms_norm(x, v, residual=r)[0], (x, v, r), r), (lambda: trk.rms_norm(x.detach(), v, residual=r)[0], (v, r), r)]
+    for rows, N, K in ((550, 40, 24), (3105, 1301, 1111)):  # (the second one's rows are copied to padded ones)
+        a = torch.randn(rows, K, device=gpu, generator=g).to(BF).requires_grad_()
+        w = torch.randn(3, N, K, device=gpu, generator=g).to(BF).requires_grad_()
+        cases += [(lambda a=a, w=w: trk.matmul_grouped(a, w, c), (a, w), a), (lambda a=a, w=w: trk.matmul_grouped(a, w, c), (a, w), w)]
+    for call, leaves, of in cases:
+        for way in ("backward", "grad"):
+            ds = torch.autograd.grad(call().sum(), leaves, create_graph=True)
+            assert all(d.requires_grad for d in ds)
+            loss = sum(d.float().square().sum() for d in ds) + of.float().square().sum()
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                loss.backward() if way == "backward" else torch.autograd.grad(loss, of)
+        # the values are those of a plain backward pass
+        for d, e in zip(ds, torch.autograd.grad(call().sum(), leaves)):
+            assert torch.equal(d, e)
+    # only the sum is used: what comes back is the gradient that came in
+    h = trk.rms_norm(x, residual=r)[1]
+    d = torch.autograd.grad(h.sum(), (x, r), create_graph=True)
+    assert all(torch.equal(t, torch.ones_like(x)) for t in d)
