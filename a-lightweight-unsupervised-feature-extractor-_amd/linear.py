@@ -53,7 +53,13 @@ _FLOAT = {torch.float32: _lib.TRK_F32, torch.bfloat16: _lib.TRK_BF16, torch.floa
 _HALF = {torch.bfloat16: _lib.TRK_BF16, torch.float16: _lib.TRK_F16}
 
 
-_device = torch._C._cuda_getDevice
+def _public_stream(idx: int) -> int:
+    return torch.cuda.current_stream(idx).cuda_stream
+
+
+# the raw accessors are one C call each; a torch without them has the public ones
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream_of = _raw_stream or _public_stream
 
 
 def _launch(what: str, fn: str, x: torch.Tensor, *args):
@@ -61,10 +67,10 @@ def _launch(what: str, fn: str, x: torch.Tensor, *args):
     idx = x.get_device()
     f = getattr(lib(), fn)
     if idx == _device():
-        rc = f(*args, _raw_stream(idx))
+        rc = f(*args, _stream_of(idx))
     else:
         with torch.cuda.device(idx):
-            rc = f(*args, _raw_stream(idx))
+            rc = f(*args, _stream_of(idx))
     if rc:
         check(rc, what)
 

@@ -1182,3 +1182,42 @@ def test_no_second_derivative_of_a_constant_gradient(trk, gpu):
     h = trk.rms_norm(x, residual=r)[1]
     d = torch.autograd.grad(h.sum(), (x, r), create_graph=True)
     assert all(torch.equal(t, torch.ones_like(x)) for t in d)
+
+
+def test_import_without_raw_accessors():
+    """the package imports on a torch without the private accessors that save a call some host time"""
+    import os
+    import subprocess
+    import sys
+    code = f"""
+import importlib, sys, torch
+for n in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, n):
+        delattr(torch._C, n)
+sys.path.insert(0, {os.path.dirname(os.path.dirname(os.path.abspath(__file__)))!r})
+trk = importlib.import_module("a-lightweight-unsupervised-feature-extractor-_amd")
+assert trk.rms_norm and trk.roi_align
+linear = sys.modules[trk.__name__ + ".linear"]
+assert linear._device is torch.cuda.current_device and linear._stream_of is linear._public_stream
+print("as meant")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "as meant" in r.stdout, r.stderr
+
+
+@gpu_test
+def test_calls_through_public_accessors(trk, gpu, monkeypatch):
+    import sys
+    linear = sys.modules[trk.__name__ + ".linear"]
+    monkeypatch.setattr(linear, "_device", torch.cuda.current_device)
+    monkeypatch.setattr(linear, "_stream_of", linear._public_stream)
+    side = torch.cuda.Stream()
+    assert linear._public_stream(0) == torch.cuda.current_stream().cuda_stream
+    x = torch.randn(5, 40, device=gpu, generator=gen_of(gpu, 61))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert linear._public_stream(0) == side.cuda_stream
+        y = trk.rms_norm(x)
+    torch.cuda.current_stream().wait_stream(side)
+    y64 = norm64(x, None, None, 1e-6)[2]
+    near(y, y64, F32, y64.abs() * 2.0 ** -18)
