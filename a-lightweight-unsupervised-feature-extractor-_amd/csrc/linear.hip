@@ -1222,7 +1222,8 @@ int few_strips(int64_t G, int64_t M, int64_t N) {
 // Few 128-tiles (of even groups) and long rows: K in parts, as many as give 384 tiles of at least 8 steps, up to 8.
 // In 16 / 8 bits, us, 1 part / the rule's: 8 groups, 512 x 2048 x 8192 115 / 66 and 55 / 36; 1000 x 1024 x 8192 in 4
 // 83 / 38 and 54 / 29; 600 x 1024 x 16384 in 2 162 / 50 and 100 / 36; 600 x 928 x 6288 90 / 32 and 57 / 25; 1000 x
-// 1000 x 2048 28 / 22 in 16 bits, in 8 (16 steps) 18 against 22 in 4 parts.  Rows that strips of 16 take stay whole
+// 1000 x 2048 28 / 22 in 16 bits, in 8 (16 steps) 18 against 22 in 4 parts; 16 x 20000 x 8192 128 / 85 and 52 / 38, 8
+// groups, 16 x 2304 x 8192 122 / 78 and 54 / 40.  Rows that strips of 16 take stay whole
 // (8 groups, 64 x 2048 x 8192 52 against 56 in 3 parts), and up to 64 steps 256 strips of 64 (64 x 4096 x 4096 24 /
 // 19 in 16 bits, 17 / 18 in 8).  The join costs about 8 us.
 int64_t parts_of(int64_t G, int64_t M, int64_t N, int64_t steps) {

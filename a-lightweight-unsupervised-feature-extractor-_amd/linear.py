@@ -400,7 +400,7 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     x, ldx = _rows(x)
     w, ldw = _rows(w)
     part, parts = None, 1
-    if M > 16 and K > 24 * 128:  # (one part always, else)
+    if K > 24 * 128:  # (one part always, else)
         parts = lib().trk_matmul_fp8_parts(M, N, K)
         if parts > 1:
             part = x.new_empty((parts, M, N), dtype=torch.float32)
@@ -431,7 +431,7 @@ def _grouped_forward(what, x, x_scale, w, w_scale, wb, counts, in_dt, y, zero_ta
     args = (x.data_ptr(), ldx, *sx, w.data_ptr(), ldw, w.stride(0), *sw, wb, counts.data_ptr(), G, M, N, K, in_dt,
             y.data_ptr(), y.stride(0) if M > 1 else max(N, 1), _FLOAT[y.dtype], zero_tail)
     item = x.element_size()
-    if M > 16 and K * item > 24 * 128:  # (one part always, else)
+    if K * item > 24 * 128:  # (one part always, else)
         parts = lib().trk_matmul_grouped_parts(G, M, N, K, in_dt)
         # rows off the multiples of 16 bytes that were not copied are bound by their way through the registers (64 x
         # 6000 x 3500: strips 32 us, 47 in 6 parts)

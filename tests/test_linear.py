@@ -1221,3 +1221,39 @@ def test_calls_through_public_accessors(trk, gpu, monkeypatch):
     torch.cuda.current_stream().wait_stream(side)
     y64 = norm64(x, None, None, 1e-6)[2]
     near(y, y64, F32, y64.abs() * 2.0 ** -18)
+
+
+@gpu_test
+@pytest.mark.parametrize("kind", ["fp8", "bf16"])
+@pytest.mark.parametrize("G,M,N,K", [(1, 16, 20000, 8192), (1, 3, 17000, 4224), (8, 16, 2304, 8192), (16, 9, 2304, 6400), (1, 16, 4096, 8192)])
+def test_parts_of_few_rows(trk, gpu, G, M, N, K, kind):
+    """the public call sums K in as many parts as the library suggests, with few rows as with many: the same bits"""
+    g = gen_of(gpu, 62, G, M, N)
+    L, st = trk.lib(), torch.cuda.current_stream().cuda_stream
+    counts = [M // G + (i < M % G) for i in range(G)]
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    x, sx = codes_of(g, M, K, 1, gpu)
+    w, sw = codes_of(g, N, K, 128, gpu, (G,))
+    y = torch.empty(M, N, device=gpu)
+    if kind == "fp8":
+        parts = L.trk_matmul_grouped_parts(G, M, N, K, 4)
+        assert G > 1 or parts == L.trk_matmul_fp8_parts(M, N, K)
+        part = torch.empty(parts, M, N, device=gpu)
+        got = [trk.matmul_grouped(x, w, c, x_scale=sx, w_scale=sw, out_dtype=F32)]
+        if G == 1:
+            got.append(trk.matmul_fp8(x, sx, w[0], sw[0], out_dtype=F32))
+        rc = L.trk_matmul_grouped_split(x.data_ptr(), K, sx.data_ptr(), *sx.stride(), w.data_ptr(), K, N * K, sw.data_ptr(),
+                                        sw.stride(1), sw.stride(2), sw.stride(0), 128, c.data_ptr(), G, M, N, K, 4, y.data_ptr(), N,
+                                        0, 1, part.data_ptr(), parts, st)
+    else:
+        x, w = x.to(BF), w.to(BF)
+        parts = L.trk_matmul_grouped_parts(G, M, N, K, 1)
+        part = torch.empty(parts, M, N, device=gpu)
+        got = [trk.matmul_grouped(x, w, c, out_dtype=F32)]
+        rc = L.trk_matmul_grouped_split(x.data_ptr(), K, None, 0, 0, w.data_ptr(), K, N * K, None, 0, 0, 0, 128, c.data_ptr(),
+                                        G, M, N, K, 1, y.data_ptr(), N, 0, 1, part.data_ptr(), parts, st)
+    assert rc == 0 and (parts > 1) == (N != 4096)
+    assert all(torch.equal(t, y) for t in got)
+    for i, (a, b) in enumerate(bounds_of(counts, M)[0]):
+        xv, wv = (widen(x[a:b], sx[a:b], 1), widen(w[i], sw[i], 128)) if kind == "fp8" else (x[a:b].double(), w[i].double())
+        near(y[a:b], xv @ wv.t(), F32, (xv.abs() @ wv.abs().t()) * (K + 8 + parts) * U)
