@@ -1257,3 +1257,64 @@ def test_parts_of_few_rows(trk, gpu, G, M, N, K, kind):
     for i, (a, b) in enumerate(bounds_of(counts, M)[0]):
         xv, wv = (widen(x[a:b], sx[a:b], 1), widen(w[i], sw[i], 128)) if kind == "fp8" else (x[a:b].double(), w[i].double())
         near(y[a:b], xv @ wv.t(), F32, (xv.abs() @ wv.abs().t()) * (K + 8 + parts) * U)
+
+
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_matmul_fp8_tiles_f16(trk, gpu, M, N, K, block):
+    g = gen_of(gpu, M, N, K, 57)
+    x, sx = codes_of(g, M, K, 1, gpu)
+    w, sw = codes_of(g, N, K, block, gpu)
+    sw = sw / 64  # (sums within f16's range)
+    xv, wv = widen(x, sx, 1), widen(w, sw, block)
+    want = xv @ wv.t()
+    y = trk.matmul_fp8(x, sx, w, sw, out_dtype=F16)
+    assert y.isfinite().all()
+    near(y, want, F16, product_slack(xv, wv, sx.shape[1], F16) + want.abs() * 2 * U)
+
+
+@gpu_test
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("counts,N,K", BIG, ids=lambda c: str(len(c)) + "g" if isinstance(c, list) else str(c))
+def test_matmul_grouped_tiles_f16(trk, gpu, counts, N, K, block):
+    g = gen_of(gpu, sum(counts), N, K, 58)
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    rows = sum(counts) + 77
+    x, sx = codes_of(g, rows, K, 1, gpu)
+    w, sw = codes_of(g, N, K, block, gpu, (len(counts),))
+    sw = sw / 64
+    xv, wv = widen(x, sx, 1), widen(w, sw, block)
+    want, _, end = grouped64(xv, wv, counts)
+    slack = torch.zeros_like(want)
+    for i, (a, b) in enumerate(bounds_of(counts, rows)[0]):
+        slack[a:b] = product_slack(xv[a:b], wv[i], sx.shape[1], F16)
+    y = trk.matmul_grouped(x, w, c, x_scale=sx, w_scale=sw, out_dtype=F16)
+    near(y, want, F16, slack + want.abs() * 2 * U)
+    assert (y[end:] == 0).all()
+
+
+@gpu_test
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_matmul_grouped_long_odd_rows(trk, gpu, kind):
+    """long rows of an odd length: padded to 16 bytes they run with K in parts, next to each other whole"""
+    g = gen_of(gpu, 59, len(kind))
+    counts, rows, N, K = [140, 0, 300, 61], 520, 700, 5003
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    assert trk.lib().trk_matmul_grouped_parts(4, rows, N, K, 4 if kind == "fp8" else 1) > 1
+    x, sx = codes_of(g, rows, K, 1, gpu)
+    w, sw = codes_of(g, N, K, 128, gpu, (4,))
+    if kind == "fp8":
+        more, xv, wv = dict(x_scale=sx, w_scale=sw), widen(x, sx, 1), torch.stack([widen(a, b, 128) for a, b in zip(w, sw)])
+        pad = lambda t: torch.nn.functional.pad(t.view(torch.uint8), (0, -K % 16)).view(FP8)[..., :K]  # noqa: E731
+    else:
+        x, w, more = x.to(BF), w.to(BF), {}
+        xv, wv = x.double(), w.double()
+        pad = lambda t: torch.nn.functional.pad(t, (0, -K % 16))[..., :K]  # noqa: E731
+    want, slack, end = grouped64(xv, wv, counts)
+    for a, b in ((x, w), (pad(x), pad(w))):
+        y = trk.matmul_grouped(a, b, c, out_dtype=F32, **more)
+        near(y, want, F32, slack * (K + 8) * U)
+        out = torch.full((rows, N), 3.0, device=gpu)
+        trk.matmul_grouped(a, b, c, out=out, **more)
+        assert torch.equal(out[:end], y[:end]) and (out[end:] == 3).all()
