@@ -1284,12 +1284,16 @@ int launch_tiles(const char* what, const MmArgs& A, int dt, bool aligned, float*
     case 2: return launch_few<IN, WROW, 2>(what, A, dt, st);
     case 4: return launch_few<IN, WROW, 4>(what, A, dt, st);
   }
-  // 256-tiles where whole ones alone fill the CUs (2048 x 8192 x 1024 in 8 bits 23.2 us against 25.8 with 128-tiles;
-  // 1024 x 8192 x 1024 20.2 against 15.2; 64 groups of 8 rows x 2048 x 2048 70 against 48).  f32 outputs
-  // have wider fragments, and unaligned 8-bit rows are held in registers on their way: both leave room
-  // for 128-tiles only.
+  // 256-tiles where whole ones alone fill the CUs, of even groups (a tile has rows of one): 2048 x 8192 x 1024 in 8 bits
+  // 23.2 us against 25.8 with 128-tiles, 1024 x 8192 x 1024 20.2 against 15.2.  64 groups x 2048 x 1024 in 8 / 16
+  // bits, 256 against 128: of 128 rows each 46 / 80 against 39 / 67, of 256 50 / 92 against 55 / 104, of 1024 189 / 303
+  // against 251 / 352; 256 groups of 32 rows 168 / 291 against 136 / 218.  What counts is not known here where
+  // groups are ragged: 256 rows on average 78 / 133 against 68 / 120, 1024 222 / 333 against 263 / 370.  f32
+  // outputs have wider fragments, and unaligned 8-bit rows are held in registers on their way: both leave
+  // room for 128-tiles only.
   if constexpr (IN != IN_E4M3X) {
-    if ((A.N + 255) / 256 * (A.M / 256) >= dev.cus) {
+    const int64_t groups = std::min(A.G, A.M);
+    if ((A.N + 255) / 256 * (groups * (A.M / groups / 256)) >= dev.cus) {
       if (aligned) return launch_tile<IN, WROW, true, 256, 2, 4>(what, A, dt, dev, st);
       if constexpr (!is8(IN)) return launch_tile<IN, WROW, false, 256, 2, 4>(what, A, dt, dev, st);
     }
