@@ -430,8 +430,11 @@ __device__ __forceinline__ int64_t xcd_run(int64_t id, int64_t n) {
 }
 
 // The product.  Bound by the matrix cores at the clock the chip holds under them: 8192 x 8192 x 8192 in 8 bits
-// 457 us (2.4 PFLOP/s; the library's product with one scale for all runs at 2.7, 408 us), matrix instructions busy
-// 59 % of the cycles at 1.8 GHz; in 16 bits 850 us (1.3 PFLOP/s, the library 813).  What brought the 8-bit
+// 465 us (455-480 over 100 traced launches; 2.4 PFLOP/s; the library's product with one scale for all runs at 2.7,
+// 408 us), matrix instructions busy 59 % of the cycles at 1.9 GHz; in 16 bits 835 us (1.3 PFLOP/s, the library
+// 813); in 8 bits to f32, with 128-tiles at half the rate, 950.  Few steps a tile leave more to the first copies and
+// stores: 64 ragged groups, 65536 x 2048 x 1024 in 8 bits 232 us, matrix instructions busy 29 %; 16 of 16384 x
+// 2048 x 2048 in 16 bits 179 us, 35 %.  What brought the 8-bit
 // one there, us: 128-tiles through registers 2064, 256-tiles with straight copies a step ahead 547, copies
 // spread over the step 484, several tiles a workgroup 478, rows of tiles kept in order 424-457.  Tried and
 // dropped: 128 x 256 and 256 x 128 tiles with two or three stages (562-650 us; more bytes to LDS for each
@@ -738,8 +741,8 @@ __global__ __launch_bounds__(256) void mm_join_kernel(MmArgs A, const float* par
 
 // ------------------------------------------------------------------ few rows
 // 16 JT rows by 16 columns a wave, the operands straight from memory to registers: with few rows the
-// weights are read once and that is what counts (16 x 4096 x 4096 in 8 bits 7.1 us, 2.4 TB/s: one round of latencies;
-// 16 x 8192 x 8192 20 us, 3.4 TB/s; 80 rows of 64 groups x 1024 x 1024 in 16 bits 22 us, 6 TB/s).
+// weights are read once and that is what counts (16 x 4096 x 4096 in 8 bits 7.2 us, 2.4 TB/s: one round of latencies;
+// 16 x 8192 x 8192 20 us, 3.4 TB/s).
 // KW waves of the 8 share 16 columns, each with every KW-th step, and are joined in order through
 // LDS; the others take the next columns.  U steps are loaded before they are multiplied.  Any
 // alignment.
@@ -905,9 +908,10 @@ __device__ __forceinline__ Frag<IN> frag_turned(const uint8_t* tile, uint32_t at
   return f;
 }
 
-// The gradients: 16 groups of 16384 rows in all, 2048 x 2048: both in 328 us (840 TFLOP/s; 2000 us through
-// registers with scalar turns, 390 in two launches).  The last round of tiles and each tile's first copies and
-// stores cost what is missing to the product's rate.
+// The gradients: 16 groups of 16384 rows in all, 2048 x 2048: both in 320 us (314-324 over 100 traced launches;
+// 860 TFLOP/s, matrix instructions busy 40 % of the cycles; 2000 us through registers with scalar turns, 390 in two
+// launches).  The last round of tiles and each tile's first copies and stores cost what is missing to the
+// product's rate.
 //
 // T x T tile `block` of dx (DW false: rows m of one group, columns k, contracted over n) or of dw[g] (rows n,
 // columns k, contracted over the group's rows), 8 waves, copies one step of 64 ahead.
@@ -1225,7 +1229,7 @@ int few_strips(int64_t G, int64_t M, int64_t N) {
 // 1000 x 2048 28 / 22 in 16 bits, in 8 (16 steps) 18 against 22 in 4 parts; 16 x 20000 x 8192 128 / 85 and 52 / 38, 8
 // groups, 16 x 2304 x 8192 122 / 78 and 54 / 40.  Rows that strips of 16 take stay whole
 // (8 groups, 64 x 2048 x 8192 52 against 56 in 3 parts), and up to 64 steps 256 strips of 64 (64 x 4096 x 4096 24 /
-// 19 in 16 bits, 17 / 18 in 8).  The join costs about 8 us.
+// 19 in 16 bits, 17 / 18 in 8).  The join takes 4 to 6 us of it, and a launch.
 int64_t parts_of(int64_t G, int64_t M, int64_t N, int64_t steps) {
   if (G < 1 || M < 1 || N < 1 || steps <= 24) return 1;
   const int64_t groups = std::min(G, M), tiles = groups * (((M + groups - 1) / groups + 127) / 128) * ((N + 127) / 128);
@@ -1237,8 +1241,10 @@ int64_t parts_of(int64_t G, int64_t M, int64_t N, int64_t steps) {
 template <int IN, bool WROW, int JT>
 int launch_few(const char* what, const MmArgs& A, int dt, hipStream_t st) {
   const int64_t strips = (A.N + 15) / 16, live = live_tiles(A.G, A.M, 16 * JT), steps = (A.K * (is8(IN) ? 1 : 2) + kStep - 1) / kStep;
-  // waves that share 16 columns: enough for 2048 waves in all, no more than there are steps (16 x 4096 x
-  // 4096 in 8 bits: 7.0 us with 8, 10.5 with 4; 64 groups of 1 row x 1024 x 1024: 15.2 with 1, 23.5 with 4)
+  // Waves that share 16 columns: enough for 2048 waves in all, and no more than there are steps (one step: 1).  Few
+  // strips come here (1024 at most), so the first rule ends at 2.  16 rows, us with 2 / 4 / 8: 4096 x 4096 in 8 bits
+  // 17.8 / 10.8 / 7.0, in 16 32.4 / 18.9 / 12.2; 8192 x 4096 18.8 / 11.2 / 10.9, 32.6 / 19.5 / 21.7; 16384 x 4096
+  // 19.4 / 18.4 / 19.0, 32.9 / 35.8 / 39.1
   int kw = 8;
   while (kw > 1 && (strips * live * (kw / 2) >= 2048 || kw > steps)) kw /= 2;
   const dim3 grid((unsigned)((strips + 8 / kw - 1) / (8 / kw)), (unsigned)row_tiles(A, 16 * JT));

@@ -8,9 +8,12 @@
 //
 // All of them are bound by memory (4-14 operations a value).  A row lives in the registers of
 // the T lanes that own it between its one read and its one write; every statistic is f32.
-// At 204800 x 512 bf16 with the residual the norm takes 140 us (6.0 TB/s, a large copy 5.3), its 8-bit form
-// without it 91 (3.5); the gradient of 100352 x 512 with its forward 101 us (5.1); 204800 x 1024
-// quantised 127 us (5.0).  256 x 512 to 8 bits takes 3.7 us, a launch more than that.
+// At 204800 x 512 bf16 with the residual the norm takes 142 us (5.9 TB/s, a large copy 5.3), in f32 162
+// without it (5.2) and 339 with it (5.0); its 8-bit form 135 with it (5.4), 96 without (3.3: a row's loads, its sums
+// and its stores follow one another, and what is in flight no longer covers them).  Gradients of 100352 x 512 with
+// their forward: bf16 41 + 58 + 4 us (5.0 TB/s), f32 73 + 125 + 5 (5.1).  204800 x 1024 quantised 133 us (4.8); 128 x
+// 128 blocks of 5003 x 1111 f32 12.6 us (2.2: each workgroup loads one block, joins and stores it), of 4096 x 4096
+// bf16 11.5 (4.4).  256 x 512 to 8 bits takes 3.7 us, a launch more than that.
 // The gradient is taken at the stored h (rounded to x's type) with the r of the unrounded sum.
 #include <type_traits>
 
