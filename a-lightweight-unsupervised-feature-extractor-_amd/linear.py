@@ -193,16 +193,17 @@ class _Tied(torch.autograd.Function):
 
 
 def _backward_once(what):
-    """For a backward pass without a derivative.  Where a graph of it is asked for, its gradients are hung on what came in and
+    """For a backward pass (ctx, saved tensors, gradients) without a derivative.  Where a graph of it is asked for, its gradients are hung on what came in and
     on every saved input: a second derivative is then an error for each of them.  (torch's own mark looks at
     what came in only: after a sum, whose gradient is a constant, the second derivative would silently be zero.)"""
     def mark(backward):
         def call(ctx, *grads):
+            saved = ctx.saved_tensors  # once: a checkpoint computes them again for each reading
             if not torch.is_grad_enabled():
-                return backward(ctx, *grads)
+                return backward(ctx, saved, *grads)
             with torch.no_grad():
-                out = backward(ctx, *grads)
-            of = [t for t in (*grads, *ctx.saved_tensors, *ctx.links) if t is not None and t.requires_grad]
+                out = backward(ctx, saved, *grads)
+            of = [t for t in (*grads, *saved, *ctx.links) if t is not None and t.requires_grad]
             given = [t for t in out if t is not None]
             if not of or not given:
                 return out
@@ -225,8 +226,8 @@ class _RmsNorm(torch.autograd.Function):
 
     @staticmethod
     @_backward_once("rms_norm")
-    def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
+    def backward(ctx, saved, dy, dh=None):
+        h, weight, rstd = saved
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:  # only the sum was used
             return dh if need_x else None, None, dh if need_r else None, None, None
@@ -505,8 +506,8 @@ class _Grouped(torch.autograd.Function):
 
     @staticmethod
     @_backward_once("matmul_grouped")
-    def backward(ctx, dy):
-        x, w, counts = ctx.saved_tensors
+    def backward(ctx, saved, dy):
+        x, w, counts = saved
         M, G, N, K = ctx.sizes
         read = w if x is None else x
         if dy.dtype != read.dtype:

@@ -1318,3 +1318,26 @@ def test_matmul_grouped_long_odd_rows(trk, gpu, kind):
         out = torch.full((rows, N), 3.0, device=gpu)
         trk.matmul_grouped(a, b, c, out=out, **more)
         assert torch.equal(out[:end], y[:end]) and (out[end:] == 3).all()
+
+
+@gpu_test
+def test_checkpointed(trk, gpu):
+    """recomputed forward passes, with a graph of the gradients too, and saved tensors kept on the host"""
+    from torch.utils.checkpoint import checkpoint
+    g = gen_of(gpu, 74)
+    x = torch.randn(60, 128, device=gpu, generator=g).to(BF).requires_grad_()
+    v = torch.randn(128, device=gpu, generator=g).to(BF).requires_grad_()
+    w = torch.randn(3, 64, 128, device=gpu, generator=g).to(BF).requires_grad_()
+    c = torch.tensor([20, 0, 40], device=gpu, dtype=torch.int32)
+
+    def f(x, v, w):
+        y, h = trk.rms_norm(x, v, residual=x)
+        return trk.matmul_grouped(y, w, c).float().sum() + h.float().square().sum()
+
+    want = torch.autograd.grad(f(x, v, w), (x, v, w))
+    for graph in (False, True):
+        got = torch.autograd.grad(checkpoint(f, x, v, w, use_reentrant=False), (x, v, w), create_graph=graph)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    with torch.autograd.graph.save_on_cpu():
+        y = f(x, v, w)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, v, w)), want))
