@@ -1341,3 +1341,187 @@ def test_checkpointed(trk, gpu):
     with torch.autograd.graph.save_on_cpu():
         y = f(x, v, w)
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, v, w)), want))
+
+
+# --------------------------------------------------------------------- what lies beside, behind and around
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("M,N,K", [(20, 48, 300), (200, 300, 640), (1000, 900, 272), (4096, 4096, 256), (600, 928, 6288), (900, 1000, 131)])
+def test_special_codes_stay_in_their_rows(trk, gpu, M, N, K, dtype):
+    g = gen_of(gpu, 70, M)
+    x, sx = codes_of(g, M, K, 1, gpu)
+    w, sw = codes_of(g, N, K, 1, gpu)
+    clean = trk.matmul_fp8(x, sx, w, sw, out_dtype=dtype)
+    x[M // 2, K - 1] = float("nan")
+    w[N - 2, 0] = float("nan")
+    sx[1, 0] = float("inf")
+    y = trk.matmul_fp8(x, sx, w, sw, out_dtype=dtype)
+    assert y[M // 2].isnan().all() and y[:, N - 2].isnan().all() and not y[1].isfinite().any()
+    r = [i for i in range(M) if i not in (M // 2, 1)]
+    c = [i for i in range(N) if i != N - 2]
+    assert torch.equal(y[r][:, c], clean[r][:, c])
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("counts,rows,N,K", [([3, 0, 4], 9, 40, 70), ([200, 1, 130], 400, 200, 130), ([700, 0, 513, 1200], 2500, 300, 200),
+                                             ([2000, 2048, 3500], 7700, 2304, 104), ([9000], 9100, 64, 64), ([140, 300], 520, 700, 5000)])
+def test_special_values_stay_in_their_group(trk, gpu, counts, rows, N, K, dtype):
+    """NaN rows behind the last group and in one group, NaN in the padding behind rows: nothing else sees them"""
+    g = gen_of(gpu, 71, rows)
+    c = torch.tensor(counts, device=gpu, dtype=torch.int32)
+    G, end = len(counts), sum(counts)
+    for pad in (0, 8 + -K % 8, 3):
+        bx = torch.full((rows, K + pad), float("nan"), device=gpu, dtype=dtype)
+        bw = torch.full((G, N, K + pad), float("nan"), device=gpu, dtype=dtype)
+        bd = torch.full((rows, N + pad), float("nan"), device=gpu, dtype=dtype)
+        x, w, dy = bx[:, :K], bw[..., :K], bd[:, :N]
+        x.copy_(torch.randn(rows, K, device=gpu, generator=g))
+        w.copy_(torch.randn(G, N, K, device=gpu, generator=g))
+        dy.copy_(torch.randn(rows, N, device=gpu, generator=g))
+
+        def run():
+            a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+            y = trk.matmul_grouped(a, b, c)
+            return (y.detach(),) + torch.autograd.grad(y, (a, b), dy)
+
+        y, dx, dw = run()
+        assert all(t.isfinite().all() for t in (y, dx, dw))
+        x[end:], dy[end:] = float("nan"), float("inf")
+        y2, dx2, dw2 = run()
+        assert torch.equal(y2, y) and torch.equal(dx2, dx) and torch.equal(dw2, dw)
+        x[0, K // 2], dy[counts[0] - 1, 0] = float("nan"), float("-inf")
+        y3, dx3, dw3 = run()
+        assert y3[0].isnan().all() and not dx3[counts[0] - 1].isfinite().any()
+        assert torch.equal(y3[1:], y[1:])
+        r = [i for i in range(rows) if i != counts[0] - 1]
+        assert torch.equal(dx3[r], dx[r]) and torch.equal(dw3[1:], dw[1:])
+        assert not dw3[0, 0].isfinite().any() and dw3[0, :, K // 2].isnan().all()
+        k = [i for i in range(K) if i != K // 2]
+        assert torch.equal(dw3[0, 1:][:, k], dw[0, 1:][:, k])
+
+
+@gpu_test
+def test_rows_far_apart(trk, gpu):
+    """row strides just below 16 MiB: offsets inside a tile use all 32 bits; 16 MiB is refused"""
+    g = gen_of(gpu, 72)
+    ld, K, N = (1 << 24) - 16, 272, 200
+    pool = torch.empty(257 * ld, device=gpu, dtype=torch.uint8)
+    for M in (256, 20):
+        x, sx = codes_of(g, M, K, 1, gpu)
+        w, sw = codes_of(g, N, K, 1, gpu)
+        far = torch.as_strided(pool.view(FP8), (M, K), (ld, 1))
+        far.copy_(x)
+        for dtype in (BF, F32):
+            assert torch.equal(trk.matmul_fp8(far, sx, w, sw, out_dtype=dtype), trk.matmul_fp8(x, sx, w, sw, out_dtype=dtype))
+            assert torch.equal(trk.matmul_fp8(w, sw, far, sx, out_dtype=dtype), trk.matmul_fp8(w, sw, x, sx, out_dtype=dtype))
+        if M == 256:  # (256-tiles)
+            many, sm = codes_of(g, 66000, K, 1, gpu)
+            assert torch.equal(trk.matmul_fp8(far, sx, many, sm), trk.matmul_fp8(x, sx, many, sm))
+        far = torch.as_strided(pool.view(BF), (M, K), (ld // 2, 1))
+        a, b = (torch.randn(*s, K, device=gpu, generator=g).to(BF) for s in ((M,), (2, N)))
+        far.copy_(a)
+        dy = torch.randn(M, N, device=gpu, generator=g).to(BF)
+        c = torch.tensor([M - 7, 7], device=gpu, dtype=torch.int32)
+        got = []
+        for v in (a, far):
+            p, q = v.detach().requires_grad_(), b.detach().requires_grad_()
+            y = trk.matmul_grouped(p, q, c)
+            got.append((y,) + torch.autograd.grad(y, (p, q), dy))
+        assert all(torch.equal(p, q) for p, q in zip(*got))
+    over = torch.as_strided(pool.view(FP8), (16, K), (1 << 24, 1))
+    with pytest.raises(NotImplementedError, match="16 MiB"):
+        trk.matmul_fp8(over, sx[:16], w, sw)
+    # the norm and the quantisation have no such limit
+    far = torch.as_strided(pool.view(BF), (200, K), (ld // 2 + 24, 1))
+    far.copy_(torch.randn(200, K, device=gpu, generator=g))
+    assert torch.equal(trk.rms_norm(far), trk.rms_norm(far.contiguous()))
+    assert torch.equal(trk.quantize_fp8(far)[0].float(), trk.quantize_fp8(far.contiguous())[0].float())
+
+
+@gpu_test
+@pytest.mark.parametrize("dtype", [BF, F16, F32])
+@pytest.mark.parametrize("D", [1, 7, 9, 100, 129, 500, 513, 1111, 2047, 5001, 8193, 20001])
+def test_nothing_is_written_beside_rows(trk, gpu, D, dtype):
+    """rows of every output inside wider ones, through the C interface: what lies around them stays"""
+    g = gen_of(gpu, 73, D)
+    R, L = 6, trk.lib()
+    dt = {F32: 0, BF: 1, F16: 3}[dtype]
+    st = torch.cuda.current_stream().cuda_stream
+    x, r, dy = (torch.randn(R, D, device=gpu, generator=g).to(dtype) for _ in range(3))
+
+    def room(extra, t=dtype, at=3):
+        b = torch.full((R + 2, D + extra), 9.0, device=gpu, dtype=t)
+        return b, b[1:-1, at:at + D]
+
+    def around(b, v):
+        c = b.clone()
+        torch.as_strided(c, v.shape, v.stride(), v.storage_offset()).fill_(9.0)
+        return bool((c == 9).all())
+
+    (by, y), (bh, h), (bd, dx) = (room(8) for _ in range(3))
+    rstd = torch.empty(R, device=gpu)
+    assert L.trk_rms_norm(x.data_ptr(), D, r.data_ptr(), D, None, 1e-6, R, D, dt, y.data_ptr(), D + 8, h.data_ptr(), D + 8, rstd.data_ptr(), st) == 0
+    wy, wh = trk.rms_norm(x, residual=r)
+    assert torch.equal(y, wy) and torch.equal(h, wh) and around(by, y) and around(bh, h)
+    assert L.trk_rms_norm_bwd(h.data_ptr(), D + 8, None, rstd.data_ptr(), dy.data_ptr(), D, None, 0, R, D, dt, dx.data_ptr(), D + 8, None, 1, None, st) == 0
+    assert around(bd, dx) and dx.isfinite().all()
+    # codes: no room for the padding (rows next to each other), or room and more
+    for ld in (D, -(-D // 16) * 16, -(-D // 16) * 16 + 32):
+        q = torch.full((R + 2, ld), 0x55, device=gpu, dtype=torch.uint8)
+        s = torch.full((-(-D // 128), R + 3), 9.0, device=gpu)
+        for fn in ("norm", "quant"):
+            q.fill_(0x55)
+            s.fill_(9.0)
+            if fn == "norm":
+                rc = L.trk_rms_norm_fp8(x.data_ptr(), D, None, 0, None, 1e-6, R, D, dt, q[1].data_ptr(), ld, s.data_ptr(), R + 3, None, 0, st)
+                wq, ws = trk.rms_norm_fp8(x)
+            else:
+                rc = L.trk_quantize_fp8(x.data_ptr(), D, 0, 1, R, D, 1, dt, q[1].data_ptr(), ld, 0, s.data_ptr(), R + 3, 0, st)
+                wq, ws = trk.quantize_fp8(x)
+            assert rc == 0
+            pad = -(-D // 16) * 16
+            assert torch.equal(q[1:-1, :D], wq.view(torch.uint8)) and torch.equal(s[:, :R].t(), ws)
+            assert (q[0] == 0x55).all() and (q[-1] == 0x55).all() and (s[:, R:] == 9).all()
+            if ld > pad:
+                assert (q[1:-1, pad:] == 0x55).all()
+            if ld >= pad:
+                assert (q[1:-1, D:pad] == 0).all()
+
+
+@gpu_test
+def test_functional_transforms_are_errors(trk, gpu):
+    x = torch.randn(5, 32, device=gpu)
+    a, c = x.to(BF), torch.tensor([5], device=gpu, dtype=torch.int32)
+    w = torch.randn(1, 8, 32, device=gpu).to(BF)
+    for f, arg in ((lambda t: trk.rms_norm(t), x), (lambda t: trk.matmul_grouped(t, w, c), a), (lambda t: trk.quantize_fp8(t)[1], x)):
+        for call in (lambda: torch.func.grad(lambda t: f(t).sum().float())(arg), lambda: torch.func.jvp(f, (arg,), (arg,)),
+                     lambda: torch.func.vmap(f)(arg[None].repeat(3, 1, 1)), lambda: torch.func.vjp(f, arg), lambda: torch.func.linearize(f, arg)):
+            with pytest.raises(RuntimeError):  # (NotImplementedError is one)
+                call()
+
+
+@gpu_test
+def test_two_threads(trk, gpu):
+    """two host threads, each on its own stream"""
+    import threading
+    a, b = (_chain_inputs(trk, gpu, k) for k in (5, 6))
+    want = [[t.clone() for t in _chain(trk, *v)] for v in (a, b)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(v, w):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(30):
+                got = _chain(trk, *v)
+                s.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, w)):
+                    bad.append(1)
+
+    ts = [threading.Thread(target=work, args=t) for t in zip((a, b), want)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad
