@@ -319,10 +319,10 @@ enum { IN_E4M3 = 0, IN_BF16 = 1, IN_F16 = 2, IN_E4M3X = 3 };
 constexpr bool is8(int in) { return in == IN_E4M3 || in == IN_E4M3X; }
 
 // A lane's 32 bytes of a row's K step, as the matrix instruction takes them.  IN_E4M3 is the 8-bit
-// instruction: in each 8 bytes it cuts every product, towards zero, to a multiple of 2^-13 of the largest
-// one's power of two (measured: 256 * 256 - 256 * 256 + s * 1 leaves the multiple of 8 below s in the same 8
-// columns, s in any others; 1.5e-5 of an ordinary sum in the root mean square).  That is far below half a step of a
-// 16-bit y unless products cancel, so 16-bit outputs use it, and the interface says so.  IN_E4M3X,
+// instruction: in each 8 bytes it cuts every product, towards zero, by less than 2^-13 of the largest one (to multiples
+// of 2^-13 of the power of two that the largest one's exponents add up to; measured: 256 * 256 - 256 * 256 + s * 1
+// leaves the multiple of 8 below s in the same 8 columns, s in any others; 1.5e-5 of an ordinary sum in the root
+// mean square).  That is far below half a step of a 16-bit y unless products cancel, so 16-bit outputs use it, and the interface says so.  IN_E4M3X,
 // for f32 outputs, widens the codes to bf16 (exact) and multiplies at half the rate with f32 sums.
 template <int IN> struct Frag {
   uint4 v[2];

@@ -368,11 +368,11 @@ def matmul_fp8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale:
     """y [M, N] = x [M, K] @ w [N, K]^T (+ bias [N] f32) of float8_e4m3fn codes with their scales: x_scale
     [M, ceil(K / 128)]; w_scale [N, ceil(K / 128)] (block_rows 1) or [ceil(N / 128), ceil(K / 128)] (128).
 
-    Each block's sum is scaled by the product of its two scales (which has to stay in f32's normal range) and
-    added in f32, and y is rounded once to out_dtype (bfloat16 by default; float16, float32).  For float32 the
-    products of a block are summed in f32.  For the 16-bit types the 8-bit matrix instruction sums them: in each 8
-    columns (8 i .. 8 i + 7) it cuts every product, towards zero, to a multiple of 2^-13 of the largest one's power of
-    two.  That is 1.5e-5 of an ordinary sum, far below a rounding of y; but where large products cancel, small
+    Each block's sum is scaled by the product of its two scales, taken in f32 (beyond f32's range an infinity, NaN
+    with a sum of zero), and added in f32, and y is rounded once to out_dtype (bfloat16 by default; float16, float32).
+    For float32 the products of a block are summed in f32.  For the 16-bit types the 8-bit matrix instruction sums
+    them: in each 8 columns (8 i .. 8 i + 7) it cuts every product, towards zero, by less than 2^-13 of the largest
+    one.  That is 1.5e-5 of an ordinary sum, far below a rounding of y; but where large products cancel, small
     ones beside them are lost, and float32 is the type to ask for.
 
     out: written in place of a new tensor (it must not overlap an input)."""

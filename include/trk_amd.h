@@ -339,11 +339,12 @@ int trk_quantize_fp8(const void* x, int64_t ldx, int64_t xb, int64_t B, int64_t 
 /* trk_matmul_fp8: y [M][N] = x [M][K] . w [N][K]^T + bias (f32 [N], NULL: 0) of e4m3 codes:
  *   sum over the blocks kb of 128 columns of sx[m * sx_row + kb * sx_kb] *
  *   sw[(n / w_block_rows) * sw_row + kb * sw_kb] * (the block's products); w_block_rows 1 or
- *   128; out_dtype TRK_F32 / BF16 / F16.  A product of two scales has to stay in f32's normal
- *   range.  TRK_F32: sums in f32.  BF16 / F16: a block's products are summed by the 8-bit matrix
- *   instruction, which cuts each of them, in every 8 columns (8 i .. 8 i + 7), towards zero to a
- *   multiple of 2^-13 of the largest one's power of two (1.5e-5 of an ordinary sum; small products
- *   beside large ones that cancel are lost); blocks are added in f32.  parts >= 1 (at most ceil(K / 128)): K is summed in so
+ *   128; out_dtype TRK_F32 / BF16 / F16.  The two scales are multiplied first, in f32 (beyond its
+ *   range an infinity, NaN with a sum of zero).  TRK_F32: sums in f32.  BF16 / F16: a block's
+ *   products are summed by the 8-bit matrix instruction, which cuts each of them, in every 8
+ *   columns (8 i .. 8 i + 7), towards zero by less than 2^-13 of the largest one (1.5e-5 of an
+ *   ordinary sum; small products beside large ones that cancel are lost); blocks are added in
+ *   f32.  parts >= 1 (at most ceil(K / 128)): K is summed in so
  *   many parts, joined in order, in the f32 workspace part [parts][M][N] (not read with 1);
  *   trk_matmul_fp8_parts suggests a number.
  * trk_matmul_grouped: the rows of x sorted by group, counts[g] (device, int32) of them for
