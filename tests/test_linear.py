@@ -976,7 +976,8 @@ def test_long_offsets(trk, gpu):
 @pytest.mark.parametrize("M,N,K", [(5, 40, 128), (16, 200, 1024), (200, 300, 640), (640, 1280, 256), (600, 928, 6288), (4096, 4096, 128)])
 def test_matmul_fp8_cancelling_products(trk, gpu, M, N, K):
     """Where large products cancel, f32 outputs keep what is left.  16-bit ones are within what their contract says: each
-    product cut by less than 2^-13 of the largest of its 8 columns' products; columns without a large product lose no more than a sum in f32 does."""
+    product cut by less than 2^-13 of the largest of its 8 columns' products; columns without a large product lose no
+    more than a sum in f32 does."""
     g = gen_of(gpu, 55, M, N, K)
     kb = -(-K // 128)
     sx, sw = torch.ones(M, kb, device=gpu), torch.full((N, kb), 2.0 ** -6, device=gpu)
